@@ -24,6 +24,10 @@
  *   nq_quantize          <- mx::quantize(w, gs, bits) (MLX affine; the
  *                           reference loads pre-quantized checkpoints and has
  *                           no call site of its own)
+ *   nq_paged_*, nq_pages_*  the key/value cache in pages: attention of new
+ *                           tokens over it, the append, and the page pool (no
+ *                           counterpart: the reference's caches grow by
+ *                           concatenation, llama_model.cpp:462-463)
  *   nq_bits_from_shapes  <- mlx_ops::bits  compute/src/compute/model/mlx_ops.h:20-25
  *
  * Conventions
@@ -73,9 +77,10 @@ int nq_version(void);
 const char *nq_last_error(void);
 /* Number of CUDA devices usable by the library (0 when none); never fails. */
 int nq_device_count(void);
-/* Reads and clears the device-side error word of the current device (set by a
- * kernel whose bounded wait ran out, or by an out-of-range gather index).
- * 0 = no error. */
+/* Reads and clears the device-side error word of the current device: bit 0, a
+ * kernel's bounded wait ran out; bit 1, an index that a kernel read was out of
+ * range (gather index, token, table row, length, page); bit 2, a page request
+ * was refused (nq_pages_*).  0 = no error. */
 int nq_take_device_error(unsigned int *err_out);
 
 /* mlx_ops::bits: round(32 * (w_cols / s_cols) / group_size), 4 if not positive. */
@@ -321,6 +326,126 @@ int nq_llama_prefill(nq_llama_t dec, const int32_t *tokens, int64_t n,
  * when token != NULL); tokens[i] (device int32 [n]) receives step i's argmax. */
 int nq_llama_generate(nq_llama_t dec, const int32_t *token, int64_t n,
                       int32_t *tokens, void *stream);
+
+/* ---- Paged key/value cache ----
+ * One layer's keys (and values): [n_pages][n_kv_heads][page_size][head_dim],
+ * pages page_stride elements apart.  A contiguous cache is one page per
+ * sequence.  head_dim 64, 128 or 256; page_size a multiple of 16; dtype
+ * NQ_DTYPE_BF16 or NQ_DTYPE_F16; 16-byte aligned, page_stride a multiple of 8.
+ *
+ * The page table (device int32 [n_rows][table_ld], table_width entries used)
+ * lists each sequence's pages, kv_lens [n_rows] the sequences' lengths with
+ * the new tokens included.  A batch names its sequences by table row: entry b
+ * is row seqs[b] (a negative one is padding), or row b when seqs is NULL.  The
+ * new tokens of entry b are rows q_starts[b] .. q_starts[b + 1] of q, k, v and
+ * out (device int32 [n_seqs + 1]), or row b alone when q_starts is NULL; token
+ * t of n stands at position kv_lens - n + t.  Rows behind the last entry, and
+ * those of padding, are neither read nor written.
+ *
+ * The arrays are read when the kernels run; what they say out of range (a
+ * length past the table, a table row, a missing page) is cut off or read as
+ * zeros and raises bit 1 of the device error word. */
+typedef struct nq_paged_cache {
+    void *k, *v;
+    int64_t n_pages, page_stride;
+    int n_kv_heads, page_size, head_dim, dtype;
+} nq_paged_cache_t;
+
+typedef struct nq_paged_batch {
+    const int32_t *table;
+    int64_t table_ld, table_width, n_rows;
+    const int32_t *kv_lens;
+    const int32_t *seqs;
+    const int32_t *q_starts;
+    int64_t n_seqs, n_tokens;
+} nq_paged_batch_t;
+
+/* Attention of the batch's new tokens over the cache (the keys of the new
+ * tokens have been appended):
+ *   out[t, h] = sum_j p_j v[j, h / G] / sum_j p_j,
+ *   p_j = exp(scale * q[t, h] . k[j, h / G]),  G = n_heads / n_kv_heads,
+ * over the keys j <= pos(t), and j > pos(t) - window when window > 0.  A row
+ * without any key (more new tokens than the length) is zero.  q and out rows:
+ * [n_heads][head_dim], q_ld / out_ld elements apart (multiples of 8, 16-byte
+ * aligned).  Keys and values past a sequence's length, and pages that no new
+ * token's window reaches, may hold anything; the values that the rows of one
+ * call see have to be finite.  max_q: no entry has more new tokens than this (it
+ * selects the kernel and the workspace's size, results hold for any; 0:
+ * unknown).  Softmax and sums in fp32; the weights are rounded to the cache's type
+ * for the second product, the result once.  workspace: nq_paged_attention_
+ * workspace_size() bytes for this max_q, 256-byte aligned, contents
+ * irrelevant; two calls that overlap on the GPU need one each. */
+size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q);
+int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_paged_cache_t *cache,
+                       const nq_paged_batch_t *batch, int64_t max_q, float scale, int64_t window,
+                       void *workspace, size_t workspace_bytes, uint16_t *out, int64_t out_ld,
+                       void *stream);
+
+/* Rotary positions for the new tokens' queries and keys, and their keys and
+ * values into the cache.  For i < n_freqs the pair (x_i, x_{i + n_freqs}) of
+ * each head of q and k is turned by pos * freqs[i] (device fp32, radians per
+ * position; MLX fast::rope, traditional = false, compute/src/compute/model/
+ * llama_model.cpp:446-470), the angle in 64 bits, the turn in fp32, rounded
+ * once; dims past 2 * n_freqs stay.  n_freqs is a multiple of 8, at most
+ * head_dim / 2; 0 turns nothing.  The queries go to q_out (may be q itself).
+ * A token at a negative position or whose page is missing is not stored (error
+ * word). */
+int nq_paged_append(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t k_ld,
+                    const uint16_t *v, int64_t v_ld, int n_heads, const nq_paged_cache_t *cache,
+                    const nq_paged_batch_t *batch, const float *freqs, int n_freqs, uint16_t *q_out,
+                    int64_t q_out_ld, void *stream);
+
+/* The page pool's bookkeeping, all of it in device memory, so that the calls
+ * below only enqueue work (and may be captured): refs[p] sequences hold page
+ * p (0: free), table and lens as above, -1 in unused table entries.  A pool is
+ * [outer][n_pages][page_bytes] (outer: layers x keys and values).  Sequence
+ * lists are device int32; negative entries are padding.  A refused request
+ * raises bit 2 of the device error word. */
+typedef struct nq_page_table {
+    int32_t *refs;
+    int32_t *table;
+    int32_t *lens;
+    int64_t n_pages, n_rows, table_ld, table_width;
+    int page_size;
+} nq_page_table_t;
+
+typedef struct nq_page_pool {
+    void *data;
+    int64_t outer, n_pages, page_bytes;
+} nq_page_pool_t;
+
+/* The listed sequences give their pages back and have length 0. */
+int nq_pages_free(const nq_page_table_t *table, const int32_t *seqs, int64_t n, void *stream);
+
+/* children[i] becomes a copy of parents[i] that shares all its pages.  A child
+ * that has pages, is listed twice or is also a parent of this call is refused
+ * (that pair alone). */
+int nq_pages_fork(const nq_page_table_t *table, const int32_t *parents, const int32_t *children,
+                  int64_t n, void *stream);
+
+/* Sequence seqs[i] grows to new_lens[i] tokens: a last page that is not full
+ * and has other holders is replaced by a copy, and free pages are added, the
+ * lowest first, in the list's order.  All or nothing: too few free pages, a
+ * length below the present one or past the table, a row out of range or a
+ * sequence listed twice refuse the whole call.  workspace:
+ * nq_pages_workspace_size(0, n) bytes, 256-byte aligned. */
+size_t nq_pages_workspace_size(int64_t n_pages, int64_t n);
+int nq_pages_reserve(const nq_page_table_t *table, const nq_page_pool_t *pool, const int32_t *seqs,
+                     const int32_t *new_lens, int64_t n, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
+/* The used pages past the number of used ones move into the free pages below
+ * it (the k-th lowest into the k-th lowest), contents, refs and table entries:
+ * the pool's upper end is free afterwards.  workspace:
+ * nq_pages_workspace_size(n_pages, 0) bytes, 256-byte aligned. */
+int nq_pages_compact(const nq_page_table_t *table, const nq_page_pool_t *pool, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* Copies pages src[i] to dst[i] in every outer slice; refs and tables are the
+ * caller's.  A move whose target is also a source or an earlier target is
+ * refused (that move alone). */
+int nq_pages_copy(const nq_page_pool_t *pool, const int32_t *src, const int32_t *dst, int64_t n,
+                  void *stream);
 
 /* nq_moe_switch without a workspace argument, for callers that cannot
  * allocate device memory themselves (an FFI host or a runtime that only

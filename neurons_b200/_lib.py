@@ -20,6 +20,7 @@ STATUS_NAMES = {
 
 # exported symbol -> (restype, argtypes); the full surface of include/nq.h
 P, I64, I, U64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+F32 = ctypes.c_float
 SIGNATURES = {
     "nq_version": (I, []),
     "nq_last_error": (ctypes.c_char_p, []),
@@ -46,6 +47,15 @@ SIGNATURES = {
                                   P, P, I, I, P, U64, P, P]),
     "nq_moe_switch_partial_push": (I, [P, I64, I64, I64, I64, I64, P, P, I64, I64, P, P, P, P, P, P,
                                        P, P, P, I, I, P, U64, P, P]),
+    "nq_paged_attention_workspace_size": (U64, [I, I, I, I64]),
+    "nq_paged_attention": (I, [P, I64, I, P, P, I64, F32, I64, P, U64, P, I64, P]),
+    "nq_paged_append": (I, [P, I64, P, I64, P, I64, I, P, P, P, I, P, I64, P]),
+    "nq_pages_free": (I, [P, P, I64, P]),
+    "nq_pages_fork": (I, [P, P, P, I64, P]),
+    "nq_pages_workspace_size": (U64, [I64, I64]),
+    "nq_pages_reserve": (I, [P, P, P, P, I64, P, U64, P]),
+    "nq_pages_compact": (I, [P, P, P, U64, P]),
+    "nq_pages_copy": (I, [P, P, P, I64, P]),
     "nq_llama_create": (I, [P, P, P, P, P, P]),
     "nq_llama_destroy": (I, [P]),
     "nq_llama_position": (I64, [P]),

@@ -24,9 +24,9 @@ ROOT = os.path.dirname(HERE)
 INCLUDE = os.path.join(ROOT, "include")
 
 CU_SOURCES = ["abi.cu", "quant.cu", "gemv.cu", "gemm_tc.cu", "gemm_tc_moe.cu", "moe.cu",
-              "moe_small.cu", "llama.cu"]
+              "moe_small.cu", "llama.cu", "paged.cu", "attn_paged.cu"]
 CPP_SOURCES = ["cuda_backend.cpp", "model_loader.cpp"]
-HEADERS = ["nq_common.cuh", "nq_internal.h", "cuda_backend.h", "iface/compute_types.h",
+HEADERS = ["nq_common.cuh", "nq_internal.h", "paged.cuh", "cuda_backend.h", "iface/compute_types.h",
            "iface/compute_backend.h", "model_loader.h"]
 # The reference's interface headers, restated, for building libnq on its own
 # (inside the reference tree its own core/ headers take their place).

@@ -14,6 +14,7 @@ namespace nq {
 enum DeviceError : unsigned int {
     kErrWaitTimeout = 1u,      // an mbarrier wait exceeded its time limit
     kErrBadIndex = 2u,         // a gather index was out of range
+    kErrPages = 4u,            // a page request was refused (too few free pages, bad lists)
 };
 
 // Upper bound on any spin-wait inside a kernel, in nanoseconds of %globaltimer.

@@ -1,0 +1,348 @@
+// paged.cuh -- the paged key/value cache as its kernels see it, and the split
+// of an attention call's work over the CTAs of a grid.
+//
+// A layer's cache is keys and values [n_pages][n_kv][page_size][head_dim]
+// (pages page_stride elements apart).  Row s of the page table lists the pages
+// of sequence s and lens[s] is its length, new tokens included.  The batch
+// names its sequences by table row; the new tokens of entry b are rows
+// q_starts[b] .. q_starts[b + 1] of q and stand at the sequence's end.
+#pragma once
+
+#include "nq_common.cuh"
+
+namespace nq {
+
+struct PagedBatch {
+    const int32_t *table;     // [n_rows][table_ld], table_width entries each; -1: no page
+    const int32_t *lens;      // [n_rows]
+    const int32_t *seqs;      // [n_seqs] table row of entry b (< 0: padding); nullptr: b
+    const int32_t *q_starts;  // [n_seqs + 1]; nullptr: entry b is row b of q
+    int64_t table_ld;
+    int table_width, n_rows, n_seqs, n_tokens;
+    int page_size, n_pages;
+    unsigned *err;
+};
+
+// One entry of the batch: table row, first row of q, new tokens, length.
+struct SeqView {
+    int row, q0, n, len;
+};
+
+// Reads entry b.  What the arrays say outside their ranges (a table row, a
+// length past the table's width, token rows past n_tokens) is cut to the range
+// and raises the error word; a padding entry has n == 0.
+__device__ __forceinline__ SeqView seq_view(const PagedBatch &pb, int b) {
+    SeqView s;
+    bool bad = false;
+    s.row = pb.seqs ? pb.seqs[b] : b;
+    if (pb.q_starts) {
+        s.q0 = pb.q_starts[b];
+        s.n = pb.q_starts[b + 1] - s.q0;
+    } else {
+        s.q0 = b;
+        s.n = 1;
+    }
+    if (s.q0 < 0 || s.q0 > pb.n_tokens || s.n < 0) {
+        bad = true;
+        s.q0 = 0;
+        s.n = 0;
+    } else if (s.n > pb.n_tokens - s.q0) {
+        bad = true;
+        s.n = pb.n_tokens - s.q0;
+    }
+    if (s.row < 0) {
+        s.n = 0;
+        s.len = 0;
+    } else if (s.row >= pb.n_rows) {
+        bad = true;
+        s.row = 0;
+        s.len = 0;
+    } else {
+        s.len = pb.lens[s.row];
+        const int64_t most = (int64_t)pb.table_width * pb.page_size;
+        if (s.len < 0 || s.len > most) {
+            bad = true;
+            s.len = s.len < 0 ? 0 : (int)most;
+        }
+    }
+    if (bad) atomicOr(pb.err, kErrBadIndex);
+    return s;
+}
+
+// Key blocks [lo, lo + nb) of `BK` keys that the new tokens [t0, t1) of a
+// sequence see (position of token t: len - n + t; keys up to it, and within
+// the window when there is one).  nb is at least 1, so that rows without any
+// key have a block, all of it masked, that writes their zeros.
+struct KeyRange {
+    int lo, nb;
+};
+
+template <int BK>
+__device__ __forceinline__ KeyRange key_range(const SeqView &s, int t0, int t1, int window) {
+    const int p0 = s.len - s.n + t0, p1 = s.len - s.n + t1 - 1;
+    KeyRange r;
+    const int hi = p1 < 0 ? 0 : p1 / BK + 1;
+    r.lo = window > 0 && p0 - window + 1 > 0 ? (p0 - window + 1) / BK : 0;
+    r.nb = hi - r.lo;
+    if (r.nb < 1) {
+        r.lo = max(0, hi - 1);
+        r.nb = 1;
+    }
+    return r;
+}
+
+// A position in the list of all key blocks of a call: entry b, key head h,
+// token tile t, and `off` blocks into that tile's `nb`; `left` is what the
+// CTA still has to do.
+struct Cursor {
+    int b, h, t, off;
+    int64_t left;
+    SeqView s;
+};
+
+// The list: entries in order, in each its key heads, in each the token tiles
+// (TT tokens), in each its key blocks.  Neighbouring CTAs therefore read the
+// same head's keys at the same time.  CTA c of n takes the blocks
+// [c * total / n, (c + 1) * total / n), so that all CTAs get the same number
+// whatever the lengths are; a tile cut by such a border is finished by
+// merge_kernel.
+template <int BK>
+__device__ __forceinline__ int64_t entry_blocks_warp(const SeqView &s, int TT, int window) {
+    // blocks of one head of this lane's entry; the lanes sum long entries together
+    const int lane = threadIdx.x & 31;
+    const int tiles = (s.n + TT - 1) / TT;
+    int64_t mine = 0;
+    if (tiles == 1) mine = key_range<BK>(s, 0, s.n, window).nb;
+    unsigned todo = __ballot_sync(0xffffffffu, tiles > 1);
+    while (todo) {
+        const int src = __ffs(todo) - 1;
+        todo &= todo - 1;
+        SeqView o;
+        o.n = __shfl_sync(0xffffffffu, s.n, src);
+        o.len = __shfl_sync(0xffffffffu, s.len, src);
+        const int ot = (o.n + TT - 1) / TT;
+        int64_t sum = 0;
+        for (int t = lane; t < ot; t += 32)
+            sum += key_range<BK>(o, t * TT, min((t + 1) * TT, o.n), window).nb;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == src) mine = sum;
+    }
+    return mine;
+}
+
+__device__ __forceinline__ int64_t warp_inclusive(int64_t v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// What a CTA does: its first block and how many.
+struct Share {
+    int64_t total;   // blocks of the call
+    int64_t first;   // this CTA's first
+    int n;           // CTAs that take part
+    Cursor c;        // at `first`; c.left blocks
+};
+
+// CTAs that take part in a call of `total` blocks: no share is smaller than
+// `least` blocks.
+__device__ __forceinline__ int sharers(int64_t total, int grid, int least) {
+    const int64_t n = (total + least - 1) / least;
+    return (int)(n < grid ? (n > 0 ? n : 1) : grid);
+}
+__device__ __forceinline__ int64_t share_start(int64_t total, int n, int c) {
+    return (int64_t)c * total / n;
+}
+// the CTA whose share holds block u
+__device__ __forceinline__ int share_owner(int64_t total, int n, int64_t u) {
+    return (int)(((u + 1) * n - 1) / total);
+}
+
+// Run by one whole warp.
+template <int BK>
+__device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int TT, int window, int cta, int grid,
+                            int least) {
+    const int lane = threadIdx.x & 31;
+    Share sh;
+    int64_t total = 0;
+    for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
+        SeqView s{0, 0, 0, 0};
+        if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
+        total += entry_blocks_warp<BK>(s, TT, window);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    sh.total = total * n_kv;
+    sh.n = sharers(sh.total, grid, least);
+    sh.first = 0;
+    sh.c = Cursor{0, 0, 0, 0, 0, SeqView{0, 0, 0, 0}};
+    if (sh.total == 0 || cta >= sh.n) return sh;
+    sh.first = share_start(sh.total, sh.n, cta);
+    sh.c.left = share_start(sh.total, sh.n, cta + 1) - sh.first;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
+        SeqView s{0, 0, 0, 0};
+        if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
+        const int64_t head = entry_blocks_warp<BK>(s, TT, window);
+        const int64_t end = before + warp_inclusive(head * n_kv);
+        const unsigned past = __ballot_sync(0xffffffffu, end > sh.first);
+        if (past) {
+            const int src = __ffs(past) - 1;
+            Cursor &c = sh.c;
+            c.b = b0 + src;
+            c.s.row = __shfl_sync(0xffffffffu, s.row, src);
+            c.s.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+            c.s.n = __shfl_sync(0xffffffffu, s.n, src);
+            c.s.len = __shfl_sync(0xffffffffu, s.len, src);
+            const int64_t per = __shfl_sync(0xffffffffu, head, src);
+            int64_t at = sh.first - (__shfl_sync(0xffffffffu, end, src) - per * n_kv);
+            c.h = (int)(at / per);
+            at -= c.h * per;
+            const int tiles = (c.s.n + TT - 1) / TT;
+            int64_t seen = 0;
+            for (int t0 = 0; t0 < tiles; t0 += 32) {
+                int64_t nb = 0;
+                if (t0 + lane < tiles)
+                    nb = key_range<BK>(c.s, (t0 + lane) * TT, min((t0 + lane + 1) * TT, c.s.n),
+                                       window)
+                             .nb;
+                const int64_t e = seen + warp_inclusive(nb);
+                const unsigned over = __ballot_sync(0xffffffffu, e > at);
+                if (over) {
+                    const int l = __ffs(over) - 1;
+                    c.t = t0 + l;
+                    c.off = (int)(at - __shfl_sync(0xffffffffu, e - nb, l));
+                    break;
+                }
+                seen = __shfl_sync(0xffffffffu, e, 31);
+            }
+            return sh;
+        }
+        before = __shfl_sync(0xffffffffu, end, 31);
+    }
+    return sh;
+}
+
+// One piece of work: blocks [k0, k1) of the nb blocks of a tile, which begin
+// at key block lo.
+struct Piece {
+    SeqView s;
+    int h, t0, t1;     // key head; new tokens [t0, t1)
+    int lo, k0, k1, nb;
+    int t;             // tile number (for the merge)
+};
+
+// Takes the next piece of the cursor and steps past it; false when done.
+// (Any thread: no warp-wide step.)
+template <int BK>
+__device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, int TT, int window,
+                                           Cursor &c, Piece &p) {
+    if (c.left <= 0) return false;
+    p.s = c.s;
+    p.h = c.h;
+    p.t = c.t;
+    p.t0 = c.t * TT;
+    p.t1 = min(p.t0 + TT, c.s.n);
+    const KeyRange r = key_range<BK>(c.s, p.t0, p.t1, window);
+    p.lo = r.lo;
+    p.nb = r.nb;
+    p.k0 = c.off;
+    p.k1 = (int)min((int64_t)r.nb, c.off + c.left);
+    c.left -= p.k1 - p.k0;
+    c.off = p.k1;
+    if (p.k1 == r.nb && c.left > 0) {
+        c.off = 0;
+        if (p.t1 < c.s.n) {
+            ++c.t;
+        } else {
+            c.t = 0;
+            if (++c.h == n_kv) {
+                c.h = 0;
+                do {
+                    c.s = seq_view(pb, ++c.b);
+                } while (c.s.n == 0);
+            }
+        }
+    }
+    return true;
+}
+
+// page of key `key` of table row `row`; n_pages (whose reads give zeros) when
+// the table holds none there, which raises the error word
+__device__ __forceinline__ int page_of(const PagedBatch &pb, int row, int key) {
+    const int p = pb.table[(int64_t)row * pb.table_ld + key / pb.page_size];
+    if (p >= 0 && p < pb.n_pages) return p;
+    atomicOr(pb.err, kErrBadIndex);
+    return pb.n_pages;
+}
+
+// A tile whose blocks several CTAs share: CTA c's part goes to slot 2c + 1 when
+// it begins the tile, else 2c; the CTA that begins a tile it does not finish
+// leaves this note for the merge (parts == 0: none).
+struct SplitNote {
+    int q_row, heads0, tokens, parts;
+};
+
+// An attention call as its kernels take it.
+struct PagedAttnArgs {
+    PagedBatch pb;
+    const uint16_t *q;   // [n_tokens][q_ld]: n_heads x head_dim each
+    uint16_t *out;       // [n_tokens][out_ld]
+    int64_t q_ld, out_ld;
+    int n_heads, n_kv, window;
+    int box;             // keys per TMA box
+    int least;           // fewest key blocks of a CTA's share
+    float scale;
+    SplitNote *notes;    // [CTAs]
+    float *part_ml;      // [2 CTAs][rows][2]: maximum (times scale log2 e), sum
+    float *part_o;       // [2 CTAs][rows][head_dim]
+};
+
+// A checked call, as the C ABI hands it to launch_paged_attention.
+struct PagedAttnCall {
+    PagedBatch pb;
+    const uint16_t *q, *k, *v;
+    uint16_t *out;
+    int64_t q_ld, out_ld, page_stride, max_q;
+    int n_heads, n_kv, head_dim, window;
+    bool f16;
+    float scale;
+    void *ws;
+};
+
+inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t max_q);
+cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st);
+
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem,
+                       cudaStream_t stream, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+__device__ __forceinline__ void tma_load_4d(void *smem_dst, const void *tmap, uint64_t *bar,
+                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+}  // namespace nq

@@ -1,0 +1,277 @@
+"""The key/value cache in pages, over the C ABI (nq_paged_*, nq_pages_*).
+
+    paged_append(q, k, v, k_pages, v_pages, table, kv_lens, ...)   rotary positions, store
+    paged_attention(q, k_pages, v_pages, table, kv_lens, ...)      attention of new tokens
+    pages_reserve / pages_fork / pages_free / pages_compact        the page pool
+    copy_pages(pool, src, dst)
+
+A pool is a tensor [layers, 2, pages, kv heads, page size, head dim] (bf16 or
+fp16); layer l's keys are pool[l, 0] and its values pool[l, 1].  table
+[rows, width] (int32, -1: no page) lists the pages of each sequence, kv_lens
+[rows] their lengths, new tokens included, refs [pages] how many sequences hold
+a page.  A step's batch is its sequences' new tokens one after another: those
+of entry b are rows q_starts[b] .. q_starts[b + 1] (one each without q_starts),
+its table row seqs[b] (b without seqs; negative: padding).
+
+Every call is asynchronous on torch's current stream, reads its index tensors
+on the device only, and may be captured in a CUDA graph.  Arguments that can
+be seen to be wrong raise NQError; what the index tensors say wrong raises bits
+of take_device_error() (include/nq.h).
+"""
+import ctypes
+import math
+
+import torch
+
+from ._lib import NQError, check, lib
+
+P, I64, I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+
+_DTYPES = {torch.bfloat16: 1, torch.float16: 2}
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("n_pages", I64), ("page_stride", I64), ("n_kv_heads", I),
+                ("page_size", I), ("head_dim", I), ("dtype", I)]
+
+
+class _Batch(ctypes.Structure):
+    _fields_ = [("table", P), ("table_ld", I64), ("table_width", I64), ("n_rows", I64),
+                ("kv_lens", P), ("seqs", P), ("q_starts", P), ("n_seqs", I64), ("n_tokens", I64)]
+
+
+class _Table(ctypes.Structure):
+    _fields_ = [("refs", P), ("table", P), ("lens", P), ("n_pages", I64), ("n_rows", I64),
+                ("table_ld", I64), ("table_width", I64), ("page_size", I)]
+
+
+class _Pool(ctypes.Structure):
+    _fields_ = [("data", P), ("outer", I64), ("n_pages", I64), ("page_bytes", I64)]
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _index(t, name, device, dim=1):
+    """An int32 index tensor on `device`, its last axis contiguous."""
+    if t.dtype is not torch.int32 or t.dim() != dim or t.get_device() != device or \
+            (t.numel() > 0 and t.stride(-1) != 1):
+        raise NQError(1, f"{name} must be a contiguous int32 tensor with {dim} axes on the cache's "
+                         "device")
+    return t.data_ptr()
+
+
+def _rows(t, name, heads, dim, like):
+    """Rows [tokens, heads, dim] whose heads lie one after another."""
+    if t.dtype is not like.dtype or t.dim() != 3 or t.get_device() != like.get_device():
+        raise NQError(1, f"{name} must be [tokens, heads, head dim], of the cache's type and on its "
+                         "device")
+    if t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise NQError(1, f"{name} has shape {tuple(t.shape)}, expected [tokens, "
+                         f"{heads if heads is not None else 'heads'}, {dim}]")
+    if t.stride(2) != 1 or (t.stride(1) != dim and t.shape[1] > 1):
+        raise NQError(1, f"{name}: the heads of a token must lie one after another")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * dim
+
+
+def _cache(k, v):
+    if k.dtype not in _DTYPES or k.dim() != 4 or not k.is_cuda:
+        raise NQError(1, "k_pages must be a bf16 or fp16 CUDA tensor "
+                         "[pages, kv heads, page size, head dim]")
+    if v.dtype is not k.dtype or v.shape != k.shape or v.stride() != k.stride() or \
+            v.get_device() != k.get_device():
+        raise NQError(1, "v_pages must match k_pages in type, shape, strides and device")
+    n, heads, size, dim = k.shape
+    if k.numel() > 0 and not k[0].is_contiguous():
+        raise NQError(1, "a page must be contiguous")
+    if k.get_device() != torch.cuda.current_device():
+        raise NQError(1, "the cache is not on the current device")
+    return _Cache(k.data_ptr(), v.data_ptr(), n, k.stride(0) if n > 1 else heads * size * dim,
+                  heads, size, dim, _DTYPES[k.dtype])
+
+
+def _batch(table, kv_lens, seqs, q_starts, tokens, device):
+    tp, lp = _index(table, "table", device, 2), _index(kv_lens, "kv_lens", device)
+    rows, width = table.shape
+    if kv_lens.shape[0] != rows:
+        raise NQError(1, f"kv_lens has {kv_lens.shape[0]} entries for {rows} table rows")
+    sp = qp = None
+    if seqs is not None:
+        sp, n = _index(seqs, "seqs", device), seqs.shape[0]
+        if q_starts is not None and q_starts.shape[0] != n + 1:
+            raise NQError(1, f"q_starts must have {n + 1} entries")
+    elif q_starts is not None:
+        n = q_starts.shape[0] - 1
+    else:
+        n = min(rows, tokens)
+    if q_starts is not None:
+        qp = _index(q_starts, "q_starts", device)
+    return _Batch(tp, table.stride(0) if rows > 1 else width, width, rows, lp, sp, qp, n, tokens)
+
+
+def rope_frequencies(dims, base=10000.0, device="cuda"):
+    """base^(-2 i / dims) for i < dims / 2 (radians per position), fp32: the `freqs` of
+    paged_append for a plain rotary embedding over the first `dims` dims of a head."""
+    f = [float(base) ** (-2.0 * i / dims) for i in range(dims // 2)]
+    return torch.tensor(f, dtype=torch.float64).to(torch.float32).to(device)
+
+
+def paged_attention_workspace_size(n_heads, n_kv_heads, head_dim, max_q):
+    return int(lib().nq_paged_attention_workspace_size(n_heads, n_kv_heads, head_dim, max_q))
+
+
+def paged_attention(q, k_pages, v_pages, table, kv_lens, q_starts=None, max_q=None, window=0,
+                    scale=None, seqs=None, out=None, workspace=None):
+    """Attention of the new tokens q [tokens, heads, head dim] over their sequences' pages;
+    token t of an entry's n stands at position kv_len - n + t and sees the keys up to it
+    (and only the last `window` of them when window > 0).  scale: 1 / sqrt(head dim)
+    unless given.  max_q: the longest entry's number of new tokens (the kernel is chosen
+    by it; without it, the number of rows).  out: as q, or a new tensor."""
+    c = _cache(k_pages, v_pages)
+    device = k_pages.get_device()
+    qp, q_ld = _rows(q, "q", None, c.head_dim, k_pages)
+    tokens, heads = q.shape[0], q.shape[1]
+    b = _batch(table, kv_lens, seqs, q_starts, tokens, device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise NQError(1, "out must have q's shape")
+    op, out_ld = _rows(out, "out", heads, c.head_dim, k_pages)
+    if q_starts is None:
+        max_q = 1
+    elif max_q is None:
+        max_q = tokens
+    f = lib()
+    if workspace is None:
+        need = f.nq_paged_attention_workspace_size(heads, c.n_kv_heads, c.head_dim, max_q)
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise NQError(1, "workspace must be contiguous, on the cache's device")
+    check(f.nq_paged_attention(qp, q_ld, heads, ctypes.byref(c), ctypes.byref(b), max_q,
+                               scale if scale is not None else 1.0 / math.sqrt(c.head_dim), window,
+                               workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                               op, out_ld, _stream()))
+    return out
+
+
+def paged_append(q, k, v, k_pages, v_pages, table, kv_lens, q_starts=None, freqs=None, seqs=None,
+                 q_out=None):
+    """Turns the new tokens' queries and keys by their positions (freqs: fp32, radians per
+    position of each pair of dims; None: no turn) and stores keys and values in their pages.
+    Returns the queries: in q_out (may be q), or a new tensor."""
+    c = _cache(k_pages, v_pages)
+    device = k_pages.get_device()
+    qp, q_ld = _rows(q, "q", None, c.head_dim, k_pages)
+    tokens, heads = q.shape[0], q.shape[1]
+    kp, k_ld = _rows(k, "k", c.n_kv_heads, c.head_dim, k_pages)
+    vp, v_ld = _rows(v, "v", c.n_kv_heads, c.head_dim, k_pages)
+    if k.shape[0] != tokens or v.shape[0] != tokens:
+        raise NQError(1, "q, k and v differ in tokens")
+    b = _batch(table, kv_lens, seqs, q_starts, tokens, device)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif q_out.shape != q.shape:
+        raise NQError(1, "q_out must have q's shape")
+    op, out_ld = _rows(q_out, "q_out", heads, c.head_dim, k_pages)
+    fp, nf = None, 0
+    if freqs is not None:
+        if freqs.dtype is not torch.float32 or freqs.dim() != 1 or \
+                freqs.get_device() != device or not freqs.is_contiguous():
+            raise NQError(1, "freqs must be a contiguous fp32 vector on the cache's device")
+        fp, nf = freqs.data_ptr(), freqs.shape[0]
+    check(lib().nq_paged_append(qp, q_ld, kp, k_ld, vp, v_ld, heads, ctypes.byref(c),
+                                ctypes.byref(b), fp, nf, op, out_ld, _stream()))
+    return q_out
+
+
+def _table(refs, table, lens, page_size):
+    device = refs.get_device()
+    if not refs.is_cuda or device != torch.cuda.current_device():
+        raise NQError(1, "refs must be a CUDA tensor on the current device")
+    rp, tp = _index(refs, "refs", device), _index(table, "table", device, 2)
+    rows, width = table.shape
+    lp = _index(lens, "lens", device) if lens is not None else rp
+    if lens is not None and lens.shape[0] != rows:
+        raise NQError(1, f"lens has {lens.shape[0]} entries for {rows} table rows")
+    return _Table(rp, tp, lp, refs.shape[0], rows, table.stride(0) if rows > 1 else width, width,
+                  page_size)
+
+
+def _pool(pool):
+    if not pool.is_cuda or pool.dim() < 4 or not pool.is_contiguous():
+        raise NQError(1, "pool must be a contiguous CUDA tensor "
+                         "[..., pages, kv heads, page size, head dim]")
+    if pool.get_device() != torch.cuda.current_device():
+        raise NQError(1, "the pool is not on the current device")
+    n, page = pool.shape[-4], pool.shape[-3] * pool.shape[-2] * pool.shape[-1]
+    if pool.numel() == 0:
+        raise NQError(1, "the pool is empty")
+    return _Pool(pool.data_ptr(), pool.numel() // (n * page), n, page * pool.element_size())
+
+
+def _lists(device, n, **lists):
+    for name, t in lists.items():
+        _index(t, name, device)
+        if t.shape[0] != n:
+            raise NQError(1, f"{name} must have {n} entries")
+
+
+def _workspace(ws, need, device):
+    if ws is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if ws.device != device or not ws.is_contiguous():
+        raise NQError(1, "workspace must be contiguous, on the pool's device")
+    return ws
+
+
+def pages_free(refs, table, lens, seqs):
+    """The sequences give their pages back: one holder less each, length 0."""
+    t = _table(refs, table, lens, 1)
+    _lists(refs.get_device(), seqs.shape[0], seqs=seqs)
+    check(lib().nq_pages_free(ctypes.byref(t), seqs.data_ptr(), seqs.shape[0], _stream()))
+
+
+def pages_fork(refs, table, lens, parents, children):
+    """children[i] (empty so far) becomes a copy of parents[i] that shares its pages."""
+    t = _table(refs, table, lens, 1)
+    n = parents.shape[0]
+    _lists(refs.get_device(), n, parents=parents, children=children)
+    check(lib().nq_pages_fork(ctypes.byref(t), parents.data_ptr(), children.data_ptr(), n,
+                              _stream()))
+
+
+def pages_workspace_size(n_pages, n):
+    """Bytes that pages_reserve (n sequences) and pages_compact (n_pages pages) need."""
+    return int(lib().nq_pages_workspace_size(n_pages, n))
+
+
+def pages_reserve(pool, refs, table, lens, seqs, new_lens, workspace=None):
+    """The sequences grow to new_lens tokens: shared last pages that are not full are
+    copied, free pages added.  All or nothing (see include/nq.h)."""
+    p = _pool(pool)
+    t = _table(refs, table, lens, pool.shape[-2])
+    n = seqs.shape[0]
+    _lists(pool.get_device(), n, seqs=seqs, new_lens=new_lens)
+    ws = _workspace(workspace, lib().nq_pages_workspace_size(0, n), pool.device)
+    check(lib().nq_pages_reserve(ctypes.byref(t), ctypes.byref(p), seqs.data_ptr(),
+                                 new_lens.data_ptr(), n, ws.data_ptr(),
+                                 ws.numel() * ws.element_size(), _stream()))
+
+
+def pages_compact(pool, refs, table, workspace=None):
+    """The used pages move to the pool's low end; refs and table follow."""
+    p = _pool(pool)
+    t = _table(refs, table, None, pool.shape[-2])
+    ws = _workspace(workspace, lib().nq_pages_workspace_size(t.n_pages, 0), pool.device)
+    check(lib().nq_pages_compact(ctypes.byref(t), ctypes.byref(p), ws.data_ptr(),
+                                 ws.numel() * ws.element_size(), _stream()))
+
+
+def copy_pages(pool, src, dst):
+    """Copies page src[i] to dst[i] in every layer; a target may not also be a source or
+    an earlier target (that move is refused)."""
+    p = _pool(pool)
+    n = src.shape[0]
+    _lists(pool.get_device(), n, src=src, dst=dst)
+    check(lib().nq_pages_copy(ctypes.byref(p), src.data_ptr(), dst.data_ptr(), n, _stream()))
