@@ -24,7 +24,8 @@ ROOT = os.path.dirname(HERE)
 INCLUDE = os.path.join(ROOT, "include")
 
 CU_SOURCES = ["abi.cu", "quant.cu", "gemv.cu", "gemm_tc.cu", "gemm_tc_moe.cu", "moe.cu",
-              "moe_small.cu", "llama.cu", "paged.cu", "attn_paged.cu"]
+              "moe_small.cu", "llama.cu", "paged.cu", "attn_paged.cu",
+              "attn_paged_tc.cu"]
 CPP_SOURCES = ["cuda_backend.cpp", "model_loader.cpp"]
 HEADERS = ["nq_common.cuh", "nq_internal.h", "paged.cuh", "cuda_backend.h", "iface/compute_types.h",
            "iface/compute_backend.h", "model_loader.h"]

@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
             for (int i = 0; i < 2; ++i) {
                 const int r = r0 + 8 * i;
                 if (r >= valid) continue;
-                const float f = whole ? (L[i] > 0.f ? 1.f / L[i] : 0.f) : 1.f;
+                const float f = whole ? (L[i] == 0.f ? 0.f : 1.f / L[i]) : 1.f;
                 uint16_t *op = a.out + (int64_t)(p.s.q0 + p.t0 + r / G) * a.out_ld +
                                (int64_t)(p.h * G + r % G) * HD;
                 float *pp = a.part_o + ((int64_t)slot * kRows + r) * HD;
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
     float M = -INFINITY;
     for (int i = lane; i < note.parts; i += 32) {
         const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + slot(i) * 2);
-        if (ml.y > 0.f) M = fmaxf(M, ml.x);
+        if (ml.y != 0.f) M = fmaxf(M, ml.x);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
@@ -428,12 +428,12 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
             v[j] = w.x;
             v[j + 1] = w.y;
         }
-        const float f = ml.y > 0.f ? ex2(ml.x - M) : 0.f;
+        const float f = ml.y != 0.f ? ex2(ml.x - M) : 0.f;
         L += ml.y * f;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) acc[j] = fmaf(v[j], f, acc[j]);
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
     uint16_t *op = a.out + (int64_t)(note.q_row + r / G) * a.out_ld +
                    (int64_t)(note.heads0 + r % G) * HD + lane * kPer;
 #pragma unroll
@@ -444,18 +444,38 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 // CTAs of paged_rows_kernel: as many as fit at once
 int rows_grid(int hd) { return sm_count() * (hd == 256 ? Cfg<256>::kCtas : Cfg<128>::kCtas); }
 
+// Which kernel serves a call: paged_rows_kernel while a sequence's new tokens
+// make one tile of 16 rows, so that each key is read once; the tensor-core
+// kernel (128- or 256-row tiles) from there on.
+struct Shape {
+    bool tiles;
+    int grid, rows, block;  // CTAs, rows of a part, keys of a block
+};
+
+Shape shape_of(int n_heads, int n_kv, int hd, int64_t max_q) {
+    const int G = n_heads / n_kv;
+    if (max_q * G > kRows) return Shape{true, sm_count(), paged_tiles_rows(hd), 128};
+    return Shape{false, rows_grid(hd), kRows, kBlock};
+}
+
 template <int HD, bool F16>
-cudaError_t run_rows(PagedAttnArgs a, const CUtensorMap &mk, const CUtensorMap &mv,
+cudaError_t run_rows(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
                      cudaStream_t st) {
     auto kern = paged_rows_kernel<HD, F16>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          Cfg<HD>::kSmem);
     if (e != cudaSuccess) return e;
-    const int grid = rows_grid(HD);
-    e = launch_pdl(kern, dim3((unsigned)grid), kThreads, Cfg<HD>::kSmem, st, mk, mv, a);
+    return launch_pdl(kern, dim3((unsigned)rows_grid(HD)), kThreads, Cfg<HD>::kSmem, st, mk, mv, a);
+}
+
+template <int HD, bool F16>
+cudaError_t run_attention(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
+                          const Shape &s, cudaStream_t st) {
+    const cudaError_t e = s.tiles ? launch_paged_tiles(a, mk, mv, HD, F16, st)
+                                  : run_rows<HD, F16>(a, mk, mv, st);
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_merge_kernel<HD, F16>, dim3((unsigned)grid, kRows / 4), 128, 0, st, a,
-                      (int)kRows);
+    return launch_pdl(paged_merge_kernel<HD, F16>, dim3((unsigned)s.grid, (unsigned)s.rows / 4),
+                      128, 0, st, a, s.rows);
 }
 
 // A workspace holds, for each CTA, the note and two parts of `rows` rows.
@@ -477,13 +497,12 @@ void place_workspace(PagedAttnArgs &a, int grid, int rows, void *ws) {
 }  // namespace
 
 size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t max_q) {
-    (void)n_heads;
-    (void)n_kv;
-    (void)max_q;
-    return part_bytes(rows_grid(head_dim), kRows, head_dim);
+    const Shape s = shape_of(n_heads, n_kv, head_dim, max_q);
+    return part_bytes(s.grid, s.rows, head_dim);
 }
 
 cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
+    const Shape s = shape_of(c.n_heads, c.n_kv, c.head_dim, c.max_q);
     PagedAttnArgs a;
     a.pb = c.pb;
     a.q = c.q;
@@ -496,23 +515,22 @@ cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
     a.scale = c.scale;
     a.least = 1;
     // the largest power of two that divides the page size: no box crosses a page
-    a.box = std::min(kBlock, c.pb.page_size & -c.pb.page_size);
-    const int hd = c.head_dim;
-    place_workspace(a, rows_grid(hd), kRows, c.ws);
+    a.box = std::min(s.block, c.pb.page_size & -c.pb.page_size);
+    place_workspace(a, s.grid, s.rows, c.ws);
     CUtensorMap mk, mv;
-    if (!make_map_pages(&mk, c.f16, c.k, hd, c.pb.page_size, c.n_kv, c.pb.n_pages, c.page_stride,
-                        a.box) ||
-        !make_map_pages(&mv, c.f16, c.v, hd, c.pb.page_size, c.n_kv, c.pb.n_pages, c.page_stride,
-                        a.box))
+    if (!make_map_pages(&mk, c.f16, c.k, c.head_dim, c.pb.page_size, c.n_kv, c.pb.n_pages,
+                        c.page_stride, a.box) ||
+        !make_map_pages(&mv, c.f16, c.v, c.head_dim, c.pb.page_size, c.n_kv, c.pb.n_pages,
+                        c.page_stride, a.box))
         return cudaErrorInvalidValue;
     if (c.f16) {
-        if (hd == 64) return run_rows<64, true>(a, mk, mv, st);
-        if (hd == 128) return run_rows<128, true>(a, mk, mv, st);
-        return run_rows<256, true>(a, mk, mv, st);
+        if (c.head_dim == 64) return run_attention<64, true>(a, mk, mv, s, st);
+        if (c.head_dim == 128) return run_attention<128, true>(a, mk, mv, s, st);
+        return run_attention<256, true>(a, mk, mv, s, st);
     }
-    if (hd == 64) return run_rows<64, false>(a, mk, mv, st);
-    if (hd == 128) return run_rows<128, false>(a, mk, mv, st);
-    return run_rows<256, false>(a, mk, mv, st);
+    if (c.head_dim == 64) return run_attention<64, false>(a, mk, mv, s, st);
+    if (c.head_dim == 128) return run_attention<128, false>(a, mk, mv, s, st);
+    return run_attention<256, false>(a, mk, mv, s, st);
 }
 
 }  // namespace nq

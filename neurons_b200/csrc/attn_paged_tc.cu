@@ -1,0 +1,577 @@
+// attn_paged_tc.cu -- attention of new tokens over the paged cache for many
+// query rows per key head (chunks of a prompt), on tcgen05 tensor cores.  The
+// mathematics and the split over the CTAs are attn_paged.cu's; paged.cuh has
+// the split.
+//
+// A query tile is 128 rows (the G query heads of a key head times 128 / G
+// tokens), a key block 128 keys.  One CTA per SM, persistent over its pieces:
+//   loader warp   K and V blocks into a ring of stages by TMA (128-byte
+//                 swizzle, boxes of 16 to 128 keys x 64 dims)
+//   MMA warp      S = Q K^T (both in shared memory) and O += P V (P in TMEM, V as
+//                 it lies: keys x dims, the MN-major operand), one thread
+//   softmax       one row per thread: S from TMEM, a running maximum and sum,
+//                 P back into S's columns in 16 bits
+// Two tiles S are always in flight, so that the tensor cores work on one while
+// the softmax warps work on the other:
+//   two query tiles  (more than 128 / G tokens): one warpgroup each, and each
+//                    key block is read once for 256 rows
+//   one query tile   two warpgroups take the key blocks in turn, each with a
+//                    maximum, sum and O of its own, joined at the end
+//   256 dims         O fills half of the TMEM: one warpgroup, one O, two S
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the
+// last time; until then the weights are up to 2^8, which costs neither bf16
+// nor fp16 precision.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "nq_common.cuh"
+#include "nq_internal.h"
+#include "paged.cuh"
+
+namespace nq {
+namespace {
+
+constexpr int kBlock = 128;  // keys per block, rows per query tile
+
+template <int HD>
+struct Tc {
+    static constexpr int kGroups = HD == 256 ? 1 : 2;       // softmax warpgroups
+    static constexpr int kMmaWarp = 4 * kGroups, kLoadWarp = kMmaWarp + 1;
+    static constexpr int kThreads = 32 * (kLoadWarp + 1);
+    // a ring stage: 128 keys (or values) x kUnitDims dims
+    static constexpr int kUnitDims = HD < 128 ? HD : 128;
+    static constexpr int kUnits = HD / kUnitDims;
+    static constexpr int kUnitBytes = kBlock * kUnitDims * 2;
+    static constexpr int kStages = HD == 64 ? 8 : 5;
+    static constexpr int kQBytes = kBlock * HD * 2;
+    static constexpr int kSmem = kGroups * kQBytes + kStages * kUnitBytes;
+    static constexpr int kO = 256;                          // first TMEM column of O
+    static constexpr int kRows = kGroups * kBlock;          // rows of a part
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T, kind::f16, one CTA
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u));
+}
+
+// An operand whose N (here: dims) runs along memory, 128-byte swizzle: atoms of
+// 64 dims x 8 keys, the next 8 keys 1024 bytes on (stride offset), the next 64
+// dims a 128-key column of 16 KB on (leading offset).
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(16384u >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+        "%28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]));
+}
+
+// The blocks of a piece as steps: step i works on S buffer i % 2.
+template <int HD>
+struct Plan {
+    bool two;    // two query tiles: steps 2b and 2b + 1 are block b
+    int n;       // blocks
+    int tok;     // tokens per query tile
+    __device__ __forceinline__ Plan(const Piece &p, int tok_)
+        : two(Tc<HD>::kGroups == 2 && p.t1 - p.t0 > tok_), n(p.k1 - p.k0), tok(tok_) {}
+    __device__ __forceinline__ int steps() const { return two ? 2 * n : n; }
+    __device__ __forceinline__ int block(int i) const { return two ? i >> 1 : i; }
+    __device__ __forceinline__ bool last_use(int i) const { return !two || (i & 1); }
+    // place of block b's keys and values in the loads' order, which is that of
+    // their first use
+    __device__ __forceinline__ int key_load(int b) const {
+        return two ? 2 * b : (b == 0 ? 0 : 2 * b - 1);
+    }
+    __device__ __forceinline__ int value_load(int b) const {
+        return two ? 2 * b + 1 : (b < n - 1 ? 2 * b + 2 : 2 * n - 1);
+    }
+};
+
+// One ring stage: kUnitDims dims from u * kUnitDims on of block `blk`.  Boxes
+// without a visible key of the piece read as zeros (page n_pages).
+template <int HD>
+__device__ __forceinline__ void load_unit(const PagedAttnArgs &a, const CUtensorMap *map,
+                                          const Piece &p, int blk, int u, int key_lo, int key_hi,
+                                          uint8_t *stage, uint64_t *bar) {
+    using T = Tc<HD>;
+    constexpr int kCols = T::kUnitDims / 64;
+    const int lane = threadIdx.x & 31;
+    const int r = lane / kCols, col = lane % kCols;
+    const bool on = r < kBlock / a.box;
+    const int key = blk * kBlock + r * a.box;
+    int page = a.pb.n_pages, slot = 0;
+    if (on && key < key_hi && key + a.box > key_lo) {
+        page = page_of(a.pb, p.s.row, key);
+        slot = key % a.pb.page_size;
+    }
+    if (lane == 0) mbar_expect_tx(bar, T::kUnitBytes);
+    __syncwarp();
+    if (on)
+        tma_load_4d(stage + col * (kBlock * 128) + r * a.box * 128, map, bar,
+                    u * T::kUnitDims + col * 64, slot, p.h, page);
+}
+
+template <int HD, bool F16>
+__global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
+    const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+    const PagedAttnArgs a) {
+    using T = Tc<HD>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *qs = smem, *ring = smem + T::kGroups * T::kQBytes;
+    __shared__ __align__(8) uint64_t full[T::kStages], empty[T::kStages], s_full[2], p_ready[2];
+    __shared__ __align__(8) uint64_t q_full, o_full, pv_done;
+    __shared__ uint32_t tmem_holder;
+    __shared__ int abort_flag;
+    __shared__ float xm[T::kGroups == 2 ? kBlock : 1], xl[T::kGroups == 2 ? kBlock : 1];
+    volatile int *abort = &abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = a.n_heads / a.n_kv, tok = kBlock / G, TT = T::kGroups * tok;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < T::kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_ready[i], kBlock);
+        }
+        mbar_init(&q_full, T::kGroups * kBlock);
+        mbar_init(&o_full, 1);
+        mbar_init(&pv_done, 1);
+        abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+    }
+    if (warp == T::kMmaWarp) {
+        tmem_alloc(&tmem_holder, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_holder;
+    pdl_wait();  // lengths, tables, q and the cache come from earlier kernels
+
+    const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x, a.least);
+    Cursor c = sh.c;
+    Piece p;
+
+    if (warp == T::kLoadWarp) {
+        int g = 0;  // stages filled so far
+        bool ok = true;
+        while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+            const Plan<HD> pl(p, tok);
+            const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
+            const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+            for (int t = 0; ok && t < 2 * pl.n; ++t) {
+                bool is_v;
+                int b;
+                if (pl.two) {
+                    is_v = t & 1;
+                    b = t >> 1;
+                } else if (t == 0 || t == 2 * pl.n - 1) {
+                    is_v = t != 0;
+                    b = is_v ? pl.n - 1 : 0;
+                } else {
+                    is_v = !(t & 1);
+                    b = is_v ? (t - 2) / 2 : (t + 1) / 2;
+                }
+                for (int u = 0; ok && u < T::kUnits; ++u, ++g) {
+                    const int st = g % T::kStages;
+                    ok = mbar_wait_or_abort(&empty[st], (uint32_t)(g / T::kStages + 1) & 1u, abort,
+                                            a.pb.err);
+                    if (!ok) break;
+                    load_unit<HD>(a, is_v ? &mv : &mk, p, p.lo + p.k0 + b, u, key_lo, key_hi,
+                                  ring + st * T::kUnitBytes, &full[st]);
+                }
+            }
+        }
+        if (!ok || *abort) {  // given up: the copies in flight end before this CTA does
+            for (int j = max(0, g - T::kStages); j < g; ++j) {
+                const unsigned long long t0 = global_timer_ns();
+                while (!mbar_try_wait(&full[j % T::kStages], (uint32_t)(j / T::kStages) & 1u) &&
+                       global_timer_ns() - t0 < kWaitLimitNs) {
+                }
+            }
+        }
+    } else if (warp == T::kMmaWarp) {
+        if (lane == 0) {
+            constexpr uint32_t kIdS = F16 ? idesc_f16_f32(128, 128) : idesc_bf16_f32(128, 128);
+            constexpr uint32_t kIdO = (F16 ? idesc_f16_f32(128, T::kUnitDims)
+                                           : idesc_bf16_f32(128, T::kUnitDims)) |
+                                      (1u << 16);  // B: N along memory
+            int loads = 0, pieces = 0;
+            uint32_t p_phase = 0;  // bit: parity of that buffer's next p_ready
+            bool ok = true;
+            auto wait_stage = [&](int g) {
+                ok = ok && mbar_wait_or_abort(&full[g % T::kStages],
+                                              (uint32_t)(g / T::kStages) & 1u, abort, a.pb.err);
+            };
+            while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+                const Plan<HD> pl(p, tok);
+                const int steps = pl.steps();
+                ok = mbar_wait_or_abort(&q_full, (uint32_t)pieces & 1u, abort, a.pb.err);
+                auto issue_s = [&](int i) {
+                    const int b = pl.block(i), buf = i & 1;
+                    const uint32_t qa = smem_u32(qs + (pl.two ? buf : 0) * T::kQBytes);
+#pragma unroll
+                    for (int u = 0; u < T::kUnits; ++u) {
+                        const int g = (loads + pl.key_load(b)) * T::kUnits + u;
+                        wait_stage(g);
+                        if (!ok) return;
+                        tc_fence_after();
+                        const uint32_t ka = smem_u32(ring + (g % T::kStages) * T::kUnitBytes);
+#pragma unroll
+                        for (int kk = 0; kk < T::kUnitDims / 16; ++kk) {
+                            // 16 dims: 32 bytes on in the swizzled rows; 64: the next column
+                            const uint32_t off = (kk >> 2) * (kBlock * 128) + (kk & 3) * 32;
+                            umma_ss(tmem + buf * 128,
+                                    smem_desc_k_sw128(qa + u * (T::kUnitDims / 64) * (kBlock * 128) + off),
+                                    smem_desc_k_sw128(ka + off), kIdS, (u > 0 || kk > 0) ? 1u : 0u);
+                        }
+                        if (pl.last_use(i)) umma_commit(&empty[g % T::kStages]);
+                    }
+                    umma_commit(&s_full[buf]);
+                };
+                if (ok) issue_s(0);
+                if (ok && steps > 1) issue_s(1);
+                for (int i = 0; ok && i < steps; ++i) {
+                    const int b = pl.block(i), buf = i & 1;
+                    ok = mbar_wait_or_abort(&p_ready[buf], (p_phase >> buf) & 1u, abort, a.pb.err);
+                    if (!ok) break;
+                    p_phase ^= 1u << buf;
+                    const uint32_t acc = T::kGroups == 2 ? i > 1 : i > 0;
+                    const uint32_t o = tmem + T::kO + (T::kGroups == 2 ? buf * HD : 0);
+#pragma unroll
+                    for (int u = 0; u < T::kUnits; ++u) {
+                        const int g = (loads + pl.value_load(b)) * T::kUnits + u;
+                        wait_stage(g);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t va = smem_u32(ring + (g % T::kStages) * T::kUnitBytes);
+#pragma unroll
+                        for (int kk = 0; kk < kBlock / 16; ++kk)
+                            umma_ts(o + u * T::kUnitDims, tmem + buf * 128 + kk * 8,
+                                    smem_desc_mn_sw128(va + kk * 16 * 128), kIdO,
+                                    (acc || kk > 0) ? 1u : 0u);
+                        if (pl.last_use(i)) umma_commit(&empty[g % T::kStages]);
+                    }
+                    if (T::kGroups == 1) umma_commit(&pv_done);
+                    if (ok && i + 2 < steps) issue_s(i + 2);
+                }
+                umma_commit(&o_full);
+                loads += 2 * pl.n;
+                ++pieces;
+            }
+            if (!ok && pieces > 0) {  // given up: the products in flight end first
+                const unsigned long long t0 = global_timer_ns();
+                while (!mbar_try_wait(&o_full, (uint32_t)(pieces - 1) & 1u) &&
+                       global_timer_ns() - t0 < kWaitLimitNs) {
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------- softmax
+        const int w = warp >> 2;                    // warpgroup
+        const int r = threadIdx.x & 127;            // this thread's row of the query tile
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
+        int loads = 0, pieces = 0, pvs = 0;
+        uint32_t s_phase = 0;
+        int64_t unit = sh.first;
+        bool ok = true, note_left = false;
+        while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+            const Plan<HD> pl(p, tok);
+            const int steps = pl.steps();
+            const int sub = pl.two ? w : 0;         // which query tile
+            const int t0 = p.t0 + sub * tok, t1 = min(t0 + tok, p.t1);
+            const int valid = (t1 - t0) * G;
+            const int base = p.s.len - p.s.n;
+            const int key_hi = base + p.t1;
+            const int key_lo = a.window > 0 ? max(0, base + p.t0 - a.window + 1) : 0;
+            const int my_t = t0 + r / G, my_h = p.h * G + r % G;
+            const int pos = r < valid ? base + my_t : -1;
+            if (pl.two || w == 0) {
+                // the query row, in the K-major layout with 128-byte swizzle
+                const uint4 *src = reinterpret_cast<const uint4 *>(
+                    a.q + (int64_t)(p.s.q0 + (r < valid ? my_t : t0)) * a.q_ld +
+                    (int64_t)(r < valid ? my_h : 0) * HD);
+                uint8_t *dst = qs + sub * T::kQBytes + r * 128;
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i) {
+                    const uint4 x = r < valid ? src[i] : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(dst + (i >> 3) * (kBlock * 128) +
+                                               (((i & 7) ^ (r & 7)) << 4)) = x;
+                }
+                fence_proxy_async_smem();
+            }
+            mbar_arrive(&q_full);
+
+            float m = -INFINITY, l = 0.f;
+            bool first = true;
+            for (int i = T::kGroups == 2 ? w : 0; i < steps; i += T::kGroups) {
+                const int buf = i & 1, b = pl.block(i);
+                ok = ok && !*abort &&
+                     mbar_wait_or_abort(&s_full[buf], (s_phase >> buf) & 1u, abort, a.pb.err);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                s_phase ^= 1u << buf;
+                tc_fence_after();
+                const uint32_t sc = tmem + lanes + buf * 128;
+                float s[128];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    tmem_ld_32x32b_x32(sc + j * 32,
+                                       *reinterpret_cast<uint32_t(*)[32]>(s + j * 32));
+                tmem_ld_wait();
+                const int key0 = (p.lo + p.k0 + b) * kBlock;
+                if (key0 + kBlock - 1 > base + t0 || (a.window > 0 && key0 <= base + t1 - 1 - a.window)) {
+                    const int hi = pos - key0;
+                    const int lo = a.window > 0 ? hi - a.window + 1 : 0;
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (j > hi || j < lo) s[j] = -INFINITY;
+                }
+                float x[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int j = 4; j < 128; j += 8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[e] = j + 4 + e < 128 ? fmaxf(x[e], fmaxf(s[j + e], s[j + 4 + e]))
+                                               : fmaxf(x[e], s[j + e]);
+                }
+                const float mn = fmaxf(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+                // (m == -inf: the difference is +inf, or NaN when the row has no key yet)
+                if (__any_sync(0xffffffffu, (mn - m) * cs > 8.f)) {
+                    const float f = m == -INFINITY ? 0.f : ex2((m - mn) * cs);
+                    if (!first) {
+                        if (T::kGroups == 1) {
+                            // O still takes the last block's product: wait for it
+                            ok = mbar_wait_or_abort(&pv_done, (uint32_t)(pvs + i - 1) & 1u, abort,
+                                                    a.pb.err);
+                            ok = __all_sync(0xffffffffu, ok);
+                            tc_fence_after();
+                        }
+                        const uint32_t oc = tmem + lanes + T::kO + (T::kGroups == 2 ? w * HD : 0);
+#pragma unroll 1
+                        for (int j = 0; j < HD; j += 32) {
+                            uint32_t v[32];
+                            tmem_ld_32x32b_x32(oc + j, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            tmem_st_32x32b_x32(oc + j, v);
+                        }
+                    }
+                    l *= f;
+                    m = mn;
+                }
+                first = false;
+                const float z = m == -INFINITY ? 0.f : m * cs;
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float e0 = ex2(fmaf(s[j * 32 + 2 * e], cs, -z));
+                        const float e1 = ex2(fmaf(s[j * 32 + 2 * e + 1], cs, -z));
+                        sum[0] += e0;
+                        sum[1] += e1;
+                        // rounded to the cache's type: both factors of an MMA are of one type
+                        pk[e] = pack_t2<F16>(e0, e1);
+                    }
+                    tmem_st_32x32b_x16(sc + j * 16, pk);
+                }
+                l += sum[0] + sum[1];
+                if (key0 < key_lo || key0 + kBlock > key_hi) {
+                    // values of keys that no row sees may hold anything: a NaN times a
+                    // weight of 0 would reach the sum
+                    const int key = key0 + r;
+                    const bool clear = (!pl.two || w == 0) && (key < key_lo || key >= key_hi);
+#pragma unroll
+                    for (int u = 0; u < T::kUnits; ++u) {
+                        const int g = (loads + pl.value_load(b)) * T::kUnits + u;
+                        ok = ok && mbar_wait_or_abort(&full[g % T::kStages],
+                                                      (uint32_t)(g / T::kStages) & 1u, abort,
+                                                      a.pb.err);
+                        if (ok && clear) {
+                            uint8_t *v = ring + (g % T::kStages) * T::kUnitBytes + r * 128;
+#pragma unroll
+                            for (int j = 0; j < T::kUnitDims / 8; ++j)
+                                *reinterpret_cast<uint4 *>(v + (j >> 3) * (kBlock * 128) +
+                                                           (j & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&p_ready[buf]);
+            }
+            ok = ok && !*abort &&
+                 mbar_wait_or_abort(&o_full, (uint32_t)pieces & 1u, abort, a.pb.err);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            const uint32_t oc = tmem + lanes + T::kO + (T::kGroups == 2 ? w * HD : 0);
+            const bool whole = p.k0 == 0 && p.k1 == p.nb;
+            float f0 = 1.f, f1 = 0.f;
+            const float *other = reinterpret_cast<const float *>(smem) + r;
+            float M = m, L = l;
+            if (T::kGroups == 2 && !pl.two) {
+                // join the two warpgroups' sums: the second one's through the space of
+                // the query tiles ([dim][row]), which all products have read by now
+                if (w == 1) {
+                    float *x = reinterpret_cast<float *>(smem) + r;
+                    if (ok && steps > 1) {
+#pragma unroll 1
+                        for (int j = 0; j < HD; j += 32) {
+                            uint32_t v[32];
+                            tmem_ld_32x32b_x32(oc + j, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                x[(j + e) * kBlock] = __uint_as_float(v[e]);
+                        }
+                    }
+                    xm[r] = m;
+                    xl[r] = l;
+                }
+                bar_sync(1, 256);
+                if (w == 0) {
+                    const float m1 = xm[r];
+                    M = fmaxf(m, m1);
+                    f0 = m == -INFINITY ? 0.f : ex2((m - M) * cs);
+                    f1 = m1 == -INFINITY ? 0.f : ex2((m1 - M) * cs);
+                    L = l * f0 + xl[r] * f1;
+                }
+            }
+            if (ok && (pl.two || w == 0)) {
+                const float inv = L == 0.f ? 0.f : (whole ? 1.f / L : 1.f);
+                const bool join = T::kGroups == 2 && !pl.two && steps > 1;
+                const int slot = 2 * blockIdx.x + (p.k0 == 0 ? 1 : 0);
+                const int row = sub * tok * G + r;
+                uint16_t *op = a.out + (int64_t)(p.s.q0 + my_t) * a.out_ld + (int64_t)my_h * HD;
+                float *pp = a.part_o + ((int64_t)slot * T::kRows + row) * HD;
+#pragma unroll 1
+                for (int j = 0; j < HD; j += 32) {
+                    uint32_t v[32];
+                    __syncwarp();
+                    tmem_ld_32x32b_x32(oc + j, v);
+                    tmem_ld_wait();
+                    float y[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        y[e] = __uint_as_float(v[e]) * f0;
+                        if (join && f1 != 0.f) y[e] = fmaf(other[(j + e) * kBlock], f1, y[e]);
+                        // (rows without a key: whatever O holds)
+                        y[e] = L == 0.f ? 0.f : y[e] * inv;
+                    }
+                    if (r < valid) {
+                        if (whole) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint4 o;
+                                o.x = pack_t2<F16>(y[e], y[e + 1]);
+                                o.y = pack_t2<F16>(y[e + 2], y[e + 3]);
+                                o.z = pack_t2<F16>(y[e + 4], y[e + 5]);
+                                o.w = pack_t2<F16>(y[e + 6], y[e + 7]);
+                                *reinterpret_cast<uint4 *>(op + j + e) = o;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                *reinterpret_cast<float4 *>(pp + j + e) =
+                                    make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                        }
+                    }
+                }
+                if (!whole && r < valid)
+                    *reinterpret_cast<float2 *>(a.part_ml + ((int64_t)slot * T::kRows + row) * 2) =
+                        make_float2(M * cs, L);
+            }
+            if (!whole && p.k0 == 0) {
+                note_left = true;
+                if (threadIdx.x == 0)
+                    a.notes[blockIdx.x] = SplitNote{
+                        p.s.q0 + p.t0, p.h * G, p.t1 - p.t0,
+                        share_owner(sh.total, sh.n, unit + p.nb - 1) - (int)blockIdx.x + 1};
+            }
+            tc_fence_before();  // the next piece's products may overwrite S and O
+            if (T::kGroups == 2 && !pl.two) bar_sync(1, 256);  // `other` has been read
+            unit += p.k1 - p.k0;
+            loads += 2 * pl.n;
+            pvs += steps;
+            ++pieces;
+        }
+        if (threadIdx.x == 0 && !note_left) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == T::kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+template <int HD, bool F16>
+cudaError_t run_tiles(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
+                      cudaStream_t st) {
+    auto kern = paged_tiles_kernel<HD, F16>;
+    cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<HD>::kSmem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kern, dim3((unsigned)sm_count()), Tc<HD>::kThreads, Tc<HD>::kSmem, st, mk, mv,
+                      a);
+}
+
+}  // namespace
+
+int paged_tiles_rows(int head_dim) { return head_dim == 256 ? Tc<256>::kRows : Tc<128>::kRows; }
+
+cudaError_t launch_paged_tiles(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
+                               int hd, bool f16, cudaStream_t st) {
+    if (f16) {
+        if (hd == 64) return run_tiles<64, true>(a, mk, mv, st);
+        if (hd == 128) return run_tiles<128, true>(a, mk, mv, st);
+        return run_tiles<256, true>(a, mk, mv, st);
+    }
+    if (hd == 64) return run_tiles<64, false>(a, mk, mv, st);
+    if (hd == 128) return run_tiles<128, false>(a, mk, mv, st);
+    return run_tiles<256, false>(a, mk, mv, st);
+}
+
+}  // namespace nq

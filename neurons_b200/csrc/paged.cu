@@ -599,7 +599,7 @@ extern "C" {
 
 size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q) {
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads ||
-        (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        n_heads / n_kv_heads > 128 || max_q < 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return 0;
     return paged_attention_workspace(n_heads, n_kv_heads, head_dim, max_q);
 }
@@ -612,8 +612,8 @@ int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_pa
     const std::string what(fn);
     PagedAttnCall c{};
     if (int rc = check_batch(cache, batch, n_heads, fn, &c.pb)) return rc;
-    if (n_heads / cache->n_kv_heads > 16)
-        return fail(NQ_INVALID_INPUT, what + ": at most 16 query heads per key head");
+    if (n_heads / cache->n_kv_heads > 128)
+        return fail(NQ_INVALID_INPUT, what + ": at most 128 query heads per key head");
     if (!(scale > 0.f) || !std::isfinite(scale))
         return fail(NQ_INVALID_INPUT, what + ": scale must be positive and finite");
     if (window < 0) return fail(NQ_INVALID_INPUT, what + ": window must not be negative");

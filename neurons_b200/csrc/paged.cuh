@@ -8,6 +8,8 @@
 // q_starts[b] .. q_starts[b + 1] of q and stand at the sequence's end.
 #pragma once
 
+#include <cuda.h>
+
 #include "nq_common.cuh"
 
 namespace nq {
@@ -319,6 +321,11 @@ inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t max_q);
 cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st);
+
+// attn_paged_tc.cu: rows of its parts, and its launch (one CTA per SM)
+int paged_tiles_rows(int head_dim);
+cudaError_t launch_paged_tiles(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
+                               int hd, bool f16, cudaStream_t st);
 
 template <typename... P, typename... A>
 cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem,

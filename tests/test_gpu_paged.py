@@ -50,6 +50,11 @@ ATTENTION = {
     "chunk of 512": ([3000, 700], [512, 300], 8, 2, 128, 32, BF, 0),
     "prompt of 1000": ([1000], [1000], 14, 2, 64, 16, BF, 0),
     "prompt of 700 wide": ([700, 20], [700, 3], 4, 2, 256, 128, HF, 0),
+    "group of 32": ([300, 7], [1, 5], 32, 1, 64, 16, BF, 0),
+    "group of 128": ([150], [3], 128, 1, 128, 16, HF, 0),
+    "one tile of many blocks": ([9000], [30], 8, 2, 128, 64, BF, 0),
+    "tiles end in blocks": ([128, 129, 256, 257, 383, 64], [32, 33, 64, 65, 100, 64], 8, 2, 128, 128, BF, 0),
+    "many chunks": ([40 * i + 20 for i in range(40)], [i + 1 for i in range(40)], 8, 4, 64, 16, HF, 0),
     "chunk window": ([5000, 1500], [300, 700], 4, 2, 128, 16, HF, 700),
 }
 
