@@ -373,9 +373,11 @@ typedef struct nq_paged_batch {
  * selects the kernel and the workspace's size, results hold for any; 0:
  * unknown).  Softmax and sums in fp32; the weights are rounded to the cache's type
  * for the second product, the result once.  workspace: nq_paged_attention_
- * workspace_size() bytes for this max_q, 256-byte aligned, contents
- * irrelevant; two calls that overlap on the GPU need one each. */
-size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q);
+ * workspace_size() bytes for this max_q and max_keys = table_width *
+ * page_size (0 for short tables), 256-byte aligned, contents irrelevant; two
+ * calls that overlap on the GPU need one each. */
+size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q,
+                                         int64_t max_keys);
 int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_paged_cache_t *cache,
                        const nq_paged_batch_t *batch, int64_t max_q, float scale, int64_t window,
                        void *workspace, size_t workspace_bytes, uint16_t *out, int64_t out_ld,

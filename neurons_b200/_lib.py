@@ -47,7 +47,7 @@ SIGNATURES = {
                                   P, P, I, I, P, U64, P, P]),
     "nq_moe_switch_partial_push": (I, [P, I64, I64, I64, I64, I64, P, P, I64, I64, P, P, P, P, P, P,
                                        P, P, P, I, I, P, U64, P, P]),
-    "nq_paged_attention_workspace_size": (U64, [I, I, I, I64]),
+    "nq_paged_attention_workspace_size": (U64, [I, I, I, I64, I64]),
     "nq_paged_attention": (I, [P, I64, I, P, P, I64, F32, I64, P, U64, P, I64, P]),
     "nq_paged_append": (I, [P, I64, P, I64, P, I64, I, P, P, P, I, P, I64, P]),
     "nq_pages_free": (I, [P, P, I64, P]),

@@ -134,14 +134,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     __syncthreads();
     pdl_wait();  // lengths, tables, q and the cache come from earlier kernels
 
-    const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x, a.least);
+    const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x, a.least,
+                                        a.whole);
     Cursor c = sh.c;
     int64_t unit = sh.first;
     Piece p;
     int it = 0;  // blocks so far: stage it % kStages, parity it / kStages
 
     if (warp == kWarps) {
-        while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+        while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
             const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
             const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
             for (int k = p.k0; k < p.k1; ++k, ++it) {
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
     const int r0 = lane >> 2, cq = (lane & 3) * 2;   // rows r0, r0 + 8; columns cq, cq + 1 (+ 8)
     bool note_left = false;
-    while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+    while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
         const int valid = (p.t1 - p.t0) * G;
         const int base = p.s.len - p.s.n;            // position of the first new token
         const int p0 = base + p.t0, key_hi = base + p.t1;
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
         if (stop) break;  // one decision for all four warps
         unit += p.k1 - p.k0;
     }
-    if (warp == 0 && lane == 0 && !note_left) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
+    if (warp == 0 && lane == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
 }
 
 // Joins the parts of the tiles that several CTAs shared, in the CTAs' order:
@@ -447,23 +448,27 @@ int rows_grid(int hd) { return sm_count() * (hd == 256 ? Cfg<256>::kCtas : Cfg<1
 // Which kernel serves a call: paged_rows_kernel while a sequence's new tokens
 // make one tile of 16 rows, so that each key is read once; the tensor-core
 // kernel (128- or 256-row tiles) from there on.
+// A table that holds at most kWholeKeys keys per sequence leaves the tiles whole.
 struct Shape {
-    bool tiles;
+    bool tiles, whole;
     int grid, rows, block;  // CTAs, rows of a part, keys of a block
 };
 
-Shape shape_of(int n_heads, int n_kv, int hd, int64_t max_q) {
+constexpr int64_t kWholeKeys = 512;
+
+Shape shape_of(int n_heads, int n_kv, int hd, int64_t max_q, int64_t max_keys) {
     const int G = n_heads / n_kv;
-    if (max_q * G > kRows) return Shape{true, sm_count(), paged_tiles_rows(hd), 128};
-    return Shape{false, rows_grid(hd), kRows, kBlock};
+    const bool whole = max_keys <= kWholeKeys;
+    if (max_q * G > kRows) return Shape{true, whole, sm_count(), paged_tiles_rows(hd), 128};
+    return Shape{false, whole, rows_grid(hd), kRows, kBlock};
 }
 
 template <int HD, bool F16>
 cudaError_t run_rows(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
                      cudaStream_t st) {
     auto kern = paged_rows_kernel<HD, F16>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         Cfg<HD>::kSmem);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(kern, Cfg<HD>::kSmem, allowed);
     if (e != cudaSuccess) return e;
     return launch_pdl(kern, dim3((unsigned)rows_grid(HD)), kThreads, Cfg<HD>::kSmem, st, mk, mv, a);
 }
@@ -473,7 +478,7 @@ cudaError_t run_attention(const PagedAttnArgs &a, const CUtensorMap &mk, const C
                           const Shape &s, cudaStream_t st) {
     const cudaError_t e = s.tiles ? launch_paged_tiles(a, mk, mv, HD, F16, st)
                                   : run_rows<HD, F16>(a, mk, mv, st);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || s.whole) return e;
     return launch_pdl(paged_merge_kernel<HD, F16>, dim3((unsigned)s.grid, (unsigned)s.rows / 4),
                       128, 0, st, a, s.rows);
 }
@@ -496,13 +501,15 @@ void place_workspace(PagedAttnArgs &a, int grid, int rows, void *ws) {
 
 }  // namespace
 
-size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t max_q) {
-    const Shape s = shape_of(n_heads, n_kv, head_dim, max_q);
-    return part_bytes(s.grid, s.rows, head_dim);
+size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t max_q,
+                                 int64_t max_keys) {
+    const Shape s = shape_of(n_heads, n_kv, head_dim, max_q, max_keys);
+    return s.whole ? 0 : part_bytes(s.grid, s.rows, head_dim);
 }
 
 cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
-    const Shape s = shape_of(c.n_heads, c.n_kv, c.head_dim, c.max_q);
+    const Shape s = shape_of(c.n_heads, c.n_kv, c.head_dim, c.max_q,
+                             (int64_t)c.pb.table_width * c.pb.page_size);
     PagedAttnArgs a;
     a.pb = c.pb;
     a.q = c.q;
@@ -514,9 +521,10 @@ cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
     a.window = c.window;
     a.scale = c.scale;
     a.least = 1;
+    a.whole = s.whole;
     // the largest power of two that divides the page size: no box crosses a page
     a.box = std::min(s.block, c.pb.page_size & -c.pb.page_size);
-    place_workspace(a, s.grid, s.rows, c.ws);
+    if (!s.whole) place_workspace(a, s.grid, s.rows, c.ws);
     CUtensorMap mk, mv;
     if (!make_map_pages(&mk, c.f16, c.k, c.head_dim, c.pb.page_size, c.n_kv, c.pb.n_pages,
                         c.page_stride, a.box) ||

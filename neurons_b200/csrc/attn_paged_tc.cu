@@ -182,14 +182,15 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     const uint32_t tmem = tmem_holder;
     pdl_wait();  // lengths, tables, q and the cache come from earlier kernels
 
-    const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x, a.least);
+    const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x, a.least,
+                                        a.whole);
     Cursor c = sh.c;
     Piece p;
 
     if (warp == T::kLoadWarp) {
         int g = 0;  // stages filled so far
         bool ok = true;
-        while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+        while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
             const Plan<HD> pl(p, tok);
             const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
             const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 ok = ok && mbar_wait_or_abort(&full[g % T::kStages],
                                               (uint32_t)(g / T::kStages) & 1u, abort, a.pb.err);
             };
-            while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+            while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
                 const Plan<HD> pl(p, tok);
                 const int steps = pl.steps();
                 ok = mbar_wait_or_abort(&q_full, (uint32_t)pieces & 1u, abort, a.pb.err);
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         uint32_t s_phase = 0;
         int64_t unit = sh.first;
         bool ok = true, note_left = false;
-        while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, c, p)) {
+        while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
             const Plan<HD> pl(p, tok);
             const int steps = pl.steps();
             const int sub = pl.two ? w : 0;         // which query tile
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             pvs += steps;
             ++pieces;
         }
-        if (threadIdx.x == 0 && !note_left) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
+        if (threadIdx.x == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
     }
     tc_fence_before();
     __syncthreads();
@@ -551,8 +552,8 @@ template <int HD, bool F16>
 cudaError_t run_tiles(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
                       cudaStream_t st) {
     auto kern = paged_tiles_kernel<HD, F16>;
-    cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<HD>::kSmem);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(kern, Tc<HD>::kSmem, allowed);
     if (e != cudaSuccess) return e;
     return launch_pdl(kern, dim3((unsigned)sm_count()), Tc<HD>::kThreads, Tc<HD>::kSmem, st, mk, mv,
                       a);

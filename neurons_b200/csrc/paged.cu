@@ -597,11 +597,13 @@ using namespace nq;
 
 extern "C" {
 
-size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q) {
+size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q,
+                                         int64_t max_keys) {
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads ||
-        n_heads / n_kv_heads > 128 || max_q < 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        n_heads / n_kv_heads > 128 || max_q < 0 || max_keys < 0 ||
+        (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return 0;
-    return paged_attention_workspace(n_heads, n_kv_heads, head_dim, max_q);
+    return paged_attention_workspace(n_heads, n_kv_heads, head_dim, max_q, max_keys);
 }
 
 int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_paged_cache_t *cache,
@@ -623,9 +625,11 @@ int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_pa
     if (int rc = check_rows(out, out_ld, n_heads, cache->head_dim, fn, "out")) return rc;
     if (int rc = need_gpu(fn)) return rc;
     c.max_q = !batch->q_starts ? 1 : (max_q == 0 ? batch->n_tokens : max_q);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
-        workspace_bytes < paged_attention_workspace(n_heads, cache->n_kv_heads, cache->head_dim,
-                                                    c.max_q))
+    const size_t need =
+        paged_attention_workspace(n_heads, cache->n_kv_heads, cache->head_dim, c.max_q,
+                                  (int64_t)c.pb.table_width * c.pb.page_size);
+    if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+                     workspace_bytes < need))
         return fail(NQ_INVALID_INPUT,
                     what + ": workspace must be 256-byte aligned and hold "
                            "nq_paged_attention_workspace_size() bytes");

@@ -10,6 +10,8 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 #include "nq_common.cuh"
 
 namespace nq {
@@ -107,12 +109,15 @@ struct Cursor {
 // same head's keys at the same time.  CTA c of n takes the blocks
 // [c * total / n, (c + 1) * total / n), so that all CTAs get the same number
 // whatever the lengths are; a tile cut by such a border is finished by
-// merge_kernel.
+// paged_merge_kernel.  Where no sequence can be long (`whole`) a tile counts as
+// one and is never cut: no parts, and no merge.
 template <int BK>
-__device__ __forceinline__ int64_t entry_blocks_warp(const SeqView &s, int TT, int window) {
+__device__ __forceinline__ int64_t entry_blocks_warp(const SeqView &s, int TT, int window,
+                                                     bool whole) {
     // blocks of one head of this lane's entry; the lanes sum long entries together
     const int lane = threadIdx.x & 31;
     const int tiles = (s.n + TT - 1) / TT;
+    if (whole) return tiles;
     int64_t mine = 0;
     if (tiles == 1) mine = key_range<BK>(s, 0, s.n, window).nb;
     unsigned todo = __ballot_sync(0xffffffffu, tiles > 1);
@@ -168,14 +173,14 @@ __device__ __forceinline__ int share_owner(int64_t total, int n, int64_t u) {
 // Run by one whole warp.
 template <int BK>
 __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int TT, int window, int cta, int grid,
-                            int least) {
+                                            int least, bool whole) {
     const int lane = threadIdx.x & 31;
     Share sh;
     int64_t total = 0;
     for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
         SeqView s{0, 0, 0, 0};
         if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
-        total += entry_blocks_warp<BK>(s, TT, window);
+        total += entry_blocks_warp<BK>(s, TT, window, whole);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
@@ -190,7 +195,7 @@ __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int 
     for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
         SeqView s{0, 0, 0, 0};
         if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
-        const int64_t head = entry_blocks_warp<BK>(s, TT, window);
+        const int64_t head = entry_blocks_warp<BK>(s, TT, window, whole);
         const int64_t end = before + warp_inclusive(head * n_kv);
         const unsigned past = __ballot_sync(0xffffffffu, end > sh.first);
         if (past) {
@@ -209,7 +214,9 @@ __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int 
             int64_t seen = 0;
             for (int t0 = 0; t0 < tiles; t0 += 32) {
                 int64_t nb = 0;
-                if (t0 + lane < tiles)
+                if (whole)
+                    nb = t0 + lane < tiles;
+                else if (t0 + lane < tiles)
                     nb = key_range<BK>(c.s, (t0 + lane) * TT, min((t0 + lane + 1) * TT, c.s.n),
                                        window)
                              .nb;
@@ -243,7 +250,7 @@ struct Piece {
 // (Any thread: no warp-wide step.)
 template <int BK>
 __device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, int TT, int window,
-                                           Cursor &c, Piece &p) {
+                                           bool whole, Cursor &c, Piece &p) {
     if (c.left <= 0) return false;
     p.s = c.s;
     p.h = c.h;
@@ -254,8 +261,8 @@ __device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, int T
     p.lo = r.lo;
     p.nb = r.nb;
     p.k0 = c.off;
-    p.k1 = (int)min((int64_t)r.nb, c.off + c.left);
-    c.left -= p.k1 - p.k0;
+    p.k1 = whole ? r.nb : (int)min((int64_t)r.nb, c.off + c.left);
+    c.left -= whole ? 1 : p.k1 - p.k0;
     c.off = p.k1;
     if (p.k1 == r.nb && c.left > 0) {
         c.off = 0;
@@ -298,7 +305,8 @@ struct PagedAttnArgs {
     int64_t q_ld, out_ld;
     int n_heads, n_kv, window;
     int box;             // keys per TMA box
-    int least;           // fewest key blocks of a CTA's share
+    int least;           // fewest key blocks (tiles, when whole) of a CTA's share
+    bool whole;          // tiles are not cut
     float scale;
     SplitNote *notes;    // [CTAs]
     float *part_ml;      // [2 CTAs][rows][2]: maximum (times scale log2 e), sum
@@ -319,13 +327,29 @@ struct PagedAttnCall {
 
 inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t max_q);
+// max_keys: the longest sequence that the page table can hold
+size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t max_q,
+                                 int64_t max_keys);
 cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st);
 
 // attn_paged_tc.cu: rows of its parts, and its launch (one CTA per SM)
 int paged_tiles_rows(int head_dim);
 cudaError_t launch_paged_tiles(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
                                int hd, bool f16, cudaStream_t st);
+
+// Allows a kernel `bytes` of dynamic shared memory, once per device (`done`: a
+// bit per device, one word for each kernel).
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t> &done) {
+    int d = 0;
+    cudaError_t e = cudaGetDevice(&d);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (d & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 
 template <typename... P, typename... A>
 cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem,

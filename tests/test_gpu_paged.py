@@ -164,7 +164,7 @@ def test_bad_tables_read_nothing_and_tell(news):
 
 
 def test_python_refusals():
-    b = Batch([90, 30], [1, 1], 8, 2, 128, 16, BF, seed=11)
+    b = Batch([900, 30], [1, 1], 8, 2, 128, 16, BF, seed=11)  # (long enough for a workspace)
     ok = dict(q=b.q, k_pages=b.k, v_pages=b.v, table=b.table, kv_lens=b.row_lens)
     bad = [dict(q=b.q.half()), dict(q=b.q[:, :, :64]), dict(q=b.q.transpose(0, 1)),
            dict(q=b.q[:, :7]), dict(k_pages=b.k.float(), v_pages=b.v.float()),
@@ -187,7 +187,7 @@ def test_attention_on_a_stream_and_in_a_graph(news):
     with a workspace each do not disturb one another."""
     b = Batch([400, 900, 200], news, 8, 2, 128, 16, BF, seed=12)
     want = b.call(nb, max_q=max(news)).clone()
-    size = nb.paged_attention_workspace_size(8, 2, 128, max(news))
+    size = nb.paged_attention_workspace_size(8, 2, 128, max(news), b.table.shape[1] * 16)
     ws = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
     outs = [torch.zeros_like(want) for _ in range(2)]
     s = torch.cuda.Stream()

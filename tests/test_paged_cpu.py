@@ -94,9 +94,10 @@ def test_empty_batches_are_no_ops(nqlib):
 
 
 def test_workspace_size_of_bad_shapes_is_zero(nqlib):
-    assert nqlib.nq_paged_attention_workspace_size(5, 2, 64, 1) == 0
-    assert nqlib.nq_paged_attention_workspace_size(4, 2, 80, 1) == 0
-    assert nqlib.nq_paged_attention_workspace_size(4, 2, 64, 1) > 0
+    size = nqlib.nq_paged_attention_workspace_size
+    assert size(5, 2, 64, 1, 4096) == size(4, 2, 80, 1, 4096) == size(4, 2, 64, -1, 4096) == 0
+    assert size(4, 2, 64, 1, 64) == 0  # short tables need none
+    assert size(4, 2, 64, 1, 4096) > 0
     assert nqlib.nq_pages_workspace_size(-1, 0) == 0
     assert nqlib.nq_pages_workspace_size(0, 0) > 0
 
