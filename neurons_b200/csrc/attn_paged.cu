@@ -6,14 +6,17 @@
 // over the keys j <= pos(t) = len - n + t (and j > pos(t) - window), G query
 // heads per key head.
 //
-// A tile is 16 rows: the G query heads of a key head times 16 / G tokens, the
-// M of an m16n8k16 MMA, so that each key and value is read from memory once
-// for all of them.  The call's key blocks (64 keys) are dealt out evenly over
-// the CTAs (paged.cuh); per CTA one warp brings blocks into a ring of
-// shared-memory stages by TMA (16- to 64-row boxes, as the page size allows),
-// and four warps take 16 keys of each block: S = Q K^T, a running maximum and
-// sum per row, O += P V, all in registers, without a barrier between the
-// warps until the tile's end.
+// A tile is up to 8 or 16 rows: the G query heads of a key head times as many
+// tokens as fit, so that each key and value is read from memory once for all of
+// them.  The products are taken transposed, S^T = K Q^T and O^T += V^T P^T, with
+// the keys (and dims) as the 16 rows of m16n8k16 and the query rows as its 8
+// columns: a decode step with G <= 8 pays half of the MMAs and registers that
+// 16 query rows would cost.  The call's key blocks (64 keys) are dealt out
+// evenly over the CTAs (paged.cuh); per CTA one warp brings blocks into a ring
+// of shared-memory stages by TMA (16- to 64-row boxes, as the page size
+// allows), and four warps take 16 keys of each block, with a running maximum
+// and sum of their own, all in registers, without a barrier between the warps
+// until the tile's end.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -26,21 +29,21 @@
 namespace nq {
 namespace {
 
-constexpr int kRows = 16;          // query rows per tile
 constexpr int kBlock = 64;         // keys per block
 constexpr int kWarps = 4;          // consumer warps, 16 keys of a block each
 constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kRows = 16;          // query rows of a tile at most (8 NT)
 
 template <int HD>
 struct Cfg {
     static constexpr int kTileBytes = kBlock * HD * 2;   // keys (or values) of a block
     static constexpr int kStageBytes = 2 * kTileBytes;
-    // two CTAs per SM at 64 and 128 dims, one at 256: 96 to 128 KB of loads in
-    // flight per SM, where 6.5 TB/s and about 1 us of latency ask for 44 KB
-    static constexpr int kStages = HD == 64 ? 5 : (HD == 128 ? 3 : 2);
-    static constexpr int kRedBytes = 2 * kRows * HD * 4;  // two warps' O at a tile's end
+    // 128 to 192 KB of loads in flight per SM, where 6.5 TB/s and about 1 us of
+    // latency ask for 44 KB
+    static constexpr int kCtas = HD == 64 ? 3 : (HD == 128 ? 2 : 1);  // per SM
+    static constexpr int kStages = HD == 64 ? 4 : (HD == 128 ? 3 : 2);
+    static constexpr int kRedBytes = kWarps * 8 * HD * 4;  // the warps' O of 8 rows
     static constexpr int kSmem = kStages * kStageBytes + kRedBytes;
-    static constexpr int kCtas = HD == 256 ? 1 : 2;  // per SM
 };
 
 template <bool F16>
@@ -71,6 +74,13 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(addr)
                  : "memory");
+}
+
+// transposes an 8 x 8 matrix of 16-bit values held two per lane
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -106,19 +116,43 @@ __device__ __forceinline__ void load_block(const PagedBatch &pb, const CUtensorM
                     is_v ? mv : mk, bar, col * 64, slot, p.h, page);
 }
 
-template <int HD, bool F16>
+// Q^T as the MMAs' second operand: lane l holds query row l / 4 (+ 8), dims
+// (l % 4) * 2 + {0, 1} (+ 8) of each 16.
+template <int HD, int NT>
+__device__ __forceinline__ void load_q(const PagedAttnArgs &a, const Piece &p, int G,
+                                       uint32_t (&q)[HD / 16][NT][2]) {
+    const int lane = threadIdx.x & 31;
+    const int valid = (p.t1 - p.t0) * G;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + (lane >> 2);
+        const bool in = r < valid;
+        const uint16_t *src = a.q + (int64_t)(p.s.q0 + p.t0 + (in ? r / G : 0)) * a.q_ld +
+                              (int64_t)(p.h * G + (in ? r % G : 0)) * HD + (lane & 3) * 2;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+            q[k][nt][0] = in ? *reinterpret_cast<const uint32_t *>(src + k * 16) : 0u;
+            q[k][nt][1] = in ? *reinterpret_cast<const uint32_t *>(src + k * 16 + 8) : 0u;
+        }
+    }
+}
+
+template <int HD, bool F16, int NT>
 __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
     const PagedAttnArgs a) {
     using C = Cfg<HD>;
+    // the next tile's queries are loaded while this one's keys are worked on,
+    // where registers allow
+    constexpr bool kAhead = HD / 16 * NT <= 8;
     extern __shared__ __align__(1024) uint8_t smem[];  // (the swizzle's period)
     float *red = reinterpret_cast<float *>(smem + C::kStages * C::kStageBytes);
     __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
-    __shared__ float wm[kWarps][kRows], wl[kWarps][kRows];
+    __shared__ float wm[kWarps][8 * NT], wl[kWarps][8 * NT];
     __shared__ int abort_flag, stop;
     volatile int *abort = &abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = a.n_heads / a.n_kv, TT = kRows / G;
+    const int G = a.n_heads / a.n_kv, TT = 8 * NT / G;
 
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
@@ -167,35 +201,52 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     }
 
     const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
-    const int r0 = lane >> 2, cq = (lane & 3) * 2;   // rows r0, r0 + 8; columns cq, cq + 1 (+ 8)
+    const int kr = lane >> 2, cq = (lane & 3) * 2;   // keys kr, kr + 8; rows cq, cq + 1 (+ 8 nt)
     bool note_left = false;
-    while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
+    uint32_t q[HD / 16][NT][2], qn[kAhead ? HD / 16 : 1][NT][2];
+    Piece pn;
+    bool more = next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, pn);
+    if constexpr (kAhead) {
+        if (more) load_q<HD, NT>(a, pn, G, qn);
+    }
+    while (more) {
+        p = pn;
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) q[k][nt][e] = qn[k][nt][e];
+        } else {
+            load_q<HD, NT>(a, p, G, q);
+        }
+        more = next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, pn);
+        if constexpr (kAhead) {
+            if (more) load_q<HD, NT>(a, pn, G, qn);
+        }
         const int valid = (p.t1 - p.t0) * G;
         const int base = p.s.len - p.s.n;            // position of the first new token
         const int p0 = base + p.t0, key_hi = base + p.t1;
         const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
-        int pos[2];
-        uint32_t qf[HD / 16][4];
+        int pos[NT][2];
+        float m[NT][2], l[NT][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 8 * i;
-            const bool in = r < valid;
-            const int t = p.t0 + (in ? r / G : 0);
-            pos[i] = in ? base + t : -1;
-            const uint16_t *qp =
-                a.q + (int64_t)(p.s.q0 + t) * a.q_ld + (int64_t)(p.h * G + (in ? r % G : 0)) * HD;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                qf[k][i] = in ? *reinterpret_cast<const uint32_t *>(qp + k * 16 + cq) : 0u;
-                qf[k][i + 2] = in ? *reinterpret_cast<const uint32_t *>(qp + k * 16 + cq + 8) : 0u;
+            for (int e = 0; e < 2; ++e) {
+                const int r = nt * 8 + cq + e;
+                pos[nt][e] = r < valid ? p0 + r / G : -1;
+                m[nt][e] = -INFINITY;
+                l[nt][e] = 0.f;
             }
-        }
-        float o[HD / 8][4];
+        float o[HD / 16][NT][4];
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n)
+        for (int t = 0; t < HD / 16; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[n][j] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[t][nt][j] = 0.f;
 
         for (int k = p.k0; k < p.k1; ++k, ++it) {
             const int st = it % C::kStages;
@@ -206,32 +257,39 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
             if (key0 < key_hi && key0 + 16 > key_lo) {
                 uint8_t *ks = smem + st * C::kStageBytes + warp * 16 * 128;
                 uint8_t *vs = ks + C::kTileBytes;
-                float s[2][4];
+                // two chains of sums over the dims, so that an MMA waits for the last
+                // but one
+                float s[NT][4], s2[NT][4];
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+                    for (int j = 0; j < 4; ++j) s[nt][j] = s2[nt][j] = 0.f;
                 {
-                    // matrices: keys 0-7 / dims 0-7, keys 0-7 / dims 8-15, then keys 8-15
-                    const int row = (lane & 7) + ((lane >> 4) << 3);
+                    // matrices: keys 0-7 / dims 0-7, keys 8-15 / dims 0-7, then dims 8-15
+                    const int row = lane & 15;
                     const uint32_t rowa = smem_u32(ks) + row * 128;
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
-                        const int ch = (kk & 3) * 2 + ((lane >> 3) & 1);
-                        uint32_t b[4];
-                        ldsm4(b, rowa + (kk >> 2) * (kBlock * 128) + ((ch ^ (row & 7)) << 4));
-                        mma16816<F16>(s[0], qf[kk], b[0], b[1]);
-                        mma16816<F16>(s[1], qf[kk], b[2], b[3]);
+                        const int ch = (kk & 3) * 2 + (lane >> 4);
+                        uint32_t f[4];
+                        ldsm4(f, rowa + (kk >> 2) * (kBlock * 128) + ((ch ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16816<F16>((kk & 1) ? s2[nt] : s[nt], f, q[kk][nt][0], q[kk][nt][1]);
                     }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[nt][j] += s2[nt][j];
                 }
                 if (key0 + 15 > p0 || (a.window > 0 && key0 <= key_hi - 1 - a.window)) {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int key = key0 + n * 8 + cq + (j & 1), ps = pos[j >> 1];
+                            const int key = key0 + kr + (j >> 1) * 8, ps = pos[nt][j & 1];
                             if (key > ps || (a.window > 0 && key <= ps - a.window))
-                                s[n][j] = -INFINITY;
+                                s[nt][j] = -INFINITY;
                         }
                 }
                 if (key0 < key_lo || key0 + 16 > key_hi) {
@@ -247,56 +305,65 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                     }
                     __syncwarp();
                 }
-                // running maximum and sum of rows r0 and r0 + 8, in fp32
-                float mn[2];
+                // Running maximum and sum of each row (a column here), in fp32.  The
+                // maximum follows only when a score has passed it by 2^8 (or the row has
+                // none yet): until then weights up to 2^8 do no harm, and the warp is
+                // spared the maximum over its lanes.
+                bool grow = false;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float x = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]),
-                                    fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                    mn[i] = fmaxf(m[i], x);
-                }
-                if (__any_sync(0xffffffffu, mn[0] > m[0] || mn[1] > m[1])) {
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float f = m[i] == -INFINITY ? 0.f : ex2((m[i] - mn[i]) * cs);
-                        l[i] *= f;
+                    for (int e = 0; e < 2; ++e)
+                        grow |= (fmaxf(s[nt][e], s[nt][e + 2]) - m[nt][e]) * cs > 8.f;
+                if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                        for (int n = 0; n < HD / 8; ++n) {
-                            o[n][2 * i] *= f;
-                            o[n][2 * i + 1] *= f;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float x = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1)
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                            x = fmaxf(x, m[nt][e]);
+                            const float f =
+                                m[nt][e] == -INFINITY ? 0.f : ex2((m[nt][e] - x) * cs);
+                            m[nt][e] = x;
+                            l[nt][e] *= f;
+#pragma unroll
+                            for (int t = 0; t < HD / 16; ++t) {
+                                o[t][nt][e] *= f;
+                                o[t][nt][e + 2] *= f;
+                            }
                         }
-                        m[i] = mn[i];
+                }
+                uint32_t pf[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float z = m[nt][e] == -INFINITY ? 0.f : m[nt][e] * cs;
+                        w[e] = ex2(fmaf(s[nt][e], cs, -z));
+                        w[e + 2] = ex2(fmaf(s[nt][e + 2], cs, -z));
+                        l[nt][e] += w[e] + w[e + 2];
                     }
-                }
-                uint32_t pf[4];
-                {
-                    const float z[2] = {m[0] == -INFINITY ? 0.f : m[0] * cs,
-                                        m[1] == -INFINITY ? 0.f : m[1] * cs};
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float e0 = ex2(fmaf(s[n][2 * i], cs, -z[i]));
-                            const float e1 = ex2(fmaf(s[n][2 * i + 1], cs, -z[i]));
-                            l[i] += e0 + e1;
-                            // the weights are rounded to the cache's type, as the
-                            // tensor cores take both factors in one type
-                            pf[n * 2 + i] = pack_t2<F16>(e0, e1);
-                        }
+                    // the weights are rounded to the cache's type, as the tensor cores
+                    // take both factors in one type
+                    pf[nt][0] = transpose8(pack_t2<F16>(w[0], w[1]));
+                    pf[nt][1] = transpose8(pack_t2<F16>(w[2], w[3]));
                 }
                 {
-                    // matrices: keys 0-7 and 8-15 of dims 0-7, then of dims 8-15
-                    const int row = lane & 15;
+                    // matrices: dims 0-7 / keys 0-7, dims 8-15 / keys 0-7, then keys 8-15
+                    const int row = (lane & 7) + ((lane >> 4) << 3);
                     const uint32_t rowa = smem_u32(vs) + row * 128;
 #pragma unroll
-                    for (int n = 0; n < HD / 16; ++n) {
-                        const int ch = (n & 3) * 2 + (lane >> 4);
-                        uint32_t b[4];
-                        ldsm4_t(b, rowa + (n >> 2) * (kBlock * 128) + ((ch ^ (row & 7)) << 4));
-                        mma16816<F16>(o[2 * n], pf, b[0], b[1]);
-                        mma16816<F16>(o[2 * n + 1], pf, b[2], b[3]);
+                    for (int t = 0; t < HD / 16; ++t) {
+                        const int ch = (t & 3) * 2 + ((lane >> 3) & 1);
+                        uint32_t f[4];
+                        ldsm4_t(f, rowa + (t >> 2) * (kBlock * 128) + ((ch ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16816<F16>(o[t][nt], f, pf[nt][0], pf[nt][1]);
                     }
                 }
                 if (key0 < key_lo || key0 + 16 > key_hi) fence_proxy_async_smem();
@@ -307,77 +374,76 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
 
         // the four warps' sums, one after another in a fixed order
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-            if ((lane & 3) == 0) {
-                wm[warp][r0 + 8 * i] = m[i];
-                wl[warp][r0 + 8 * i] = l[i];
-            }
-        }
-        bar_sync(1, kWarps * 32);
-        float M[2], L[2];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 8 * i;
-            M[i] = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-            L[i] = 0.f;
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-                L[i] += wm[w][r] == -INFINITY ? 0.f : wl[w][r] * ex2((wm[w][r] - M[i]) * cs);
-            const float f = m[i] == -INFINITY ? 0.f : ex2((m[i] - M[i]) * cs);
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n) {
-                o[n][2 * i] *= f;
-                o[n][2 * i + 1] *= f;
-            }
-        }
-        float *mine = red + (warp & 1) * (kRows * HD);
-        if (warp >= 2) {
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mine[(n * 4 + j) * 32 + lane] = o[n][j];
-        }
-        bar_sync(1, kWarps * 32);
-        if (warp < 2) {
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    o[n][j] += mine[(n * 4 + j) * 32 + lane];
-                    if (warp == 1) mine[(n * 4 + j) * 32 + lane] = o[n][j];
+                for (int d = 4; d < 32; d <<= 1)
+                    l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
+                if (lane < 4) {
+                    wm[warp][nt * 8 + cq + e] = m[nt][e];
+                    wl[warp][nt * 8 + cq + e] = l[nt][e];
                 }
-        }
+            }
         bar_sync(1, kWarps * 32);
-        if (warp == 0) {
-            const float *other = red + kRows * HD;
-            const bool whole = p.k0 == 0 && p.k1 == p.nb;
-            const int slot = 2 * blockIdx.x + (p.k0 == 0 ? 1 : 0);
+        const bool uncut = p.k0 == 0 && p.k1 == p.nb;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = r0 + 8 * i;
+        for (int nt = 0; nt < NT; ++nt) {
+            if (nt > 0) bar_sync(1, kWarps * 32);  // (the last rows have been read)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = nt * 8 + cq + e;
+                const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+                const float f = m[nt][e] == -INFINITY ? 0.f : ex2((m[nt][e] - M) * cs);
+                // [warp][row][dim], the dims swizzled so that neither side has bank conflicts
+                float *dst = red + (warp * 8 + cq + e) * HD;
+                const int sw = (cq >> 1) * 8;
+#pragma unroll
+                for (int t = 0; t < HD / 16; ++t) {
+                    dst[(t * 16 + kr) ^ sw] = o[t][nt][e] * f;
+                    dst[(t * 16 + 8 + kr) ^ sw] = o[t][nt][e + 2] * f;
+                }
+            }
+            bar_sync(1, kWarps * 32);
+            for (int i = threadIdx.x; i < HD; i += kWarps * 32) {  // 8 rows x HD / 8 pieces
+                const int rr = i / (HD / 8), d0 = i % (HD / 8) * 8, r = nt * 8 + rr;
                 if (r >= valid) continue;
-                const float f = whole ? (L[i] == 0.f ? 0.f : 1.f / L[i]) : 1.f;
-                uint16_t *op = a.out + (int64_t)(p.s.q0 + p.t0 + r / G) * a.out_ld +
-                               (int64_t)(p.h * G + r % G) * HD;
-                float *pp = a.part_o + ((int64_t)slot * kRows + r) * HD;
+                float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, L = 0.f;
+                const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
 #pragma unroll
-                for (int n = 0; n < HD / 8; ++n) {
-                    const float x = (o[n][2 * i] + other[(n * 4 + 2 * i) * 32 + lane]) * f;
-                    const float y = (o[n][2 * i + 1] + other[(n * 4 + 2 * i + 1) * 32 + lane]) * f;
-                    if (whole)
-                        *reinterpret_cast<uint32_t *>(op + n * 8 + cq) = pack_t2<F16>(x, y);
-                    else
-                        *reinterpret_cast<float2 *>(pp + n * 8 + cq) = make_float2(x, y);
+                for (int w = 0; w < kWarps; ++w) {
+                    L += wm[w][r] == -INFINITY ? 0.f : wl[w][r] * ex2((wm[w][r] - M) * cs);
+                    const float *src = red + (w * 8 + rr) * HD + (d0 ^ (rr >> 1) * 8);
+                    const float4 u = *reinterpret_cast<const float4 *>(src);
+                    const float4 v = *reinterpret_cast<const float4 *>(src + 4);
+                    y[0] += u.x;
+                    y[1] += u.y;
+                    y[2] += u.z;
+                    y[3] += u.w;
+                    y[4] += v.x;
+                    y[5] += v.y;
+                    y[6] += v.z;
+                    y[7] += v.w;
                 }
-                if (!whole && (lane & 3) == 0) {
-                    float *ml = a.part_ml + ((int64_t)slot * kRows + r) * 2;
-                    ml[0] = M[i] * cs;
-                    ml[1] = L[i];
+                if (uncut) {
+                    const float f = L == 0.f ? 0.f : 1.f / L;
+                    const uint4 v = make_uint4(
+                        pack_t2<F16>(y[0] * f, y[1] * f), pack_t2<F16>(y[2] * f, y[3] * f),
+                        pack_t2<F16>(y[4] * f, y[5] * f), pack_t2<F16>(y[6] * f, y[7] * f));
+                    *reinterpret_cast<uint4 *>(a.out + (int64_t)(p.s.q0 + p.t0 + r / G) * a.out_ld +
+                                               (int64_t)(p.h * G + r % G) * HD + d0) = v;
+                } else {
+                    const int64_t row = (int64_t)(2 * blockIdx.x + (p.k0 == 0 ? 1 : 0)) * kRows + r;
+                    float4 *dst = reinterpret_cast<float4 *>(a.part_o + row * HD + d0);
+                    dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+                    dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+                    if (d0 == 0)
+                        *reinterpret_cast<float2 *>(a.part_ml + row * 2) = make_float2(M * cs, L);
                 }
             }
-            if (!whole && p.k0 == 0) {
+        }
+        if (warp == 0) {
+            if (!uncut && p.k0 == 0) {
                 note_left = true;
                 if (lane == 0)
                     a.notes[blockIdx.x] = SplitNote{
@@ -393,16 +459,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     if (warp == 0 && lane == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
 }
 
-// Joins the parts of the tiles that several CTAs shared, in the CTAs' order:
-// one warp per query row.
-template <int HD, bool F16>
+// Joins the parts of the tiles that several CTAs shared, in the CTAs' order.
+// W warps take the parts of a query row in turn: one where a tile has few parts
+// and many rows, four where a decode step has few rows in many parts.
+template <int HD, bool F16, int W>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a, int rows) {
     pdl_launch_dependents();
     pdl_wait();
+    __shared__ float sums[W == 1 ? 1 : 4][HD + 1];
     const SplitNote note = a.notes[blockIdx.x];
     if (note.parts == 0) return;
     const int G = a.n_heads / a.n_kv;
-    const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = W == 1 ? blockIdx.y * 4 + warp : blockIdx.y;
+    const int first = W == 1 ? 0 : warp;
     if (r >= note.tokens * G) return;
     constexpr int kPer = HD / 32;
     auto slot = [&](int i) -> int64_t {
@@ -419,7 +489,7 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 #pragma unroll
     for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
 #pragma unroll 4
-    for (int i = 0; i < note.parts; ++i) {
+    for (int i = first; i < note.parts; i += W) {
         const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + slot(i) * 2);
         const float *po = a.part_o + slot(i) * HD + lane * kPer;
         float v[kPer];
@@ -434,6 +504,22 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 #pragma unroll
         for (int j = 0; j < kPer; ++j) acc[j] = fmaf(v[j], f, acc[j]);
     }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) sums[warp][lane * kPer + j] = acc[j];
+        if (lane == 0) sums[warp][HD] = L;
+        __syncthreads();
+        if (warp > 0) return;
+        L = 0.f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            L += sums[w][HD];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) acc[j] += sums[w][lane * kPer + j];
+        }
+    }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     uint16_t *op = a.out + (int64_t)(note.q_row + r / G) * a.out_ld +
                    (int64_t)(note.heads0 + r % G) * HD + lane * kPer;
@@ -443,7 +529,10 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 }
 
 // CTAs of paged_rows_kernel: as many as fit at once
-int rows_grid(int hd) { return sm_count() * (hd == 256 ? Cfg<256>::kCtas : Cfg<128>::kCtas); }
+int rows_grid(int hd) {
+    return sm_count() *
+           (hd == 64 ? Cfg<64>::kCtas : (hd == 128 ? Cfg<128>::kCtas : Cfg<256>::kCtas));
+}
 
 // Which kernel serves a call: paged_rows_kernel while a sequence's new tokens
 // make one tile of 16 rows, so that each key is read once; the tensor-core
@@ -463,10 +552,10 @@ Shape shape_of(int n_heads, int n_kv, int hd, int64_t max_q, int64_t max_keys) {
     return Shape{false, whole, rows_grid(hd), kRows, kBlock};
 }
 
-template <int HD, bool F16>
+template <int HD, bool F16, int NT>
 cudaError_t run_rows(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
                      cudaStream_t st) {
-    auto kern = paged_rows_kernel<HD, F16>;
+    auto kern = paged_rows_kernel<HD, F16, NT>;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(kern, Cfg<HD>::kSmem, allowed);
     if (e != cudaSuccess) return e;
@@ -475,11 +564,16 @@ cudaError_t run_rows(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtens
 
 template <int HD, bool F16>
 cudaError_t run_attention(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
-                          const Shape &s, cudaStream_t st) {
-    const cudaError_t e = s.tiles ? launch_paged_tiles(a, mk, mv, HD, F16, st)
-                                  : run_rows<HD, F16>(a, mk, mv, st);
+                          const Shape &s, int64_t rows, cudaStream_t st) {
+    const cudaError_t e = s.tiles     ? launch_paged_tiles(a, mk, mv, HD, F16, st)
+                          : rows <= 8 ? run_rows<HD, F16, 1>(a, mk, mv, st)
+                                      : run_rows<HD, F16, 2>(a, mk, mv, st);
     if (e != cudaSuccess || s.whole) return e;
-    return launch_pdl(paged_merge_kernel<HD, F16>, dim3((unsigned)s.grid, (unsigned)s.rows / 4),
+    if (s.tiles)
+        return launch_pdl(paged_merge_kernel<HD, F16, 1>,
+                          dim3((unsigned)s.grid, (unsigned)s.rows / 4), 128, 0, st, a, s.rows);
+    // (a caller's max_q may be too small: every row of a tile has its CTA)
+    return launch_pdl(paged_merge_kernel<HD, F16, 4>, dim3((unsigned)s.grid, rows <= 8 ? 8u : 16u),
                       128, 0, st, a, s.rows);
 }
 
@@ -510,6 +604,7 @@ size_t paged_attention_workspace(int n_heads, int n_kv, int head_dim, int64_t ma
 cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
     const Shape s = shape_of(c.n_heads, c.n_kv, c.head_dim, c.max_q,
                              (int64_t)c.pb.table_width * c.pb.page_size);
+    const int64_t rows = c.max_q * (c.n_heads / c.n_kv);
     PagedAttnArgs a;
     a.pb = c.pb;
     a.q = c.q;
@@ -532,13 +627,13 @@ cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
                         c.page_stride, a.box))
         return cudaErrorInvalidValue;
     if (c.f16) {
-        if (c.head_dim == 64) return run_attention<64, true>(a, mk, mv, s, st);
-        if (c.head_dim == 128) return run_attention<128, true>(a, mk, mv, s, st);
-        return run_attention<256, true>(a, mk, mv, s, st);
+        if (c.head_dim == 64) return run_attention<64, true>(a, mk, mv, s, rows, st);
+        if (c.head_dim == 128) return run_attention<128, true>(a, mk, mv, s, rows, st);
+        return run_attention<256, true>(a, mk, mv, s, rows, st);
     }
-    if (c.head_dim == 64) return run_attention<64, false>(a, mk, mv, s, st);
-    if (c.head_dim == 128) return run_attention<128, false>(a, mk, mv, s, st);
-    return run_attention<256, false>(a, mk, mv, s, st);
+    if (c.head_dim == 64) return run_attention<64, false>(a, mk, mv, s, rows, st);
+    if (c.head_dim == 128) return run_attention<128, false>(a, mk, mv, s, rows, st);
+    return run_attention<256, false>(a, mk, mv, s, rows, st);
 }
 
 }  // namespace nq
