@@ -90,19 +90,20 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Loads key block `blk` (keys and values) of a piece into one stage: boxes of
-// `box` keys x 64 dims, one lane each.  Boxes without a visible key of the
-// piece read as zeros through a coordinate outside of the tensor (their pages
-// need not exist).
+// `box` keys x all dims (as columns of 64 dims, one after another), one lane
+// each.  An SM starts a box about every 40 ns, which is why they are as large
+// as the page size allows (64 keys: 0.6 us, 16 keys x 64 dims: 1.05 us a block
+// where one CTA works alone).  Boxes without a visible key of the piece read as
+// zeros through a coordinate outside of the tensor (their pages need not
+// exist).
 template <int HD>
 __device__ __forceinline__ void load_block(const PagedBatch &pb, const CUtensorMap *mk,
                                            const CUtensorMap *mv, const Piece &p, int blk, int box,
                                            int key_lo, int key_hi, uint8_t *stage, uint64_t *bar) {
-    constexpr int kCols = HD / 64;
     const int lane = threadIdx.x & 31;
-    const int per = kBlock / box * kCols;  // boxes of the keys; as many of the values
+    const int per = kBlock / box;  // boxes of the keys; as many of the values
     const bool is_v = lane >= per;
-    const int i = is_v ? lane - per : lane;
-    const int r = i / kCols, col = i % kCols;
+    const int r = is_v ? lane - per : lane;
     const int key = blk * kBlock + r * box;
     int page = pb.n_pages, slot = 0;
     if (lane < 2 * per && key < key_hi && key + box > key_lo) {
@@ -112,8 +113,8 @@ __device__ __forceinline__ void load_block(const PagedBatch &pb, const CUtensorM
     if (lane == 0) mbar_expect_tx(bar, Cfg<HD>::kStageBytes);
     __syncwarp();
     if (lane < 2 * per)
-        tma_load_4d(stage + (is_v ? Cfg<HD>::kTileBytes : 0) + col * (kBlock * 128) + r * box * 128,
-                    is_v ? mv : mk, bar, col * 64, slot, p.h, page);
+        tma_load_5d(stage + (is_v ? Cfg<HD>::kTileBytes : 0) + r * box * HD * 2, is_v ? mv : mk, bar,
+                    0, slot, 0, p.h, page);
 }
 
 // Q^T as the MMAs' second operand: lane l holds query row l / 4 (+ 8), dims
@@ -202,6 +203,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
 
     const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
     const int kr = lane >> 2, cq = (lane & 3) * 2;   // keys kr, kr + 8; rows cq, cq + 1 (+ 8 nt)
+    // this warp's 16 keys in a stage, and the distance of the columns of 64 dims
+    const int key_at = warp * 16 / a.box * a.box * (HD * 2) + warp * 16 % a.box * 128;
+    const int col_ld = a.box * 128;
     bool note_left = false;
     uint32_t q[HD / 16][NT][2], qn[kAhead ? HD / 16 : 1][NT][2];
     Piece pn;
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
             if (!mbar_wait_or_abort(&full[st], (uint32_t)(it / C::kStages) & 1u, abort, a.pb.err))
                 break;
             if (key0 < key_hi && key0 + 16 > key_lo) {
-                uint8_t *ks = smem + st * C::kStageBytes + warp * 16 * 128;
+                uint8_t *ks = smem + st * C::kStageBytes + key_at;
                 uint8_t *vs = ks + C::kTileBytes;
                 // two chains of sums over the dims, so that an MMA waits for the last
                 // but one
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                     for (int kk = 0; kk < HD / 16; ++kk) {
                         const int ch = (kk & 3) * 2 + (lane >> 4);
                         uint32_t f[4];
-                        ldsm4(f, rowa + (kk >> 2) * (kBlock * 128) + ((ch ^ (row & 7)) << 4));
+                        ldsm4(f, rowa + (kk >> 2) * col_ld + ((ch ^ (row & 7)) << 4));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
                             mma16816<F16>((kk & 1) ? s2[nt] : s[nt], f, q[kk][nt][0], q[kk][nt][1]);
@@ -300,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                         const int row = i & 15, cc = i >> 4;
                         const int key = key0 + row;
                         if (key < key_lo || key >= key_hi)
-                            *reinterpret_cast<uint4 *>(vs + (cc >> 3) * (kBlock * 128) + row * 128 +
+                            *reinterpret_cast<uint4 *>(vs + (cc >> 3) * col_ld + row * 128 +
                                                        (cc & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     __syncwarp();
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                     for (int t = 0; t < HD / 16; ++t) {
                         const int ch = (t & 3) * 2 + ((lane >> 3) & 1);
                         uint32_t f[4];
-                        ldsm4_t(f, rowa + (t >> 2) * (kBlock * 128) + ((ch ^ (row & 7)) << 4));
+                        ldsm4_t(f, rowa + (t >> 2) * col_ld + ((ch ^ (row & 7)) << 4));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
                             mma16816<F16>(o[t][nt], f, pf[nt][0], pf[nt][1]);
@@ -543,7 +547,7 @@ struct Shape {
     int grid, rows, block;  // CTAs, rows of a part, keys of a block
 };
 
-constexpr int64_t kWholeKeys = 512;
+constexpr int64_t kWholeKeys = 256;
 
 Shape shape_of(int n_heads, int n_kv, int hd, int64_t max_q, int64_t max_keys) {
     const int G = n_heads / n_kv;
@@ -619,12 +623,14 @@ cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
     a.whole = s.whole;
     // the largest power of two that divides the page size: no box crosses a page
     a.box = std::min(s.block, c.pb.page_size & -c.pb.page_size);
+    // (the tensor-core kernel's stages hold 128 dims, its columns 128 keys)
+    a.box_cols = !s.tiles ? c.head_dim / 64 : (a.box == s.block && c.head_dim > 64 ? 2 : 1);
     if (!s.whole) place_workspace(a, s.grid, s.rows, c.ws);
     CUtensorMap mk, mv;
     if (!make_map_pages(&mk, c.f16, c.k, c.head_dim, c.pb.page_size, c.n_kv, c.pb.n_pages,
-                        c.page_stride, a.box) ||
+                        c.page_stride, a.box, a.box_cols) ||
         !make_map_pages(&mv, c.f16, c.v, c.head_dim, c.pb.page_size, c.n_kv, c.pb.n_pages,
-                        c.page_stride, a.box))
+                        c.page_stride, a.box, a.box_cols))
         return cudaErrorInvalidValue;
     if (c.f16) {
         if (c.head_dim == 64) return run_attention<64, true>(a, mk, mv, s, rows, st);

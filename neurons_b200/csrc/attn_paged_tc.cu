@@ -114,8 +114,9 @@ struct Plan {
     }
 };
 
-// One ring stage: kUnitDims dims from u * kUnitDims on of block `blk`.  Boxes
-// without a visible key of the piece read as zeros (page n_pages).
+// One ring stage: kUnitDims dims from u * kUnitDims on of block `blk`, as columns
+// of 64 dims (16 KB each), in boxes of a.box keys; a box of all 128 keys takes
+// both columns.  Boxes without a visible key of the piece read as zeros (page n_pages).
 template <int HD>
 __device__ __forceinline__ void load_unit(const PagedAttnArgs &a, const CUtensorMap *map,
                                           const Piece &p, int blk, int u, int key_lo, int key_hi,
@@ -123,7 +124,8 @@ __device__ __forceinline__ void load_unit(const PagedAttnArgs &a, const CUtensor
     using T = Tc<HD>;
     constexpr int kCols = T::kUnitDims / 64;
     const int lane = threadIdx.x & 31;
-    const int r = lane / kCols, col = lane % kCols;
+    const int per = kCols / a.box_cols;  // boxes beside one another: 1 or kCols
+    const int r = lane / per, col = lane % per;
     const bool on = r < kBlock / a.box;
     const int key = blk * kBlock + r * a.box;
     int page = a.pb.n_pages, slot = 0;
@@ -134,8 +136,8 @@ __device__ __forceinline__ void load_unit(const PagedAttnArgs &a, const CUtensor
     if (lane == 0) mbar_expect_tx(bar, T::kUnitBytes);
     __syncwarp();
     if (on)
-        tma_load_4d(stage + col * (kBlock * 128) + r * a.box * 128, map, bar,
-                    u * T::kUnitDims + col * 64, slot, p.h, page);
+        tma_load_5d(stage + col * (kBlock * 128) + r * a.box * 128, map, bar, 0, slot,
+                    u * kCols + col, p.h, page);
 }
 
 template <int HD, bool F16>

@@ -1000,16 +1000,16 @@ bool make_map_2d(CUtensorMap *m, CUtensorMapDataType dt, const void *base, uint6
 }
 
 bool make_map_pages(CUtensorMap *m, bool f16, const void *base, int head_dim, int page_size,
-                    int n_kv, int n_pages, int64_t page_stride, int box) {
+                    int n_kv, int n_pages, int64_t page_stride, int box, int cols) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t row = (cuuint64_t)head_dim * 2;
-    cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)n_kv,
+    cuuint64_t dims[5] = {64, (cuuint64_t)page_size, (cuuint64_t)head_dim / 64, (cuuint64_t)n_kv,
                           (cuuint64_t)n_pages};
-    cuuint64_t strides[3] = {row, row * page_size, (cuuint64_t)page_stride * 2};
-    cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+    cuuint64_t strides[4] = {row, 128, row * page_size, (cuuint64_t)page_stride * 2};
+    cuuint32_t boxes[5] = {64, (cuuint32_t)box, (cuuint32_t)cols, 1, 1};
+    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
               const_cast<void *>(base), dims, strides, boxes, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -133,9 +133,10 @@ cudaError_t launch_tc_gemm(const TcGemmArgs &a, cudaStream_t stream);
 int tc_gemm_launches(const TcGemmArgs &a);
 
 // The keys or values of a paged cache [n_pages][n_kv][page_size][head_dim] as a
-// 4-D tensor (128-byte swizzle, boxes of `box` keys x 64 dims).
+// tensor (64 dims, page_size, head_dim / 64, n_kv, n_pages) with 128-byte
+// swizzle; a box is `box` keys of `cols` columns of 64 dims, column by column.
 bool make_map_pages(CUtensorMap *m, bool f16, const void *base, int head_dim, int page_size,
-                    int n_kv, int n_pages, int64_t page_stride, int box);
+                    int n_kv, int n_pages, int64_t page_stride, int box, int cols);
 
 // True when cuTensorMapEncodeTiled could be resolved from the driver.
 bool tensor_maps_available();

@@ -304,7 +304,7 @@ struct PagedAttnArgs {
     uint16_t *out;       // [n_tokens][out_ld]
     int64_t q_ld, out_ld;
     int n_heads, n_kv, window;
-    int box;             // keys per TMA box
+    int box, box_cols;   // keys and columns of 64 dims per TMA box
     int least;           // fewest key blocks (tiles, when whole) of a CTA's share
     bool whole;          // tiles are not cut
     float scale;
@@ -367,12 +367,13 @@ cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, unsigned threads, size_t s
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-__device__ __forceinline__ void tma_load_4d(void *smem_dst, const void *tmap, uint64_t *bar,
-                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
+__device__ __forceinline__ void tma_load_5d(void *smem_dst, const void *tmap, uint64_t *bar,
+                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3,
+                                            int32_t c4) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
-        "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
         : "memory");
 }
 
