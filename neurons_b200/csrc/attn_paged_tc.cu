@@ -39,7 +39,11 @@ template <int HD>
 struct Tc {
     static constexpr int kGroups = HD == 256 ? 1 : 2;       // softmax warpgroups
     static constexpr int kMmaWarp = 4 * kGroups, kLoadWarp = kMmaWarp + 1;
-    static constexpr int kThreads = 32 * (kLoadWarp + 1);
+    // With two softmax warpgroups the MMA and loader warps are half of a third, so
+    // that registers can be moved between warpgroups: 168 each at launch (all of the
+    // SM's 64 K), then 208 for a softmax thread, which holds a row of 128 scores, and
+    // 88 for the others; 2 * 208 + 88 = 3 * 168.
+    static constexpr int kThreads = kGroups == 2 ? 384 : 32 * (kLoadWarp + 1);
     // a ring stage: 128 keys (or values) x kUnitDims dims
     static constexpr int kUnitDims = HD < 128 ? HD : 128;
     static constexpr int kUnits = HD / kUnitDims;
@@ -114,6 +118,14 @@ struct Plan {
     }
 };
 
+// A piece as the loader warp, which alone walks the list, hands it to the others
+// (two slots, so that it runs a piece ahead).  parts: of a tile that this CTA
+// begins and does not finish, else 0; n == 0 ends the list.
+struct Job {
+    Piece p;
+    int n, parts;
+};
+
 // One ring stage: kUnitDims dims from u * kUnitDims on of block `blk`, as columns
 // of 64 dims (16 KB each), in boxes of a.box keys; a box of all 128 keys takes
 // both columns.  Boxes without a visible key of the piece read as zeros (page n_pages).
@@ -150,8 +162,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     __shared__ __align__(8) uint64_t full[T::kStages], empty[T::kStages], s_full[2], p_ready[2];
     __shared__ __align__(8) uint64_t q_full, o_full, pv_done;
     __shared__ uint32_t tmem_holder;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, stop;
     __shared__ float xm[T::kGroups == 2 ? kBlock : 1], xl[T::kGroups == 2 ? kBlock : 1];
+    __shared__ Job jobs[2];
+    __shared__ __align__(8) uint64_t job_full[2], job_empty[2];
     volatile int *abort = &abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.n_heads / a.n_kv, tok = kBlock / G, TT = T::kGroups * tok;
@@ -165,11 +179,13 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], kBlock);
+            mbar_init(&job_full[i], 1);
+            mbar_init(&job_empty[i], 1 + 4 * T::kGroups);  // the MMA and softmax warps
         }
         mbar_init(&q_full, T::kGroups * kBlock);
         mbar_init(&o_full, 1);
         mbar_init(&pv_done, 1);
-        abort_flag = 0;
+        abort_flag = stop = 0;
         fence_barrier_init();
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
@@ -184,15 +200,37 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     const uint32_t tmem = tmem_holder;
     pdl_wait();  // lengths, tables, q and the cache come from earlier kernels
 
-    const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x, a.least,
-                                        a.whole);
-    Cursor c = sh.c;
-    Piece p;
-
+    if (warp >= 4 * T::kGroups) {
+    if constexpr (T::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == T::kLoadWarp) {
-        int g = 0;  // stages filled so far
-        bool ok = true;
+        const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x,
+                                            a.least, a.whole);
+        Cursor c = sh.c;
+        Piece p;
+        int64_t unit = sh.first;
+        int g = 0, jobs_out = 0;  // stages filled and jobs handed out so far
+        bool ok = true, note_left = false;
+        auto hand_out = [&](int n, int parts) {
+            const int slot = jobs_out & 1;
+            ok = mbar_wait_or_abort(&job_empty[slot], (uint32_t)(jobs_out / 2 + 1) & 1u, abort,
+                                    a.pb.err);
+            if (ok && lane == 0) {
+                jobs[slot].p = p;
+                jobs[slot].n = n;
+                jobs[slot].parts = parts;
+                mbar_arrive(&job_full[slot]);
+            }
+            ++jobs_out;
+        };
         while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
+            int parts = 0;
+            if (p.k0 == 0 && p.k1 < p.nb) {
+                parts = share_owner(sh.total, sh.n, unit + p.nb - 1) - (int)blockIdx.x + 1;
+                note_left = true;
+            }
+            unit += p.k1 - p.k0;
+            hand_out(p.k1 - p.k0, parts);
+            if (!ok) break;
             const Plan<HD> pl(p, tok);
             const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
             const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
@@ -219,6 +257,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 }
             }
         }
+        if (ok) hand_out(0, 0);
+        if (lane == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
         if (!ok || *abort) {  // given up: the copies in flight end before this CTA does
             for (int j = max(0, g - T::kStages); j < g; ++j) {
                 const unsigned long long t0 = global_timer_ns();
@@ -240,9 +280,14 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 ok = ok && mbar_wait_or_abort(&full[g % T::kStages],
                                               (uint32_t)(g / T::kStages) & 1u, abort, a.pb.err);
             };
-            while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
-                const Plan<HD> pl(p, tok);
+            while (ok) {
+                const int slot = pieces & 1;
+                ok = mbar_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort,
+                                        a.pb.err);
+                if (!ok || jobs[slot].n == 0) break;
+                const Plan<HD> pl(jobs[slot].p, tok);
                 const int steps = pl.steps();
+                mbar_arrive(&job_empty[slot]);
                 ok = mbar_wait_or_abort(&q_full, (uint32_t)pieces & 1u, abort, a.pb.err);
                 auto issue_s = [&](int i) {
                     const int b = pl.block(i), buf = i & 1;
@@ -304,27 +349,45 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             }
         }
         __syncwarp();
+    }
     } else {
         // ---------------------------------------------------------- softmax
+        if constexpr (T::kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int w = warp >> 2;                    // warpgroup
         const int r = threadIdx.x & 127;            // this thread's row of the query tile
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
         int loads = 0, pieces = 0, pvs = 0;
         uint32_t s_phase = 0;
-        int64_t unit = sh.first;
-        bool ok = true, note_left = false;
-        while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
+        bool ok = true;
+        while (true) {
+            // What a piece says stays in shared memory until it is needed: the scores take
+            // most of the registers.
+            const Job &job = jobs[pieces & 1];
+            ok = ok && !*abort &&
+                 mbar_wait_or_abort(&job_full[pieces & 1], (uint32_t)(pieces / 2) & 1u, abort,
+                                    a.pb.err);
+            // (without the job nobody knows whether a barrier follows: both warpgroups stop)
+            if (T::kGroups == 2) {
+                if (!ok) stop = 1;
+                bar_sync(1, 256);
+                ok = !stop;
+            }
+            if (!__all_sync(0xffffffffu, ok) || job.n == 0) break;
+            const Piece &p = job.p;
             const Plan<HD> pl(p, tok);
             const int steps = pl.steps();
             const int sub = pl.two ? w : 0;         // which query tile
             const int t0 = p.t0 + sub * tok, t1 = min(t0 + tok, p.t1);
             const int valid = (t1 - t0) * G;
             const int base = p.s.len - p.s.n;
-            const int key_hi = base + p.t1;
-            const int key_lo = a.window > 0 ? max(0, base + p.t0 - a.window + 1) : 0;
             const int my_t = t0 + r / G, my_h = p.h * G + r % G;
             const int pos = r < valid ? base + my_t : -1;
+            // steps whose block reaches past the first row's position, or below the last
+            // row's window, are masked
+            const int full_to = base + t0 + 1 - kBlock;
+            const int full_from = a.window > 0 ? base + t1 - a.window : 0;
+            const int block0 = p.lo + p.k0;
             if (pl.two || w == 0) {
                 // the query row, in the K-major layout with 128-byte swizzle
                 const uint4 *src = reinterpret_cast<const uint4 *>(
@@ -360,8 +423,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     tmem_ld_32x32b_x32(sc + j * 32,
                                        *reinterpret_cast<uint32_t(*)[32]>(s + j * 32));
                 tmem_ld_wait();
-                const int key0 = (p.lo + p.k0 + b) * kBlock;
-                if (key0 + kBlock - 1 > base + t0 || (a.window > 0 && key0 <= base + t1 - 1 - a.window)) {
+                const int key0 = (block0 + b) * kBlock;
+                if (key0 > full_to || key0 < full_from) {
                     const int hi = pos - key0;
                     const int lo = a.window > 0 ? hi - a.window + 1 : 0;
 #pragma unroll
@@ -421,6 +484,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     tmem_st_32x32b_x16(sc + j * 16, pk);
                 }
                 l += sum[0] + sum[1];
+                const int key_hi = p.s.len - p.s.n + p.t1;
+                const int key_lo = a.window > 0 ? p.s.len - p.s.n + p.t0 - a.window + 1 : 0;
                 if (key0 < key_lo || key0 + kBlock > key_hi) {
                     // values of keys that no row sees may hold anything: a NaN times a
                     // weight of 0 would reach the sum
@@ -528,21 +593,16 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     *reinterpret_cast<float2 *>(a.part_ml + ((int64_t)slot * T::kRows + row) * 2) =
                         make_float2(M * cs, L);
             }
-            if (!whole && p.k0 == 0) {
-                note_left = true;
-                if (threadIdx.x == 0)
-                    a.notes[blockIdx.x] = SplitNote{
-                        p.s.q0 + p.t0, p.h * G, p.t1 - p.t0,
-                        share_owner(sh.total, sh.n, unit + p.nb - 1) - (int)blockIdx.x + 1};
-            }
+            if (threadIdx.x == 0 && job.parts > 0)
+                a.notes[blockIdx.x] = SplitNote{p.s.q0 + p.t0, p.h * G, p.t1 - p.t0, job.parts};
             tc_fence_before();  // the next piece's products may overwrite S and O
             if (T::kGroups == 2 && !pl.two) bar_sync(1, 256);  // `other` has been read
-            unit += p.k1 - p.k0;
             loads += 2 * pl.n;
             pvs += steps;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&job_empty[pieces & 1]);
             ++pieces;
         }
-        if (threadIdx.x == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
     }
     tc_fence_before();
     __syncthreads();
