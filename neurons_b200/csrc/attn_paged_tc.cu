@@ -61,6 +61,24 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// two fp32 values per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "mov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, kind::f16, one CTA
 __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                         uint32_t idesc, uint32_t accumulate) {
@@ -178,11 +196,11 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_ready[i], kBlock);
+            mbar_init(&p_ready[i], 4);  // (one arrival per warp)
             mbar_init(&job_full[i], 1);
             mbar_init(&job_empty[i], 1 + 4 * T::kGroups);  // the MMA and softmax warps
         }
-        mbar_init(&q_full, T::kGroups * kBlock);
+        mbar_init(&q_full, T::kGroups * 4);
         mbar_init(&o_full, 1);
         mbar_init(&pv_done, 1);
         abort_flag = stop = 0;
@@ -402,7 +420,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 }
                 fence_proxy_async_smem();
             }
-            mbar_arrive(&q_full);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
 
             float m = -INFINITY, l = 0.f;
             bool first = true;
@@ -468,22 +487,22 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 }
                 first = false;
                 const float z = m == -INFINITY ? 0.f : m * cs;
-                float sum[2] = {0.f, 0.f};
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float e0 = ex2(fmaf(s[j * 32 + 2 * e], cs, -z));
-                        const float e1 = ex2(fmaf(s[j * 32 + 2 * e + 1], cs, -z));
-                        sum[0] += e0;
-                        sum[1] += e1;
+                        const float2 x2 = fma2(make_float2(s[j * 32 + 2 * e], s[j * 32 + 2 * e + 1]),
+                                               make_float2(cs, cs), make_float2(-z, -z));
+                        const float e0 = ex2(x2.x), e1 = ex2(x2.y);
+                        sum[e & 1] = add2(sum[e & 1], make_float2(e0, e1));
                         // rounded to the cache's type: both factors of an MMA are of one type
                         pk[e] = pack_t2<F16>(e0, e1);
                     }
                     tmem_st_32x32b_x16(sc + j * 16, pk);
                 }
-                l += sum[0] + sum[1];
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 const int key_hi = p.s.len - p.s.n + p.t1;
                 const int key_lo = a.window > 0 ? p.s.len - p.s.n + p.t0 - a.window + 1 : 0;
                 if (key0 < key_lo || key0 + kBlock > key_hi) {
@@ -510,7 +529,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&p_ready[buf]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[buf]);
             }
             ok = ok && !*abort &&
                  mbar_wait_or_abort(&o_full, (uint32_t)pieces & 1u, abort, a.pb.err);
