@@ -465,7 +465,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
 
 // Joins the parts of the tiles that several CTAs shared, in the CTAs' order.
 // W warps take the parts of a query row in turn: one where a tile has few parts
-// and many rows, four where a decode step has few rows in many parts.
+// and many rows (attn_paged_tc.cu, whose parts lie [dim / 4][row][4], as its
+// threads, a row each, write them), four where a decode step has few rows in
+// many parts (paged_rows_kernel's, [row][dim]).
 template <int HD, bool F16, int W>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a, int rows) {
     pdl_launch_dependents();
@@ -495,11 +497,13 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 #pragma unroll 4
     for (int i = first; i < note.parts; i += W) {
         const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + slot(i) * 2);
-        const float *po = a.part_o + slot(i) * HD + lane * kPer;
         float v[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; j += 2) {
-            const float2 w = *reinterpret_cast<const float2 *>(po + j);
+            const int d = lane * kPer + j;
+            const float *po = W == 1 ? a.part_o + (slot(i) - r) * HD + ((d >> 2) * rows + r) * 4 + (d & 3)
+                                     : a.part_o + slot(i) * HD + d;
+            const float2 w = *reinterpret_cast<const float2 *>(po);
             v[j] = w.x;
             v[j + 1] = w.y;
         }
@@ -541,19 +545,20 @@ int rows_grid(int hd) {
 // Which kernel serves a call: paged_rows_kernel while a sequence's new tokens
 // make one tile of 16 rows, so that each key is read once; the tensor-core
 // kernel (128- or 256-row tiles) from there on.
-// A table that holds at most kWholeKeys keys per sequence leaves the tiles whole.
+// A table that holds at most kWholeKeys (kWholeKeysTiles) keys per sequence
+// leaves the tiles whole.
 struct Shape {
     bool tiles, whole;
     int grid, rows, block;  // CTAs, rows of a part, keys of a block
 };
 
-constexpr int64_t kWholeKeys = 256;
+constexpr int64_t kWholeKeys = 256, kWholeKeysTiles = 1024;
 
 Shape shape_of(int n_heads, int n_kv, int hd, int64_t max_q, int64_t max_keys) {
     const int G = n_heads / n_kv;
-    const bool whole = max_keys <= kWholeKeys;
-    if (max_q * G > kRows) return Shape{true, whole, sm_count(), paged_tiles_rows(hd), 128};
-    return Shape{false, whole, rows_grid(hd), kRows, kBlock};
+    if (max_q * G > kRows)
+        return Shape{true, max_keys <= kWholeKeysTiles, sm_count(), paged_tiles_rows(hd), 128};
+    return Shape{false, max_keys <= kWholeKeys, rows_grid(hd), kRows, kBlock};
 }
 
 template <int HD, bool F16, int NT>

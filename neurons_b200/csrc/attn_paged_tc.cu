@@ -9,6 +9,8 @@
 //                 swizzle, boxes of 16 to 128 keys x 64 dims)
 //   MMA warp      S = Q K^T (both in shared memory) and O += P V (P in TMEM, V as
 //                 it lies: keys x dims, the MN-major operand), one thread
+//   query warps   the next tile's queries, as soon as the last S that reads the
+//                 present ones is done
 //   softmax       one row per thread: S from TMEM, a running maximum and sum,
 //                 P back into S's columns in 16 bits
 // Two tiles S are always in flight, so that the tensor cores work on one while
@@ -39,18 +41,21 @@ template <int HD>
 struct Tc {
     static constexpr int kGroups = HD == 256 ? 1 : 2;       // softmax warpgroups
     static constexpr int kMmaWarp = 4 * kGroups, kLoadWarp = kMmaWarp + 1;
-    // With two softmax warpgroups the MMA and loader warps are half of a third, so
-    // that registers can be moved between warpgroups: 168 each at launch (all of the
-    // SM's 64 K), then 208 for a softmax thread, which holds a row of 128 scores, and
-    // 88 for the others; 2 * 208 + 88 = 3 * 168.
-    static constexpr int kThreads = kGroups == 2 ? 384 : 32 * (kLoadWarp + 1);
+    static constexpr int kQueryWarp = kLoadWarp + 1;        // and the next
+    // A third (second) warpgroup of one MMA, one loader and two query warps.  With
+    // two softmax warpgroups registers are moved between them: 168 each at launch
+    // (all of the SM's 64 K), then 208 for a softmax thread, which holds a row of 128
+    // scores, and 88 for the others; 2 * 208 + 88 = 3 * 168.
+    static constexpr int kThreads = 128 * (kGroups + 1);
     // a ring stage: 128 keys (or values) x kUnitDims dims
     static constexpr int kUnitDims = HD < 128 ? HD : 128;
     static constexpr int kUnits = HD / kUnitDims;
     static constexpr int kUnitBytes = kBlock * kUnitDims * 2;
-    static constexpr int kStages = HD == 64 ? 8 : 5;
+    static constexpr int kStages = HD == 64 ? 8 : 4;  // 128 KB
     static constexpr int kQBytes = kBlock * HD * 2;
-    static constexpr int kSmem = kGroups * kQBytes + kStages * kUnitBytes;
+    static constexpr int kOutBytes = 2048;                  // a warp's 32 rows x 32 dims
+    static constexpr int kSmem =
+        kGroups * kQBytes + kStages * kUnitBytes + 4 * kGroups * kOutBytes;
     static constexpr int kO = 256;                          // first TMEM column of O
     static constexpr int kRows = kGroups * kBlock;          // rows of a part
 };
@@ -177,11 +182,12 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     using T = Tc<HD>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *qs = smem, *ring = smem + T::kGroups * T::kQBytes;
+    uint8_t *outs = ring + T::kStages * T::kUnitBytes;
     __shared__ __align__(8) uint64_t full[T::kStages], empty[T::kStages], s_full[2], p_ready[2];
-    __shared__ __align__(8) uint64_t q_full, o_full, pv_done;
+    __shared__ __align__(8) uint64_t q_full, q_empty, o_full, pv_done;
     __shared__ uint32_t tmem_holder;
     __shared__ int abort_flag, stop;
-    __shared__ float xm[T::kGroups == 2 ? kBlock : 1], xl[T::kGroups == 2 ? kBlock : 1];
+    __shared__ float2 xml[T::kGroups == 2 ? 2 * kBlock : 1];
     __shared__ Job jobs[2];
     __shared__ __align__(8) uint64_t job_full[2], job_empty[2];
     volatile int *abort = &abort_flag;
@@ -198,9 +204,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], 4);  // (one arrival per warp)
             mbar_init(&job_full[i], 1);
-            mbar_init(&job_empty[i], 1 + 4 * T::kGroups);  // the MMA and softmax warps
+            mbar_init(&job_empty[i], 3 + 4 * T::kGroups);  // the other warps
         }
-        mbar_init(&q_full, T::kGroups * 4);
+        mbar_init(&q_full, 2);
+        mbar_init(&q_empty, 1);
         mbar_init(&o_full, 1);
         mbar_init(&pv_done, 1);
         abort_flag = stop = 0;
@@ -328,6 +335,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                         if (pl.last_use(i)) umma_commit(&empty[g % T::kStages]);
                     }
                     umma_commit(&s_full[buf]);
+                    if (i + 1 == steps) umma_commit(&q_empty);
                 };
                 if (ok) issue_s(0);
                 if (ok && steps > 1) issue_s(1);
@@ -367,6 +375,40 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             }
         }
         __syncwarp();
+    } else {
+        // ---------------------------------------------------------- query rows
+        constexpr int kLanes = HD / 8, kStep = 64 / kLanes;  // lanes per row, rows at a time
+        const int lid = threadIdx.x - T::kQueryWarp * 32;
+        const uint32_t inv_g = (65535 + G) / G;  // r / G = r * inv_g >> 16 for r < 128
+        for (int pieces = 0;; ++pieces) {
+            const int slot = pieces & 1;
+            if (!mbar_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort, a.pb.err))
+                break;
+            if (jobs[slot].n == 0) break;
+            const Piece p = jobs[slot].p;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&job_empty[slot]);
+            if (!mbar_wait_or_abort(&q_empty, (uint32_t)(pieces + 1) & 1u, abort, a.pb.err)) break;
+            const bool two = T::kGroups == 2 && p.t1 - p.t0 > tok;
+            for (int sub = 0; sub <= (two ? 1 : 0); ++sub) {
+                const int t0 = p.t0 + sub * tok, valid = (min(t0 + tok, p.t1) - t0) * G;
+                const int ch = lid % kLanes;
+                // the K-major layout with 128-byte swizzle, columns of 64 dims
+                uint8_t *dst = qs + sub * T::kQBytes + (ch >> 3) * (kBlock * 128);
+#pragma unroll 4
+                for (int r = lid / kLanes; r < kBlock; r += kStep) {
+                    const int t = (int)((uint32_t)r * inv_g >> 16), g = r - t * G;
+                    const uint16_t *src = a.q + (int64_t)(p.s.q0 + t0 + (r < valid ? t : 0)) * a.q_ld +
+                                          (int64_t)(p.h * G + (r < valid ? g : 0)) * HD + ch * 8;
+                    cp_async16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, r < valid ? 16 : 0);
+                }
+            }
+            cp_async_commit();
+            cp_async_wait_group<0>();
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
+        }
     }
     } else {
         // ---------------------------------------------------------- softmax
@@ -375,6 +417,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         const int r = threadIdx.x & 127;            // this thread's row of the query tile
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
+        const uint32_t inv_g = (65535 + G) / G;  // r / G = r * inv_g >> 16 for r < 128
         int loads = 0, pieces = 0, pvs = 0;
         uint32_t s_phase = 0;
         bool ok = true;
@@ -399,30 +442,12 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             const int t0 = p.t0 + sub * tok, t1 = min(t0 + tok, p.t1);
             const int valid = (t1 - t0) * G;
             const int base = p.s.len - p.s.n;
-            const int my_t = t0 + r / G, my_h = p.h * G + r % G;
-            const int pos = r < valid ? base + my_t : -1;
+            const int pos = r < valid ? base + t0 + (int)((uint32_t)r * inv_g >> 16) : -1;
             // steps whose block reaches past the first row's position, or below the last
             // row's window, are masked
             const int full_to = base + t0 + 1 - kBlock;
             const int full_from = a.window > 0 ? base + t1 - a.window : 0;
             const int block0 = p.lo + p.k0;
-            if (pl.two || w == 0) {
-                // the query row, in the K-major layout with 128-byte swizzle
-                const uint4 *src = reinterpret_cast<const uint4 *>(
-                    a.q + (int64_t)(p.s.q0 + (r < valid ? my_t : t0)) * a.q_ld +
-                    (int64_t)(r < valid ? my_h : 0) * HD);
-                uint8_t *dst = qs + sub * T::kQBytes + r * 128;
-#pragma unroll
-                for (int i = 0; i < HD / 8; ++i) {
-                    const uint4 x = r < valid ? src[i] : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4 *>(dst + (i >> 3) * (kBlock * 128) +
-                                               (((i & 7) ^ (r & 7)) << 4)) = x;
-                }
-                fence_proxy_async_smem();
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full);
-
             float m = -INFINITY, l = 0.f;
             bool first = true;
             for (int i = T::kGroups == 2 ? w : 0; i < steps; i += T::kGroups) {
@@ -536,87 +561,91 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                  mbar_wait_or_abort(&o_full, (uint32_t)pieces & 1u, abort, a.pb.err);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
-            const uint32_t oc = tmem + lanes + T::kO + (T::kGroups == 2 ? w * HD : 0);
             const bool whole = p.k0 == 0 && p.k1 == p.nb;
-            float f0 = 1.f, f1 = 0.f;
-            const float *other = reinterpret_cast<const float *>(smem) + r;
-            float M = m, L = l;
-            if (T::kGroups == 2 && !pl.two) {
-                // join the two warpgroups' sums: the second one's through the space of
-                // the query tiles ([dim][row]), which all products have read by now
-                if (w == 1) {
-                    float *x = reinterpret_cast<float *>(smem) + r;
-                    if (ok && steps > 1) {
-#pragma unroll 1
-                        for (int j = 0; j < HD; j += 32) {
-                            uint32_t v[32];
-                            tmem_ld_32x32b_x32(oc + j, v);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                x[(j + e) * kBlock] = __uint_as_float(v[e]);
-                        }
-                    }
-                    xm[r] = m;
-                    xl[r] = l;
-                }
+            // One query tile in two warpgroups' sums: each thread can read its row of both
+            // O, so a warpgroup writes half of the dims, joining the two as it goes.
+            const bool join = T::kGroups == 2 && !pl.two;
+            float f0 = 1.f, f1 = 0.f, M = m, L = l;
+            if (join) {
+                xml[w * kBlock + r] = make_float2(m, l);
                 bar_sync(1, 256);
-                if (w == 0) {
-                    const float m1 = xm[r];
-                    M = fmaxf(m, m1);
-                    f0 = m == -INFINITY ? 0.f : ex2((m - M) * cs);
-                    f1 = m1 == -INFINITY ? 0.f : ex2((m1 - M) * cs);
-                    L = l * f0 + xl[r] * f1;
-                }
+                const float2 a0 = xml[r], a1 = xml[kBlock + r];
+                M = fmaxf(a0.x, a1.x);
+                f0 = a0.x == -INFINITY ? 0.f : ex2((a0.x - M) * cs);
+                f1 = a1.x == -INFINITY ? 0.f : ex2((a1.x - M) * cs);
+                L = a0.y * f0 + a1.y * f1;
             }
-            if (ok && (pl.two || w == 0)) {
+            if (ok) {
+                // (a row without a key: whatever O holds)
                 const float inv = L == 0.f ? 0.f : (whole ? 1.f / L : 1.f);
-                const bool join = T::kGroups == 2 && !pl.two && steps > 1;
+                f0 *= inv;
+                f1 *= inv;
+                const bool both = join && steps > 1;
+                const bool none = L == 0.f;
                 const int slot = 2 * blockIdx.x + (p.k0 == 0 ? 1 : 0);
                 const int row = sub * tok * G + r;
-                uint16_t *op = a.out + (int64_t)(p.s.q0 + my_t) * a.out_ld + (int64_t)my_h * HD;
-                float *pp = a.part_o + ((int64_t)slot * T::kRows + row) * HD;
+                const uint32_t oc = tmem + lanes + T::kO + (pl.two ? w * HD : 0);
+                const int from = join ? w * (HD / 2) : 0, to = join ? from + HD / 2 : HD;
+                uint8_t *stage = outs + warp * T::kOutBytes;
 #pragma unroll 1
-                for (int j = 0; j < HD; j += 32) {
+                for (int j = from; j < to; j += 32) {
                     uint32_t v[32];
                     __syncwarp();
                     tmem_ld_32x32b_x32(oc + j, v);
                     tmem_ld_wait();
                     float y[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        y[e] = __uint_as_float(v[e]) * f0;
-                        if (join && f1 != 0.f) y[e] = fmaf(other[(j + e) * kBlock], f1, y[e]);
-                        // (rows without a key: whatever O holds)
-                        y[e] = L == 0.f ? 0.f : y[e] * inv;
-                    }
-                    if (r < valid) {
-                        if (whole) {
+                    for (int e = 0; e < 32; ++e) y[e] = none ? 0.f : __uint_as_float(v[e]) * f0;
+                    if (both) {
+                        tmem_ld_32x32b_x32(oc + HD + j, v);
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint4 o;
-                                o.x = pack_t2<F16>(y[e], y[e + 1]);
-                                o.y = pack_t2<F16>(y[e + 2], y[e + 3]);
-                                o.z = pack_t2<F16>(y[e + 4], y[e + 5]);
-                                o.w = pack_t2<F16>(y[e + 6], y[e + 7]);
-                                *reinterpret_cast<uint4 *>(op + j + e) = o;
-                            }
-                        } else {
+                        for (int e = 0; e < 32; ++e)
+                            if (f1 != 0.f) y[e] = fmaf(__uint_as_float(v[e]), f1, y[e]);
+                    }
+                    if (!whole) {
+                        // [dim / 4][row][4]: neighbouring threads write neighbouring 16 bytes
+                        float *pp = a.part_o + (int64_t)slot * T::kRows * HD + row * 4;
+                        if (r < valid) {
 #pragma unroll
                             for (int e = 0; e < 32; e += 4)
-                                *reinterpret_cast<float4 *>(pp + j + e) =
+                                *reinterpret_cast<float4 *>(pp + ((j + e) >> 2) * (T::kRows * 4)) =
                                     make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
                         }
+                        continue;
+                    }
+                    // a warp's 32 rows x 32 dims turn in shared memory into stores of 64
+                    // bytes of a row (16-byte chunks swizzled by the row)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<uint4 *>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
+                            make_uint4(pack_t2<F16>(y[8 * e], y[8 * e + 1]),
+                                       pack_t2<F16>(y[8 * e + 2], y[8 * e + 3]),
+                                       pack_t2<F16>(y[8 * e + 4], y[8 * e + 5]),
+                                       pack_t2<F16>(y[8 * e + 6], y[8 * e + 7]));
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = i * 8 + (lane >> 2), e = lane & 3;
+                        const int R = (warp & 3) * 32 + rr;
+                        const int t = (int)((uint32_t)R * inv_g >> 16);
+                        if (R < valid)
+                            *reinterpret_cast<uint4 *>(
+                                a.out + (int64_t)(p.s.q0 + t0 + t) * a.out_ld +
+                                (int64_t)(p.h * G + R - t * G) * HD + j + e * 8) =
+                                *reinterpret_cast<const uint4 *>(
+                                    stage + rr * 64 + ((e ^ ((rr >> 1) & 3)) << 4));
                     }
                 }
-                if (!whole && r < valid)
+                if (!whole && r < valid && (!join || w == 0))
                     *reinterpret_cast<float2 *>(a.part_ml + ((int64_t)slot * T::kRows + row) * 2) =
                         make_float2(M * cs, L);
             }
             if (threadIdx.x == 0 && job.parts > 0)
                 a.notes[blockIdx.x] = SplitNote{p.s.q0 + p.t0, p.h * G, p.t1 - p.t0, job.parts};
-            tc_fence_before();  // the next piece's products may overwrite S and O
-            if (T::kGroups == 2 && !pl.two) bar_sync(1, 256);  // `other` has been read
+            // (the next piece's first product into O waits for this warpgroup's weights,
+            // and the barrier above for both warpgroups)
+            tc_fence_before();
             loads += 2 * pl.n;
             pvs += steps;
             __syncwarp();

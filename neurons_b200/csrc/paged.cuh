@@ -96,16 +96,22 @@ __device__ __forceinline__ KeyRange key_range(const SeqView &s, int t0, int t1, 
 }
 
 // A position in the list of all key blocks of a call: entry b, key head h,
-// token tile t, and `off` blocks into that tile's `nb`; `left` is what the
-// CTA still has to do.
+// place t in the order of the token tiles, and `off` blocks into that tile's
+// `nb`; `left` is what the CTA still has to do.
 struct Cursor {
     int b, h, t, off;
     int64_t left;
     SeqView s;
 };
 
+// The token tile at place i of n: first, last, second, last but one, ...  A
+// prompt's first tiles see few keys and its last ones many; in this order each
+// stretch of the list holds both, and no CTA gets only short tiles, whose
+// beginnings and ends cost more than their products.
+__device__ __forceinline__ int tile_at(int i, int n) { return i & 1 ? n - 1 - (i >> 1) : i >> 1; }
+
 // The list: entries in order, in each its key heads, in each the token tiles
-// (TT tokens), in each its key blocks.  Neighbouring CTAs therefore read the
+// (TT tokens) in tile_at()'s order, in each its key blocks.  Neighbouring CTAs therefore read the
 // same head's keys at the same time.  CTA c of n takes the blocks
 // [c * total / n, (c + 1) * total / n), so that all CTAs get the same number
 // whatever the lengths are; a tile cut by such a border is finished by
@@ -156,31 +162,43 @@ struct Share {
     Cursor c;        // at `first`; c.left blocks
 };
 
+// a * b / c; in 32 bits, which is several times faster, where the product fits
+__device__ __forceinline__ int64_t mul_div(int64_t a, int64_t b, int64_t c) {
+    if (((a | b | c) >> 32) == 0 && a * b < (1ll << 32))
+        return (uint32_t)(a * b) / (uint32_t)c;
+    return a * b / c;
+}
+
 // CTAs that take part in a call of `total` blocks: no share is smaller than
 // `least` blocks.
 __device__ __forceinline__ int sharers(int64_t total, int grid, int least) {
-    const int64_t n = (total + least - 1) / least;
-    return (int)(n < grid ? (n > 0 ? n : 1) : grid);
+    if (total >= (int64_t)grid * least) return grid;
+    const int n = ((int)total + least - 1) / least;
+    return n > 0 ? n : 1;
 }
 __device__ __forceinline__ int64_t share_start(int64_t total, int n, int c) {
-    return (int64_t)c * total / n;
+    return mul_div(c, total, n);
 }
 // the CTA whose share holds block u
 __device__ __forceinline__ int share_owner(int64_t total, int n, int64_t u) {
+    if ((u + 1) * n - 1 < (1ll << 32) && total < (1ll << 32))
+        return (int)((uint32_t)((u + 1) * n - 1) / (uint32_t)total);
     return (int)(((u + 1) * n - 1) / total);
 }
 
 // Run by one whole warp.
 template <int BK>
-__device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int TT, int window, int cta, int grid,
-                                            int least, bool whole) {
+__device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int TT, int window,
+                                            int cta, int grid, int least, bool whole) {
     const int lane = threadIdx.x & 31;
     Share sh;
-    int64_t total = 0;
+    SeqView s{0, 0, 0, 0};
+    int64_t head = 0, total = 0;
     for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
-        SeqView s{0, 0, 0, 0};
+        s = SeqView{0, 0, 0, 0};
         if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
-        total += entry_blocks_warp<BK>(s, TT, window, whole);
+        head = entry_blocks_warp<BK>(s, TT, window, whole);
+        total += head;
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
@@ -193,9 +211,11 @@ __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int 
     sh.c.left = share_start(sh.total, sh.n, cta + 1) - sh.first;
     int64_t before = 0;
     for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
-        SeqView s{0, 0, 0, 0};
-        if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
-        const int64_t head = entry_blocks_warp<BK>(s, TT, window, whole);
+        if (pb.n_seqs > 32) {  // (else the first pass left them)
+            s = SeqView{0, 0, 0, 0};
+            if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
+            head = entry_blocks_warp<BK>(s, TT, window, whole);
+        }
         const int64_t end = before + warp_inclusive(head * n_kv);
         const unsigned past = __ballot_sync(0xffffffffu, end > sh.first);
         if (past) {
@@ -208,23 +228,23 @@ __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int 
             c.s.len = __shfl_sync(0xffffffffu, s.len, src);
             const int64_t per = __shfl_sync(0xffffffffu, head, src);
             int64_t at = sh.first - (__shfl_sync(0xffffffffu, end, src) - per * n_kv);
-            c.h = (int)(at / per);
+            c.h = (int)mul_div(at, 1, per);
             at -= c.h * per;
             const int tiles = (c.s.n + TT - 1) / TT;
             int64_t seen = 0;
-            for (int t0 = 0; t0 < tiles; t0 += 32) {
+            for (int i0 = 0; i0 < tiles; i0 += 32) {
                 int64_t nb = 0;
-                if (whole)
-                    nb = t0 + lane < tiles;
-                else if (t0 + lane < tiles)
-                    nb = key_range<BK>(c.s, (t0 + lane) * TT, min((t0 + lane + 1) * TT, c.s.n),
-                                       window)
-                             .nb;
+                if (whole) {
+                    nb = i0 + lane < tiles;
+                } else if (i0 + lane < tiles) {
+                    const int t = tile_at(i0 + lane, tiles);
+                    nb = key_range<BK>(c.s, t * TT, min((t + 1) * TT, c.s.n), window).nb;
+                }
                 const int64_t e = seen + warp_inclusive(nb);
                 const unsigned over = __ballot_sync(0xffffffffu, e > at);
                 if (over) {
                     const int l = __ffs(over) - 1;
-                    c.t = t0 + l;
+                    c.t = i0 + l;
                     c.off = (int)(at - __shfl_sync(0xffffffffu, e - nb, l));
                     break;
                 }
@@ -243,7 +263,6 @@ struct Piece {
     SeqView s;
     int h, t0, t1;     // key head; new tokens [t0, t1)
     int lo, k0, k1, nb;
-    int t;             // tile number (for the merge)
 };
 
 // Takes the next piece of the cursor and steps past it; false when done.
@@ -254,8 +273,8 @@ __device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, int T
     if (c.left <= 0) return false;
     p.s = c.s;
     p.h = c.h;
-    p.t = c.t;
-    p.t0 = c.t * TT;
+    const int tiles = (c.s.n + TT - 1) / TT;
+    p.t0 = tile_at(c.t, tiles) * TT;
     p.t1 = min(p.t0 + TT, c.s.n);
     const KeyRange r = key_range<BK>(c.s, p.t0, p.t1, window);
     p.lo = r.lo;
@@ -266,9 +285,7 @@ __device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, int T
     c.off = p.k1;
     if (p.k1 == r.nb && c.left > 0) {
         c.off = 0;
-        if (p.t1 < c.s.n) {
-            ++c.t;
-        } else {
+        if (++c.t == tiles) {
             c.t = 0;
             if (++c.h == n_kv) {
                 c.h = 0;
