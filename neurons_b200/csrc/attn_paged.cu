@@ -463,30 +463,30 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     if (warp == 0 && lane == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
 }
 
-// Joins the parts of the tiles that several CTAs shared, in the CTAs' order.
-// W warps take the parts of a query row in turn: one where a tile has few parts
-// and many rows (attn_paged_tc.cu, whose parts lie [dim / 4][row][4], as its
-// threads, a row each, write them), four where a decode step has few rows in
-// many parts (paged_rows_kernel's, [row][dim]).
-template <int HD, bool F16, int W>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a, int rows) {
+// slot of part i of the tile that CTA c begins
+__device__ __forceinline__ int64_t part_slot(int c, int i) {
+    return i == 0 ? 2 * (int64_t)c + 1 : 2 * ((int64_t)c + i);
+}
+
+// Joins the parts of the tiles that several CTAs shared, in the CTAs' order:
+// paged_rows_kernel's, [row][dim], few rows in many parts.  One CTA per row, its
+// four warps take the parts in turn.
+template <int HD, bool F16>
+__global__ void __launch_bounds__(128) paged_merge_rows_kernel(const PagedAttnArgs a, int rows) {
     pdl_launch_dependents();
     pdl_wait();
-    __shared__ float sums[W == 1 ? 1 : 4][HD + 1];
+    __shared__ float sums[4][HD + 1];
     const SplitNote note = a.notes[blockIdx.x];
     if (note.parts == 0) return;
     const int G = a.n_heads / a.n_kv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int r = W == 1 ? blockIdx.y * 4 + warp : blockIdx.y;
-    const int first = W == 1 ? 0 : warp;
+    const int r = blockIdx.y;
     if (r >= note.tokens * G) return;
     constexpr int kPer = HD / 32;
-    auto slot = [&](int i) -> int64_t {
-        return (int64_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * rows + r;
-    };
     float M = -INFINITY;
     for (int i = lane; i < note.parts; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + slot(i) * 2);
+        const float2 ml = *reinterpret_cast<const float2 *>(
+            a.part_ml + (part_slot(blockIdx.x, i) * rows + r) * 2);
         if (ml.y != 0.f) M = fmaxf(M, ml.x);
     }
 #pragma unroll
@@ -495,15 +495,14 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 #pragma unroll
     for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
 #pragma unroll 4
-    for (int i = first; i < note.parts; i += W) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + slot(i) * 2);
+    for (int i = warp; i < note.parts; i += 4) {
+        const int64_t at = part_slot(blockIdx.x, i) * rows + r;
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
+        const float *po = a.part_o + at * HD + lane * kPer;
         float v[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; j += 2) {
-            const int d = lane * kPer + j;
-            const float *po = W == 1 ? a.part_o + (slot(i) - r) * HD + ((d >> 2) * rows + r) * 4 + (d & 3)
-                                     : a.part_o + slot(i) * HD + d;
-            const float2 w = *reinterpret_cast<const float2 *>(po);
+            const float2 w = *reinterpret_cast<const float2 *>(po + j);
             v[j] = w.x;
             v[j + 1] = w.y;
         }
@@ -512,21 +511,19 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 #pragma unroll
         for (int j = 0; j < kPer; ++j) acc[j] = fmaf(v[j], f, acc[j]);
     }
-    if constexpr (W > 1) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) sums[warp][lane * kPer + j] = acc[j];
-        if (lane == 0) sums[warp][HD] = L;
-        __syncthreads();
-        if (warp > 0) return;
-        L = 0.f;
+    for (int j = 0; j < kPer; ++j) sums[warp][lane * kPer + j] = acc[j];
+    if (lane == 0) sums[warp][HD] = L;
+    __syncthreads();
+    if (warp > 0) return;
+    L = 0.f;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+    for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            L += sums[w][HD];
+    for (int w = 0; w < 4; ++w) {
+        L += sums[w][HD];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) acc[j] += sums[w][lane * kPer + j];
-        }
+        for (int j = 0; j < kPer; ++j) acc[j] += sums[w][lane * kPer + j];
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     uint16_t *op = a.out + (int64_t)(note.q_row + r / G) * a.out_ld +
@@ -534,6 +531,58 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttnArgs a,
 #pragma unroll
     for (int j = 0; j < kPer; j += 2)
         *reinterpret_cast<uint32_t *>(op + j) = pack_t2<F16>(acc[j] * inv, acc[j + 1] * inv);
+}
+
+// The same for paged_tiles_kernel's parts, [dim / 4][row][4] (its threads have a
+// row each), many rows in few parts: one thread takes 16 dims of a row, so that
+// a warp reads 512 bytes in one piece.
+template <int HD, bool F16>
+__global__ void __launch_bounds__(128) paged_merge_tiles_kernel(const PagedAttnArgs a, int rows) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const SplitNote note = a.notes[blockIdx.x];
+    if (note.parts == 0) return;
+    const int G = a.n_heads / a.n_kv;
+    const int r = blockIdx.z * 128 + threadIdx.x, d0 = blockIdx.y * 16;
+    if (r >= note.tokens * G) return;
+    float M = -INFINITY;
+#pragma unroll 4
+    for (int i = 0; i < note.parts; ++i) {
+        const float2 ml = *reinterpret_cast<const float2 *>(
+            a.part_ml + (part_slot(blockIdx.x, i) * rows + r) * 2);
+        if (ml.y != 0.f) M = fmaxf(M, ml.x);
+    }
+    float L = 0.f, acc[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < note.parts; ++i) {
+        const int64_t at = part_slot(blockIdx.x, i) * rows;
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (at + r) * 2);
+        const float *po = a.part_o + at * HD + ((d0 >> 2) * rows + r) * 4;
+        float4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4 *>(po + j * rows * 4);
+        const float f = ml.y != 0.f ? ex2(ml.x - M) : 0.f;
+        L += ml.y * f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[4 * j] = fmaf(v[j].x, f, acc[4 * j]);
+            acc[4 * j + 1] = fmaf(v[j].y, f, acc[4 * j + 1]);
+            acc[4 * j + 2] = fmaf(v[j].z, f, acc[4 * j + 2]);
+            acc[4 * j + 3] = fmaf(v[j].w, f, acc[4 * j + 3]);
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    uint16_t *op = a.out + (int64_t)(note.q_row + r / G) * a.out_ld +
+                   (int64_t)(note.heads0 + r % G) * HD + d0;
+#pragma unroll
+    for (int j = 0; j < 16; j += 8)
+        *reinterpret_cast<uint4 *>(op + j) =
+            make_uint4(pack_t2<F16>(acc[j] * inv, acc[j + 1] * inv),
+                       pack_t2<F16>(acc[j + 2] * inv, acc[j + 3] * inv),
+                       pack_t2<F16>(acc[j + 4] * inv, acc[j + 5] * inv),
+                       pack_t2<F16>(acc[j + 6] * inv, acc[j + 7] * inv));
 }
 
 // CTAs of paged_rows_kernel: as many as fit at once
@@ -579,10 +628,11 @@ cudaError_t run_attention(const PagedAttnArgs &a, const CUtensorMap &mk, const C
                                       : run_rows<HD, F16, 2>(a, mk, mv, st);
     if (e != cudaSuccess || s.whole) return e;
     if (s.tiles)
-        return launch_pdl(paged_merge_kernel<HD, F16, 1>,
-                          dim3((unsigned)s.grid, (unsigned)s.rows / 4), 128, 0, st, a, s.rows);
+        return launch_pdl(paged_merge_tiles_kernel<HD, F16>,
+                          dim3((unsigned)s.grid, HD / 16, (unsigned)s.rows / 128), 128, 0, st, a,
+                          s.rows);
     // (a caller's max_q may be too small: every row of a tile has its CTA)
-    return launch_pdl(paged_merge_kernel<HD, F16, 4>, dim3((unsigned)s.grid, rows <= 8 ? 8u : 16u),
+    return launch_pdl(paged_merge_rows_kernel<HD, F16>, dim3((unsigned)s.grid, rows <= 8 ? 8u : 16u),
                       128, 0, st, a, s.rows);
 }
 

@@ -115,7 +115,7 @@ __device__ __forceinline__ int tile_at(int i, int n) { return i & 1 ? n - 1 - (i
 // same head's keys at the same time.  CTA c of n takes the blocks
 // [c * total / n, (c + 1) * total / n), so that all CTAs get the same number
 // whatever the lengths are; a tile cut by such a border is finished by
-// paged_merge_kernel.  Where no sequence can be long (`whole`) a tile counts as
+// a merge kernel.  Where no sequence can be long (`whole`) a tile counts as
 // one and is never cut: no parts, and no merge.
 template <int BK>
 __device__ __forceinline__ int64_t entry_blocks_warp(const SeqView &s, int TT, int window,
