@@ -84,28 +84,50 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// D[tmem] (+)= A[smem] * B[smem]^T, kind::f16, one CTA
-__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                        uint32_t idesc, uint32_t accumulate) {
+// MMAs and commits run by a whole warp, one lane of which issues.  Under a
+// branch on the lane every operand of every MMA would be moved from vector to
+// uniform registers first, about 100 cycles for an MMA that takes 64; with
+// warp-uniform operands they stay in uniform registers.
+// D[tmem] (+)= A[smem] * B[smem]^T, kind::f16; the descriptors' upper halves are
+// constants.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                       uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u));
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 x, y;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]^T
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 y;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tmov.b64 y, {%2, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            smem_u32(bar))
+        : "memory");
 }
 
-// An operand whose N (here: dims) runs along memory, 128-byte swizzle: atoms of
-// 64 dims x 8 keys, the next 8 keys 1024 bytes on (stride offset), the next 64
-// dims a 128-key column of 16 KB on (leading offset).
-__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(16384u >> 4) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1u << 46;
-    d |= (uint64_t)2u << 61;
-    return d;
+// The lower half of a descriptor of an operand at 1024-byte aligned smem_addr,
+// and the upper halves (128-byte swizzle, stride offset 1024 bytes).  K along
+// memory: smem_desc_k_sw128().  N (here: dims) along memory: atoms of 64 dims x 8
+// keys, the next 8 keys 1024 bytes on (stride offset), the next 64 dims a
+// 128-key column of 16 KB on (leading offset).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t smem_addr) {
+    return ((smem_addr >> 4) & 0x3FFFu) | (1u << 16);
+}
+__device__ __forceinline__ uint32_t desc_mn(uint32_t smem_addr) {
+    return ((smem_addr >> 4) & 0x3FFFu) | ((16384u >> 4) << 16);
 }
 
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -293,85 +315,90 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             }
         }
     } else if (warp == T::kMmaWarp) {
-        if (lane == 0) {
-            constexpr uint32_t kIdS = F16 ? idesc_f16_f32(128, 128) : idesc_bf16_f32(128, 128);
-            constexpr uint32_t kIdO = (F16 ? idesc_f16_f32(128, T::kUnitDims)
-                                           : idesc_bf16_f32(128, T::kUnitDims)) |
-                                      (1u << 16);  // B: N along memory
-            int loads = 0, pieces = 0;
-            uint32_t p_phase = 0;  // bit: parity of that buffer's next p_ready
-            bool ok = true;
-            auto wait_stage = [&](int g) {
-                ok = ok && mbar_wait_or_abort(&full[g % T::kStages],
-                                              (uint32_t)(g / T::kStages) & 1u, abort, a.pb.err);
+        constexpr uint32_t kIdS = F16 ? idesc_f16_f32(128, 128) : idesc_bf16_f32(128, 128);
+        constexpr uint32_t kIdO = (F16 ? idesc_f16_f32(128, T::kUnitDims)
+                                       : idesc_bf16_f32(128, T::kUnitDims)) |
+                                  (1u << 16);  // B: N along memory
+        const uint32_t q_lo = desc_k(smem_u32(qs)), k_lo = desc_k(smem_u32(ring)),
+                       v_lo = desc_mn(smem_u32(ring));
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        int loads = 0, pieces = 0;
+        uint32_t p_phase = 0;  // bit: parity of that buffer's next p_ready
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, abort, a.pb.err)) != 0;
+        };
+        auto wait_stage = [&](int g) {
+            ok = ok && wait(&full[g % T::kStages], (uint32_t)(g / T::kStages) & 1u);
+        };
+        while (ok) {
+            const int slot = pieces & 1;
+            ok = wait(&job_full[slot], (uint32_t)(pieces / 2) & 1u);
+            if (!ok) break;
+            Plan<HD> pl(jobs[slot].p, tok);
+            pl.n = __shfl_sync(0xffffffffu, jobs[slot].n, 0);
+            pl.two = __all_sync(0xffffffffu, pl.two);
+            if (pl.n == 0) break;
+            const int steps = pl.steps();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&job_empty[slot]);
+            ok = wait(&q_full, (uint32_t)pieces & 1u);
+            auto issue_s = [&](int i) {
+                const int b = pl.block(i), buf = i & 1;
+                const uint32_t qd = q_lo + (pl.two && buf ? T::kQBytes >> 4 : 0);
+#pragma unroll
+                for (int u = 0; u < T::kUnits; ++u) {
+                    const int g = (loads + pl.key_load(b)) * T::kUnits + u;
+                    wait_stage(g);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t kd = k_lo + (g % T::kStages) * (T::kUnitBytes >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < T::kUnitDims / 16; ++kk) {
+                        // 16 dims: 32 bytes on in the swizzled rows; 64: the next column
+                        const uint32_t off = ((kk >> 2) * (kBlock * 128) + (kk & 3) * 32) >> 4;
+                        mma_ss(tm + buf * 128,
+                               qd + (u * (T::kUnitDims / 64) * (kBlock * 128) >> 4) + off, kDescHi,
+                               kd + off, kDescHi, kIdS, (u > 0 || kk > 0) ? 1u : 0u);
+                    }
+                    if (pl.last_use(i)) mma_commit(&empty[g % T::kStages]);
+                }
+                mma_commit(&s_full[buf]);
+                if (i + 1 == steps) mma_commit(&q_empty);
             };
-            while (ok) {
-                const int slot = pieces & 1;
-                ok = mbar_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort,
-                                        a.pb.err);
-                if (!ok || jobs[slot].n == 0) break;
-                const Plan<HD> pl(jobs[slot].p, tok);
-                const int steps = pl.steps();
-                mbar_arrive(&job_empty[slot]);
-                ok = mbar_wait_or_abort(&q_full, (uint32_t)pieces & 1u, abort, a.pb.err);
-                auto issue_s = [&](int i) {
-                    const int b = pl.block(i), buf = i & 1;
-                    const uint32_t qa = smem_u32(qs + (pl.two ? buf : 0) * T::kQBytes);
+            if (ok) issue_s(0);
+            if (ok && steps > 1) issue_s(1);
+            for (int i = 0; ok && i < steps; ++i) {
+                const int b = pl.block(i), buf = i & 1;
+                ok = wait(&p_ready[buf], (p_phase >> buf) & 1u);
+                if (!ok) break;
+                p_phase ^= 1u << buf;
+                const uint32_t acc = T::kGroups == 2 ? i > 1 : i > 0;
+                const uint32_t o = tm + T::kO + (T::kGroups == 2 ? buf * HD : 0);
 #pragma unroll
-                    for (int u = 0; u < T::kUnits; ++u) {
-                        const int g = (loads + pl.key_load(b)) * T::kUnits + u;
-                        wait_stage(g);
-                        if (!ok) return;
-                        tc_fence_after();
-                        const uint32_t ka = smem_u32(ring + (g % T::kStages) * T::kUnitBytes);
-#pragma unroll
-                        for (int kk = 0; kk < T::kUnitDims / 16; ++kk) {
-                            // 16 dims: 32 bytes on in the swizzled rows; 64: the next column
-                            const uint32_t off = (kk >> 2) * (kBlock * 128) + (kk & 3) * 32;
-                            umma_ss(tmem + buf * 128,
-                                    smem_desc_k_sw128(qa + u * (T::kUnitDims / 64) * (kBlock * 128) + off),
-                                    smem_desc_k_sw128(ka + off), kIdS, (u > 0 || kk > 0) ? 1u : 0u);
-                        }
-                        if (pl.last_use(i)) umma_commit(&empty[g % T::kStages]);
-                    }
-                    umma_commit(&s_full[buf]);
-                    if (i + 1 == steps) umma_commit(&q_empty);
-                };
-                if (ok) issue_s(0);
-                if (ok && steps > 1) issue_s(1);
-                for (int i = 0; ok && i < steps; ++i) {
-                    const int b = pl.block(i), buf = i & 1;
-                    ok = mbar_wait_or_abort(&p_ready[buf], (p_phase >> buf) & 1u, abort, a.pb.err);
+                for (int u = 0; u < T::kUnits; ++u) {
+                    const int g = (loads + pl.value_load(b)) * T::kUnits + u;
+                    wait_stage(g);
                     if (!ok) break;
-                    p_phase ^= 1u << buf;
-                    const uint32_t acc = T::kGroups == 2 ? i > 1 : i > 0;
-                    const uint32_t o = tmem + T::kO + (T::kGroups == 2 ? buf * HD : 0);
+                    tc_fence_after();
+                    const uint32_t vd = v_lo + (g % T::kStages) * (T::kUnitBytes >> 4);
 #pragma unroll
-                    for (int u = 0; u < T::kUnits; ++u) {
-                        const int g = (loads + pl.value_load(b)) * T::kUnits + u;
-                        wait_stage(g);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t va = smem_u32(ring + (g % T::kStages) * T::kUnitBytes);
-#pragma unroll
-                        for (int kk = 0; kk < kBlock / 16; ++kk)
-                            umma_ts(o + u * T::kUnitDims, tmem + buf * 128 + kk * 8,
-                                    smem_desc_mn_sw128(va + kk * 16 * 128), kIdO,
-                                    (acc || kk > 0) ? 1u : 0u);
-                        if (pl.last_use(i)) umma_commit(&empty[g % T::kStages]);
-                    }
-                    if (T::kGroups == 1) umma_commit(&pv_done);
-                    if (ok && i + 2 < steps) issue_s(i + 2);
+                    for (int kk = 0; kk < kBlock / 16; ++kk)
+                        mma_ts(o + u * T::kUnitDims, tm + buf * 128 + kk * 8,
+                               vd + (kk * 16 * 128 >> 4), kDescHi, kIdO, (acc || kk > 0) ? 1u : 0u);
+                    if (pl.last_use(i)) mma_commit(&empty[g % T::kStages]);
                 }
-                umma_commit(&o_full);
-                loads += 2 * pl.n;
-                ++pieces;
+                if (T::kGroups == 1) mma_commit(&pv_done);
+                if (ok && i + 2 < steps) issue_s(i + 2);
             }
-            if (!ok && pieces > 0) {  // given up: the products in flight end first
-                const unsigned long long t0 = global_timer_ns();
-                while (!mbar_try_wait(&o_full, (uint32_t)(pieces - 1) & 1u) &&
-                       global_timer_ns() - t0 < kWaitLimitNs) {
-                }
+            mma_commit(&o_full);
+            loads += 2 * pl.n;
+            ++pieces;
+        }
+        if (!ok && pieces > 0) {  // given up: the products in flight end first
+            const unsigned long long t0 = global_timer_ns();
+            while (!mbar_try_wait(&o_full, (uint32_t)(pieces - 1) & 1u) &&
+                   global_timer_ns() - t0 < kWaitLimitNs) {
             }
         }
         __syncwarp();
