@@ -36,6 +36,9 @@ namespace nq {
 namespace {
 
 constexpr int kBlock = 128;  // keys per block, rows per query tile
+// The weights of a block's first kMost keys are handed over early, so that most
+// of P V runs while the rest are still being made.
+constexpr int kMost = 96;
 
 template <int HD>
 struct Tc {
@@ -82,6 +85,45 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
+}
+
+// Named barrier over `count` threads; whether any of them said so.
+__device__ __forceinline__ bool bar_any(int id, int count, bool x) {
+    int y;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+        : "=r"(y)
+        : "r"((int)x), "r"(id), "r"(count)
+        : "memory");
+    return y != 0;
+}
+
+// mbar_wait_or_abort() for the hand-overs between the MMA and softmax warps,
+// which happen every microsecond: a thread that suspends in try_wait wakes up
+// to 300 cycles after the last arrival, one that polls within 50.
+__device__ __forceinline__ bool mbar_poll_or_abort(uint64_t *bar, uint32_t parity,
+                                                   volatile int *abort, unsigned int *err) {
+    unsigned long long t0 = 0;
+    for (int i = 0;; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((i & 255) != 255) continue;
+        if (*abort) return false;
+        if (t0 == 0) t0 = global_timer_ns();
+        if (global_timer_ns() - t0 > kWaitLimitNs) {
+            *abort = 1;
+            atomicOr(err, kErrWaitTimeout);
+            return false;
+        }
+    }
 }
 
 // MMAs and commits run by a whole warp, one lane of which issues.  Under a
@@ -205,15 +247,18 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *qs = smem, *ring = smem + T::kGroups * T::kQBytes;
     uint8_t *outs = ring + T::kStages * T::kUnitBytes;
-    __shared__ __align__(8) uint64_t full[T::kStages], empty[T::kStages], s_full[2], p_ready[2];
+    __shared__ __align__(8) uint64_t full[T::kStages], empty[T::kStages], s_full[2];
+    __shared__ __align__(8) uint64_t p_most[2], p_rest[2];
     __shared__ __align__(8) uint64_t q_full, q_empty, o_full, pv_done;
     __shared__ uint32_t tmem_holder;
-    __shared__ int abort_flag, stop;
+    __shared__ int abort_flag;
     __shared__ float2 xml[T::kGroups == 2 ? 2 * kBlock : 1];
     __shared__ Job jobs[2];
     __shared__ __align__(8) uint64_t job_full[2], job_empty[2];
     volatile int *abort = &abort_flag;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (the shuffle tells the compiler that the roles' branches are warp-uniform)
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
     const int G = a.n_heads / a.n_kv, tok = kBlock / G, TT = T::kGroups * tok;
 
     pdl_launch_dependents();
@@ -224,7 +269,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_ready[i], 4);  // (one arrival per warp)
+            mbar_init(&p_most[i], 4);  // (one arrival per warp)
+            mbar_init(&p_rest[i], 4);
             mbar_init(&job_full[i], 1);
             mbar_init(&job_empty[i], 3 + 4 * T::kGroups);  // the other warps
         }
@@ -232,7 +278,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         mbar_init(&q_empty, 1);
         mbar_init(&o_full, 1);
         mbar_init(&pv_done, 1);
-        abort_flag = stop = 0;
+        abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
@@ -323,10 +369,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                        v_lo = desc_mn(smem_u32(ring));
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         int loads = 0, pieces = 0;
-        uint32_t p_phase = 0;  // bit: parity of that buffer's next p_ready
+        uint32_t p_phase = 0;  // bit: parity of that buffer's next p_most and p_rest
         bool ok = true;
         auto wait = [&](uint64_t *bar, uint32_t parity) {
-            return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, abort, a.pb.err)) != 0;
+            return __all_sync(0xffffffffu, mbar_poll_or_abort(bar, parity, abort, a.pb.err)) != 0;
         };
         auto wait_stage = [&](int g) {
             ok = ok && wait(&full[g % T::kStages], (uint32_t)(g / T::kStages) & 1u);
@@ -370,9 +416,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             if (ok && steps > 1) issue_s(1);
             for (int i = 0; ok && i < steps; ++i) {
                 const int b = pl.block(i), buf = i & 1;
-                ok = wait(&p_ready[buf], (p_phase >> buf) & 1u);
+                ok = wait(&p_most[buf], (p_phase >> buf) & 1u);
                 if (!ok) break;
-                p_phase ^= 1u << buf;
                 const uint32_t acc = T::kGroups == 2 ? i > 1 : i > 0;
                 const uint32_t o = tm + T::kO + (T::kGroups == 2 ? buf * HD : 0);
 #pragma unroll
@@ -383,9 +428,17 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     tc_fence_after();
                     const uint32_t vd = v_lo + (g % T::kStages) * (T::kUnitBytes >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < kBlock / 16; ++kk)
+                    for (int kk = 0; kk < kBlock / 16; ++kk) {
+                        if (u == 0 && kk == kMost / 16) {
+                            ok = wait(&p_rest[buf], (p_phase >> buf) & 1u);
+                            if (!ok) break;
+                            p_phase ^= 1u << buf;
+                            tc_fence_after();
+                        }
                         mma_ts(o + u * T::kUnitDims, tm + buf * 128 + kk * 8,
                                vd + (kk * 16 * 128 >> 4), kDescHi, kIdO, (acc || kk > 0) ? 1u : 0u);
+                    }
+                    if (!ok) break;
                     if (pl.last_use(i)) mma_commit(&empty[g % T::kStages]);
                 }
                 if (T::kGroups == 1) mma_commit(&pv_done);
@@ -455,13 +508,13 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             ok = ok && !*abort &&
                  mbar_wait_or_abort(&job_full[pieces & 1], (uint32_t)(pieces / 2) & 1u, abort,
                                     a.pb.err);
-            // (without the job nobody knows whether a barrier follows: both warpgroups stop)
-            if (T::kGroups == 2) {
-                if (!ok) stop = 1;
-                bar_sync(1, 256);
-                ok = !stop;
-            }
-            if (!__all_sync(0xffffffffu, ok) || job.n == 0) break;
+            // (one decision for both warpgroups: each takes part in the barrier below, or
+            // neither does)
+            if (T::kGroups == 2)
+                ok = !bar_any(1, 256, !ok);
+            else
+                ok = __all_sync(0xffffffffu, ok);
+            if (!ok || job.n == 0) break;
             const Piece &p = job.p;
             const Plan<HD> pl(p, tok);
             const int steps = pl.steps();
@@ -480,7 +533,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             for (int i = T::kGroups == 2 ? w : 0; i < steps; i += T::kGroups) {
                 const int buf = i & 1, b = pl.block(i);
                 ok = ok && !*abort &&
-                     mbar_wait_or_abort(&s_full[buf], (s_phase >> buf) & 1u, abort, a.pb.err);
+                     mbar_poll_or_abort(&s_full[buf], (s_phase >> buf) & 1u, abort, a.pb.err);
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
@@ -489,26 +542,28 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 tc_fence_after();
                 const uint32_t sc = tmem + lanes + buf * 128;
                 float s[128];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    tmem_ld_32x32b_x32(sc + j * 32,
-                                       *reinterpret_cast<uint32_t(*)[32]>(s + j * 32));
-                tmem_ld_wait();
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 const int key0 = (block0 + b) * kBlock;
-                if (key0 > full_to || key0 < full_from) {
-                    const int hi = pos - key0;
-                    const int lo = a.window > 0 ? hi - a.window + 1 : 0;
+                const bool masked = key0 > full_to || key0 < full_from;
+                const int hi = pos - key0, lo = a.window > 0 ? hi - a.window + 1 : 0;
+                tmem_ld_32x32b_x32(sc, *reinterpret_cast<uint32_t(*)[32]>(s));
+                tmem_ld_32x32b_x32(sc + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+                tmem_ld_wait();
+                tmem_ld_32x32b_x32(sc + 64, *reinterpret_cast<uint32_t(*)[32]>(s + 64));
+                tmem_ld_32x32b_x32(sc + 96, *reinterpret_cast<uint32_t(*)[32]>(s + 96));
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
-                        if (j > hi || j < lo) s[j] = -INFINITY;
-                }
-                float x[4] = {s[0], s[1], s[2], s[3]};
+                for (int c = 0; c < 128; c += 64) {
+                    if (c > 0) tmem_ld_wait();
+                    if (masked) {
 #pragma unroll
-                for (int j = 4; j < 128; j += 8) {
+                        for (int j = c; j < c + 64; ++j)
+                            if (j > hi || j < lo) s[j] = -INFINITY;
+                    }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[e] = j + 4 + e < 128 ? fmaxf(x[e], fmaxf(s[j + e], s[j + 4 + e]))
-                                               : fmaxf(x[e], s[j + e]);
+                    for (int j = c; j < c + 64; j += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            x[e] = fmaxf(x[e], fmaxf(s[j + e], s[j + 4 + e]));
                 }
                 const float mn = fmaxf(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
                 // (m == -inf: the difference is +inf, or NaN when the row has no key yet)
@@ -538,23 +593,6 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     m = mn;
                 }
                 first = false;
-                const float z = m == -INFINITY ? 0.f : m * cs;
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float2 x2 = fma2(make_float2(s[j * 32 + 2 * e], s[j * 32 + 2 * e + 1]),
-                                               make_float2(cs, cs), make_float2(-z, -z));
-                        const float e0 = ex2(x2.x), e1 = ex2(x2.y);
-                        sum[e & 1] = add2(sum[e & 1], make_float2(e0, e1));
-                        // rounded to the cache's type: both factors of an MMA are of one type
-                        pk[e] = pack_t2<F16>(e0, e1);
-                    }
-                    tmem_st_32x32b_x16(sc + j * 16, pk);
-                }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 const int key_hi = p.s.len - p.s.n + p.t1;
                 const int key_lo = a.window > 0 ? p.s.len - p.s.n + p.t0 - a.window + 1 : 0;
                 if (key0 < key_lo || key0 + kBlock > key_hi) {
@@ -579,10 +617,33 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
+                const float z = m == -INFINITY ? 0.f : m * cs;
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 x2 = fma2(make_float2(s[j * 32 + 2 * e], s[j * 32 + 2 * e + 1]),
+                                               make_float2(cs, cs), make_float2(-z, -z));
+                        const float e0 = ex2(x2.x), e1 = ex2(x2.y);
+                        sum[e & 1] = add2(sum[e & 1], make_float2(e0, e1));
+                        // rounded to the cache's type: both factors of an MMA are of one type
+                        pk[e] = pack_t2<F16>(e0, e1);
+                    }
+                    tmem_st_32x32b_x16(sc + j * 16, pk);
+                    if (j * 32 + 32 == kMost) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_most[buf]);
+                    }
+                }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_ready[buf]);
+                if (lane == 0) mbar_arrive(&p_rest[buf]);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             ok = ok && !*abort &&
                  mbar_wait_or_abort(&o_full, (uint32_t)pieces & 1u, abort, a.pb.err);
