@@ -169,15 +169,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     __syncthreads();
     pdl_wait();  // lengths, tables, q and the cache come from earlier kernels
 
-    const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x, a.least,
-                                        a.whole);
-    Cursor c = sh.c;
-    int64_t unit = sh.first;
+    const Tiling tl{TT, TT, a.window, a.whole};
+    Share sh = find_share<kBlock>(a.pb, a.n_kv, tl, blockIdx.x, gridDim.x, a.least);
     Piece p;
     int it = 0;  // blocks so far: stage it % kStages, parity it / kStages
 
     if (warp == kWarps) {
-        while (next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
+        while (next_piece<kBlock>(a.pb, a.n_kv, tl, sh, blockIdx.x, p)) {
             const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
             const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
             for (int k = p.k0; k < p.k1; ++k, ++it) {
@@ -209,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     bool note_left = false;
     uint32_t q[HD / 16][NT][2], qn[kAhead ? HD / 16 : 1][NT][2];
     Piece pn;
-    bool more = next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, pn);
+    bool more = next_piece<kBlock>(a.pb, a.n_kv, tl, sh, blockIdx.x, pn);
     if constexpr (kAhead) {
         if (more) load_q<HD, NT>(a, pn, G, qn);
     }
@@ -225,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
         } else {
             load_q<HD, NT>(a, p, G, q);
         }
-        more = next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, pn);
+        more = next_piece<kBlock>(a.pb, a.n_kv, tl, sh, blockIdx.x, pn);
         if constexpr (kAhead) {
             if (more) load_q<HD, NT>(a, pn, G, qn);
         }
@@ -447,18 +445,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
             }
         }
         if (warp == 0) {
-            if (!uncut && p.k0 == 0) {
+            if (p.parts > 0) {
                 note_left = true;
                 if (lane == 0)
-                    a.notes[blockIdx.x] = SplitNote{
-                        p.s.q0 + p.t0, p.h * G, p.t1 - p.t0,
-                        share_owner(sh.total, sh.n, unit + p.nb - 1) - (int)blockIdx.x + 1};
+                    a.notes[blockIdx.x] = SplitNote{p.s.q0 + p.t0, p.h * G, p.t1 - p.t0, p.parts};
             }
             if (lane == 0) stop = *abort;
         }
         bar_sync(1, kWarps * 32);
         if (stop) break;  // one decision for all four warps
-        unit += p.k1 - p.k0;
     }
     if (warp == 0 && lane == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
 }
@@ -674,7 +669,7 @@ cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
     a.n_kv = c.n_kv;
     a.window = c.window;
     a.scale = c.scale;
-    a.least = 1;
+    a.least = s.whole ? 1 : Tiling::kMost;
     a.whole = s.whole;
     // the largest power of two that divides the page size: no box crosses a page
     a.box = std::min(s.block, c.pb.page_size & -c.pb.page_size);

@@ -5,11 +5,12 @@
 //
 // A query tile is 128 rows (the G query heads of a key head times 128 / G
 // tokens), a key block 128 keys.  One CTA per SM, persistent over its pieces:
-//   loader warp   K and V blocks into a ring of stages by TMA (128-byte
-//                 swizzle, boxes of 16 to 128 keys x 64 dims)
+//   key and value warp   K and V blocks into a ring of stages each by TMA (128-byte
+//                 swizzle, boxes of 16 to 128 keys x 64 dims; a warp starts a box
+//                 about every 65 ns, so small pages ask for two warps)
 //   MMA warp      S = Q K^T (both in shared memory) and O += P V (P in TMEM, V as
 //                 it lies: keys x dims, the MN-major operand), one thread
-//   query warps   the next tile's queries, as soon as the last S that reads the
+//   query warp    the next tile's queries, as soon as the last S that reads the
 //                 present ones is done
 //   softmax       one row per thread: S from TMEM, a running maximum and sum,
 //                 P back into S's columns in 16 bits
@@ -43,9 +44,9 @@ constexpr int kMost = 96;
 template <int HD>
 struct Tc {
     static constexpr int kGroups = HD == 256 ? 1 : 2;       // softmax warpgroups
-    static constexpr int kMmaWarp = 4 * kGroups, kLoadWarp = kMmaWarp + 1;
-    static constexpr int kQueryWarp = kLoadWarp + 1;        // and the next
-    // A third (second) warpgroup of one MMA, one loader and two query warps.  With
+    static constexpr int kMmaWarp = 4 * kGroups, kKeyWarp = kMmaWarp + 1;
+    static constexpr int kValueWarp = kKeyWarp + 1, kQueryWarp = kValueWarp + 1;
+    // A third (second) warpgroup of MMA, key, value and query warp.  With
     // two softmax warpgroups registers are moved between them: 168 each at launch
     // (all of the SM's 64 K), then 208 for a softmax thread, which holds a row of 128
     // scores, and 88 for the others; 2 * 208 + 88 = 3 * 168.
@@ -54,11 +55,11 @@ struct Tc {
     static constexpr int kUnitDims = HD < 128 ? HD : 128;
     static constexpr int kUnits = HD / kUnitDims;
     static constexpr int kUnitBytes = kBlock * kUnitDims * 2;
-    static constexpr int kStages = HD == 64 ? 8 : 4;  // 128 KB
+    static constexpr int kStages = HD == 64 ? 4 : 2;  // of keys, and as many of values: 128 KB
     static constexpr int kQBytes = kBlock * HD * 2;
     static constexpr int kOutBytes = 2048;                  // a warp's 32 rows x 32 dims
     static constexpr int kSmem =
-        kGroups * kQBytes + kStages * kUnitBytes + 4 * kGroups * kOutBytes;
+        kGroups * kQBytes + 2 * kStages * kUnitBytes + 4 * kGroups * kOutBytes;
     static constexpr int kO = 256;                          // first TMEM column of O
     static constexpr int kRows = kGroups * kBlock;          // rows of a part
 };
@@ -195,48 +196,28 @@ struct Plan {
     __device__ __forceinline__ int steps() const { return two ? 2 * n : n; }
     __device__ __forceinline__ int block(int i) const { return two ? i >> 1 : i; }
     __device__ __forceinline__ bool last_use(int i) const { return !two || (i & 1); }
-    // place of block b's keys and values in the loads' order, which is that of
-    // their first use
-    __device__ __forceinline__ int key_load(int b) const {
-        return two ? 2 * b : (b == 0 ? 0 : 2 * b - 1);
-    }
-    __device__ __forceinline__ int value_load(int b) const {
-        return two ? 2 * b + 1 : (b < n - 1 ? 2 * b + 2 : 2 * n - 1);
-    }
 };
 
-// A piece as the loader warp, which alone walks the list, hands it to the others
-// (two slots, so that it runs a piece ahead).  parts: of a tile that this CTA
-// begins and does not finish, else 0; n == 0 ends the list.
+// A piece as the key warp, which alone walks the list, hands it to the others
+// (two slots, so that it runs a piece ahead); n: its blocks, 0 at the list's end.
 struct Job {
     Piece p;
-    int n, parts;
+    int n;
 };
 
-// One ring stage: kUnitDims dims from u * kUnitDims on of block `blk`, as columns
-// of 64 dims (16 KB each), in boxes of a.box keys; a box of all 128 keys takes
-// both columns.  Boxes without a visible key of the piece read as zeros (page n_pages).
-template <int HD>
-__device__ __forceinline__ void load_unit(const PagedAttnArgs &a, const CUtensorMap *map,
-                                          const Piece &p, int blk, int u, int key_lo, int key_hi,
-                                          uint8_t *stage, uint64_t *bar) {
-    using T = Tc<HD>;
-    constexpr int kCols = T::kUnitDims / 64;
-    const int lane = threadIdx.x & 31;
-    const int per = kCols / a.box_cols;  // boxes beside one another: 1 or kCols
-    const int r = lane / per, col = lane % per;
-    const bool on = r < kBlock / a.box;
-    const int key = blk * kBlock + r * a.box;
-    int page = a.pb.n_pages, slot = 0;
+// Where a lane's box of a key block lies: its page (n_pages, whose reads give
+// zeros, for a box without a visible key of the piece) and row in the page.
+struct Place {
+    int page, slot;
+};
+__device__ __forceinline__ Place box_place(const PagedAttnArgs &a, int row, int key, bool on,
+                                           int key_lo, int key_hi) {
+    Place p{a.pb.n_pages, 0};
     if (on && key < key_hi && key + a.box > key_lo) {
-        page = page_of(a.pb, p.s.row, key);
-        slot = key % a.pb.page_size;
+        p.page = page_of(a.pb, row, key);
+        p.slot = key % a.pb.page_size;
     }
-    if (lane == 0) mbar_expect_tx(bar, T::kUnitBytes);
-    __syncwarp();
-    if (on)
-        tma_load_5d(stage + col * (kBlock * 128) + r * a.box * 128, map, bar, 0, slot,
-                    u * kCols + col, p.h, page);
+    return p;
 }
 
 template <int HD, bool F16>
@@ -245,9 +226,13 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     const PagedAttnArgs a) {
     using T = Tc<HD>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t *qs = smem, *ring = smem + T::kGroups * T::kQBytes;
-    uint8_t *outs = ring + T::kStages * T::kUnitBytes;
-    __shared__ __align__(8) uint64_t full[T::kStages], empty[T::kStages], s_full[2];
+    uint8_t *qs = smem, *ring_k = smem + T::kGroups * T::kQBytes;
+    uint8_t *ring_v = ring_k + T::kStages * T::kUnitBytes;
+    uint8_t *outs = ring_v + T::kStages * T::kUnitBytes;
+    // a ring of keys and one of values: a ring has one producer, or its waits would be
+    // ambiguous
+    __shared__ __align__(8) uint64_t full_k[T::kStages], empty_k[T::kStages];
+    __shared__ __align__(8) uint64_t full_v[T::kStages], empty_v[T::kStages], s_full[2];
     __shared__ __align__(8) uint64_t p_most[2], p_rest[2];
     __shared__ __align__(8) uint64_t q_full, q_empty, o_full, pv_done;
     __shared__ uint32_t tmem_holder;
@@ -264,8 +249,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < T::kStages; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&full_k[i], 1);
+            mbar_init(&empty_k[i], 1);
+            mbar_init(&full_v[i], 1);
+            mbar_init(&empty_v[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
@@ -274,7 +261,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             mbar_init(&job_full[i], 1);
             mbar_init(&job_empty[i], 3 + 4 * T::kGroups);  // the other warps
         }
-        mbar_init(&q_full, 2);
+        mbar_init(&q_full, 1);
         mbar_init(&q_empty, 1);
         mbar_init(&o_full, 1);
         mbar_init(&pv_done, 1);
@@ -295,86 +282,89 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
 
     if (warp >= 4 * T::kGroups) {
     if constexpr (T::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == T::kLoadWarp) {
-        const Share sh = find_share<kBlock>(a.pb, a.n_kv, TT, a.window, blockIdx.x, gridDim.x,
-                                            a.least, a.whole);
-        Cursor c = sh.c;
+    // K and V of a block: kUnitDims dims per ring stage, as columns of 64 dims (16 KB
+    // each), in boxes of a.box keys, a lane each; a box of all 128 keys takes both
+    // columns.  The pages of the next block are looked up ahead.
+    auto load = [&](const Piece &p, const CUtensorMap *map, uint8_t *ring, uint64_t *full,
+                    uint64_t *empty, int &g) {
+        constexpr int kCols = T::kUnitDims / 64;
+        const int per = kCols / a.box_cols, box_r = lane / per, box_c = lane % per;
+        const bool on = box_r < kBlock / a.box;
+        const uint32_t box_at = box_c * (kBlock * 128) + box_r * a.box * 128;
+        const int n = p.k1 - p.k0;
+        const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
+        const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+        const int key0 = (p.lo + p.k0) * kBlock + box_r * a.box;
+        Place next = box_place(a, p.s.row, key0, on, key_lo, key_hi);
+        for (int b = 0; b < n; ++b) {
+            const Place at = next;
+            next = box_place(a, p.s.row, key0 + (b + 1) * kBlock, on && b + 1 < n, key_lo, key_hi);
+#pragma unroll
+            for (int u = 0; u < T::kUnits; ++u, ++g) {
+                const int st = g % T::kStages;
+                if (!mbar_wait_or_abort(&empty[st], (uint32_t)(g / T::kStages + 1) & 1u, abort,
+                                        a.pb.err))
+                    return false;
+                if (lane == 0) mbar_expect_tx(&full[st], T::kUnitBytes);
+                __syncwarp();
+                if (on)
+                    tma_load_5d(ring + st * T::kUnitBytes + box_at, map, &full[st], 0, at.slot,
+                                u * kCols + box_c, p.h, at.page);
+            }
+        }
+        return true;
+    };
+    if (warp == T::kKeyWarp) {
+        const Tiling tl{TT, T::kGroups == 2 ? tok : TT, a.window, a.whole};
+        Share sh = find_share<kBlock>(a.pb, a.n_kv, tl, blockIdx.x, gridDim.x, a.least);
         Piece p;
-        int64_t unit = sh.first;
-        int g = 0, jobs_out = 0;  // stages filled and jobs handed out so far
+        int filled = 0, jobs_out = 0;
         bool ok = true, note_left = false;
-        auto hand_out = [&](int n, int parts) {
+        auto hand_out = [&](int n) {
             const int slot = jobs_out & 1;
             ok = mbar_wait_or_abort(&job_empty[slot], (uint32_t)(jobs_out / 2 + 1) & 1u, abort,
                                     a.pb.err);
             if (ok && lane == 0) {
                 jobs[slot].p = p;
                 jobs[slot].n = n;
-                jobs[slot].parts = parts;
                 mbar_arrive(&job_full[slot]);
             }
             ++jobs_out;
         };
-        while (ok && next_piece<kBlock>(a.pb, a.n_kv, TT, a.window, a.whole, c, p)) {
-            int parts = 0;
-            if (p.k0 == 0 && p.k1 < p.nb) {
-                parts = share_owner(sh.total, sh.n, unit + p.nb - 1) - (int)blockIdx.x + 1;
-                note_left = true;
-            }
-            unit += p.k1 - p.k0;
-            hand_out(p.k1 - p.k0, parts);
-            if (!ok) break;
-            const Plan<HD> pl(p, tok);
-            const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
-            const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
-            for (int t = 0; ok && t < 2 * pl.n; ++t) {
-                bool is_v;
-                int b;
-                if (pl.two) {
-                    is_v = t & 1;
-                    b = t >> 1;
-                } else if (t == 0 || t == 2 * pl.n - 1) {
-                    is_v = t != 0;
-                    b = is_v ? pl.n - 1 : 0;
-                } else {
-                    is_v = !(t & 1);
-                    b = is_v ? (t - 2) / 2 : (t + 1) / 2;
-                }
-                for (int u = 0; ok && u < T::kUnits; ++u, ++g) {
-                    const int st = g % T::kStages;
-                    ok = mbar_wait_or_abort(&empty[st], (uint32_t)(g / T::kStages + 1) & 1u, abort,
-                                            a.pb.err);
-                    if (!ok) break;
-                    load_unit<HD>(a, is_v ? &mv : &mk, p, p.lo + p.k0 + b, u, key_lo, key_hi,
-                                  ring + st * T::kUnitBytes, &full[st]);
-                }
-            }
+        while (ok && next_piece<kBlock>(a.pb, a.n_kv, tl, sh, blockIdx.x, p)) {
+            note_left |= p.parts > 0;
+            hand_out(p.k1 - p.k0);
+            ok = ok && load(p, &mk, ring_k, full_k, empty_k, filled);
         }
-        if (ok) hand_out(0, 0);
+        if (ok) hand_out(0);
         if (lane == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
-        if (!ok || *abort) {  // given up: the copies in flight end before this CTA does
-            for (int j = max(0, g - T::kStages); j < g; ++j) {
-                const unsigned long long t0 = global_timer_ns();
-                while (!mbar_try_wait(&full[j % T::kStages], (uint32_t)(j / T::kStages) & 1u) &&
-                       global_timer_ns() - t0 < kWaitLimitNs) {
-                }
-            }
+    } else if (warp == T::kValueWarp) {
+        int filled = 0;
+        for (int pieces = 0;; ++pieces) {
+            const int slot = pieces & 1;
+            if (!mbar_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort, a.pb.err) ||
+                jobs[slot].n == 0)
+                break;
+            const Piece p = jobs[slot].p;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&job_empty[slot]);
+            if (!load(p, &mv, ring_v, full_v, empty_v, filled)) break;
         }
     } else if (warp == T::kMmaWarp) {
         constexpr uint32_t kIdS = F16 ? idesc_f16_f32(128, 128) : idesc_bf16_f32(128, 128);
         constexpr uint32_t kIdO = (F16 ? idesc_f16_f32(128, T::kUnitDims)
                                        : idesc_bf16_f32(128, T::kUnitDims)) |
                                   (1u << 16);  // B: N along memory
-        const uint32_t q_lo = desc_k(smem_u32(qs)), k_lo = desc_k(smem_u32(ring)),
-                       v_lo = desc_mn(smem_u32(ring));
+        const uint32_t q_lo = desc_k(smem_u32(qs)), k_lo = desc_k(smem_u32(ring_k)),
+                       v_lo = desc_mn(smem_u32(ring_v));
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        int loads = 0, pieces = 0;
+        int blocks = 0, pieces = 0;  // finished
         uint32_t p_phase = 0;  // bit: parity of that buffer's next p_most and p_rest
         bool ok = true;
         auto wait = [&](uint64_t *bar, uint32_t parity) {
             return __all_sync(0xffffffffu, mbar_poll_or_abort(bar, parity, abort, a.pb.err)) != 0;
         };
-        auto wait_stage = [&](int g) {
+        auto wait_stage = [&](uint64_t *full, int g) {
             ok = ok && wait(&full[g % T::kStages], (uint32_t)(g / T::kStages) & 1u);
         };
         while (ok) {
@@ -394,8 +384,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 const uint32_t qd = q_lo + (pl.two && buf ? T::kQBytes >> 4 : 0);
 #pragma unroll
                 for (int u = 0; u < T::kUnits; ++u) {
-                    const int g = (loads + pl.key_load(b)) * T::kUnits + u;
-                    wait_stage(g);
+                    const int g = (blocks + b) * T::kUnits + u;
+                    wait_stage(full_k, g);
                     if (!ok) return;
                     tc_fence_after();
                     const uint32_t kd = k_lo + (g % T::kStages) * (T::kUnitBytes >> 4);
@@ -407,7 +397,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                                qd + (u * (T::kUnitDims / 64) * (kBlock * 128) >> 4) + off, kDescHi,
                                kd + off, kDescHi, kIdS, (u > 0 || kk > 0) ? 1u : 0u);
                     }
-                    if (pl.last_use(i)) mma_commit(&empty[g % T::kStages]);
+                    if (pl.last_use(i)) mma_commit(&empty_k[g % T::kStages]);
                 }
                 mma_commit(&s_full[buf]);
                 if (i + 1 == steps) mma_commit(&q_empty);
@@ -422,8 +412,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 const uint32_t o = tm + T::kO + (T::kGroups == 2 ? buf * HD : 0);
 #pragma unroll
                 for (int u = 0; u < T::kUnits; ++u) {
-                    const int g = (loads + pl.value_load(b)) * T::kUnits + u;
-                    wait_stage(g);
+                    const int g = (blocks + b) * T::kUnits + u;
+                    wait_stage(full_v, g);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t vd = v_lo + (g % T::kStages) * (T::kUnitBytes >> 4);
@@ -439,13 +429,13 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                                vd + (kk * 16 * 128 >> 4), kDescHi, kIdO, (acc || kk > 0) ? 1u : 0u);
                     }
                     if (!ok) break;
-                    if (pl.last_use(i)) mma_commit(&empty[g % T::kStages]);
+                    if (pl.last_use(i)) mma_commit(&empty_v[g % T::kStages]);
                 }
                 if (T::kGroups == 1) mma_commit(&pv_done);
                 if (ok && i + 2 < steps) issue_s(i + 2);
             }
             mma_commit(&o_full);
-            loads += 2 * pl.n;
+            blocks += pl.n;
             ++pieces;
         }
         if (!ok && pieces > 0) {  // given up: the products in flight end first
@@ -455,10 +445,9 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             }
         }
         __syncwarp();
-    } else {
+    } else if (warp == T::kQueryWarp) {
         // ---------------------------------------------------------- query rows
-        constexpr int kLanes = HD / 8, kStep = 64 / kLanes;  // lanes per row, rows at a time
-        const int lid = threadIdx.x - T::kQueryWarp * 32;
+        constexpr int kLanes = HD / 8, kStep = 32 / kLanes;  // lanes per row, rows at a time
         const uint32_t inv_g = (65535 + G) / G;  // r / G = r * inv_g >> 16 for r < 128
         for (int pieces = 0;; ++pieces) {
             const int slot = pieces & 1;
@@ -472,11 +461,11 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             const bool two = T::kGroups == 2 && p.t1 - p.t0 > tok;
             for (int sub = 0; sub <= (two ? 1 : 0); ++sub) {
                 const int t0 = p.t0 + sub * tok, valid = (min(t0 + tok, p.t1) - t0) * G;
-                const int ch = lid % kLanes;
+                const int ch = lane % kLanes;
                 // the K-major layout with 128-byte swizzle, columns of 64 dims
                 uint8_t *dst = qs + sub * T::kQBytes + (ch >> 3) * (kBlock * 128);
 #pragma unroll 4
-                for (int r = lid / kLanes; r < kBlock; r += kStep) {
+                for (int r = lane / kLanes; r < kBlock; r += kStep) {
                     const int t = (int)((uint32_t)r * inv_g >> 16), g = r - t * G;
                     const uint16_t *src = a.q + (int64_t)(p.s.q0 + t0 + (r < valid ? t : 0)) * a.q_ld +
                                           (int64_t)(p.h * G + (r < valid ? g : 0)) * HD + ch * 8;
@@ -498,7 +487,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
         const uint32_t inv_g = (65535 + G) / G;  // r / G = r * inv_g >> 16 for r < 128
-        int loads = 0, pieces = 0, pvs = 0;
+        int blocks = 0, pieces = 0, pvs = 0;
         uint32_t s_phase = 0;
         bool ok = true;
         while (true) {
@@ -600,14 +589,19 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     // weight of 0 would reach the sum
                     const int key = key0 + r;
                     const bool clear = (!pl.two || w == 0) && (key < key_lo || key >= key_hi);
+                    // (256 dims: the stage's last values may still be under way, and a wait two
+                    // phases ahead would be ambiguous)
+                    if (T::kGroups == 1 && i > 0)
+                        ok = ok && mbar_wait_or_abort(&pv_done, (uint32_t)(pvs + i - 1) & 1u, abort,
+                                                      a.pb.err);
 #pragma unroll
                     for (int u = 0; u < T::kUnits; ++u) {
-                        const int g = (loads + pl.value_load(b)) * T::kUnits + u;
-                        ok = ok && mbar_wait_or_abort(&full[g % T::kStages],
+                        const int g = (blocks + b) * T::kUnits + u;
+                        ok = ok && mbar_wait_or_abort(&full_v[g % T::kStages],
                                                       (uint32_t)(g / T::kStages) & 1u, abort,
                                                       a.pb.err);
                         if (ok && clear) {
-                            uint8_t *v = ring + (g % T::kStages) * T::kUnitBytes + r * 128;
+                            uint8_t *v = ring_v + (g % T::kStages) * T::kUnitBytes + r * 128;
 #pragma unroll
                             for (int j = 0; j < T::kUnitDims / 8; ++j)
                                 *reinterpret_cast<uint4 *>(v + (j >> 3) * (kBlock * 128) +
@@ -729,12 +723,12 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     *reinterpret_cast<float2 *>(a.part_ml + ((int64_t)slot * T::kRows + row) * 2) =
                         make_float2(M * cs, L);
             }
-            if (threadIdx.x == 0 && job.parts > 0)
-                a.notes[blockIdx.x] = SplitNote{p.s.q0 + p.t0, p.h * G, p.t1 - p.t0, job.parts};
+            if (threadIdx.x == 0 && job.p.parts > 0)
+                a.notes[blockIdx.x] = SplitNote{p.s.q0 + p.t0, p.h * G, p.t1 - p.t0, p.parts};
             // (the next piece's first product into O waits for this warpgroup's weights,
             // and the barrier above for both warpgroups)
             tc_fence_before();
-            loads += 2 * pl.n;
+            blocks += pl.n;
             pvs += steps;
             __syncwarp();
             if (lane == 0) mbar_arrive(&job_empty[pieces & 1]);
@@ -744,6 +738,11 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (*abort) {  // given up: the copies in flight end before this CTA does (they take microseconds)
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 10000000ull) {
+        }
+    }
     if (warp == T::kMmaWarp) tmem_dealloc(tmem, 512);
 }
 

@@ -95,12 +95,22 @@ __device__ __forceinline__ KeyRange key_range(const SeqView &s, int t0, int t1, 
     return r;
 }
 
-// A position in the list of all key blocks of a call: entry b, key head h,
-// place t in the order of the token tiles, and `off` blocks into that tile's
-// `nb`; `left` is what the CTA still has to do.
+// How a kernel cuts an entry's new tokens: tiles of TT tokens.  A key block costs
+// 3 units of work for a tile of up to `half` tokens and 4 for a larger one
+// (attn_paged_tc.cu, 1.6 and 2.2 us at 128 dims).
+struct Tiling {
+    static constexpr int kMost = 4;
+    int TT, half, window;
+    bool whole;  // a tile counts as one unit and is never cut
+    __device__ __forceinline__ int weight(int t0, int t1) const { return t1 - t0 > half ? 4 : 3; }
+};
+
+// A position in the list of all units of a call: entry b, key head h, place t in
+// the order of the token tiles, and `off` units into that tile; `at` is its
+// number and `left` what the CTA still has to do.
 struct Cursor {
     int b, h, t, off;
-    int64_t left;
+    int64_t at, left;
     SeqView s;
 };
 
@@ -110,22 +120,28 @@ struct Cursor {
 // beginnings and ends cost more than their products.
 __device__ __forceinline__ int tile_at(int i, int n) { return i & 1 ? n - 1 - (i >> 1) : i >> 1; }
 
-// The list: entries in order, in each its key heads, in each the token tiles
-// (TT tokens) in tile_at()'s order, in each its key blocks.  Neighbouring CTAs therefore read the
-// same head's keys at the same time.  CTA c of n takes the blocks
-// [c * total / n, (c + 1) * total / n), so that all CTAs get the same number
-// whatever the lengths are; a tile cut by such a border is finished by
-// a merge kernel.  Where no sequence can be long (`whole`) a tile counts as
-// one and is never cut: no parts, and no merge.
+// Units of the tile at place i of `tiles`.
 template <int BK>
-__device__ __forceinline__ int64_t entry_blocks_warp(const SeqView &s, int TT, int window,
-                                                     bool whole) {
-    // blocks of one head of this lane's entry; the lanes sum long entries together
+__device__ __forceinline__ int tile_units(const SeqView &s, const Tiling &tl, int i, int tiles) {
+    const int t0 = tile_at(i, tiles) * tl.TT, t1 = min(t0 + tl.TT, s.n);
+    return key_range<BK>(s, t0, t1, tl.window).nb * tl.weight(t0, t1);
+}
+
+// The list: entries in order, in each its key heads, in each the token tiles in
+// tile_at()'s order, in each its key blocks.  Neighbouring CTAs therefore read
+// the same head's keys at the same time.  CTA c of n takes the units
+// [c * total / n, (c + 1) * total / n) (a block goes with its first unit), so that all CTAs get the same work whatever the lengths are; a
+// tile cut by such a border is finished by a merge kernel.  Where no sequence
+// can be long (`whole`) a tile counts as one and is never cut: no parts, and no
+// merge.
+template <int BK>
+__device__ __forceinline__ int64_t entry_units_warp(const SeqView &s, const Tiling &tl) {
+    // units of one head of this lane's entry; the lanes sum long entries together
     const int lane = threadIdx.x & 31;
-    const int tiles = (s.n + TT - 1) / TT;
-    if (whole) return tiles;
+    const int tiles = (s.n + tl.TT - 1) / tl.TT;
+    if (tl.whole) return tiles;
     int64_t mine = 0;
-    if (tiles == 1) mine = key_range<BK>(s, 0, s.n, window).nb;
+    if (tiles == 1) mine = tile_units<BK>(s, tl, 0, 1);
     unsigned todo = __ballot_sync(0xffffffffu, tiles > 1);
     while (todo) {
         const int src = __ffs(todo) - 1;
@@ -133,10 +149,9 @@ __device__ __forceinline__ int64_t entry_blocks_warp(const SeqView &s, int TT, i
         SeqView o;
         o.n = __shfl_sync(0xffffffffu, s.n, src);
         o.len = __shfl_sync(0xffffffffu, s.len, src);
-        const int ot = (o.n + TT - 1) / TT;
+        const int ot = (o.n + tl.TT - 1) / tl.TT;
         int64_t sum = 0;
-        for (int t = lane; t < ot; t += 32)
-            sum += key_range<BK>(o, t * TT, min((t + 1) * TT, o.n), window).nb;
+        for (int t = lane; t < ot; t += 32) sum += tile_units<BK>(o, tl, t, ot);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (lane == src) mine = sum;
@@ -154,12 +169,11 @@ __device__ __forceinline__ int64_t warp_inclusive(int64_t v) {
     return v;
 }
 
-// What a CTA does: its first block and how many.
+// What a CTA does.
 struct Share {
-    int64_t total;   // blocks of the call
-    int64_t first;   // this CTA's first
+    int64_t total;   // units of the call
     int n;           // CTAs that take part
-    Cursor c;        // at `first`; c.left blocks
+    Cursor c;        // at this CTA's first unit; c.left of them
 };
 
 // a * b / c; in 32 bits, which is several times faster, where the product fits
@@ -169,17 +183,18 @@ __device__ __forceinline__ int64_t mul_div(int64_t a, int64_t b, int64_t c) {
     return a * b / c;
 }
 
-// CTAs that take part in a call of `total` blocks: no share is smaller than
-// `least` blocks.
+// CTAs that take part in a call of `total` units: no share is smaller than
+// `least` units (at least a block's: every share between a tile's first and
+// last one then holds a block of it).
 __device__ __forceinline__ int sharers(int64_t total, int grid, int least) {
     if (total >= (int64_t)grid * least) return grid;
-    const int n = ((int)total + least - 1) / least;
+    const int n = (int)total / least;
     return n > 0 ? n : 1;
 }
 __device__ __forceinline__ int64_t share_start(int64_t total, int n, int c) {
     return mul_div(c, total, n);
 }
-// the CTA whose share holds block u
+// the CTA whose share holds unit u
 __device__ __forceinline__ int share_owner(int64_t total, int n, int64_t u) {
     if ((u + 1) * n - 1 < (1ll << 32) && total < (1ll << 32))
         return (int)((uint32_t)((u + 1) * n - 1) / (uint32_t)total);
@@ -188,8 +203,8 @@ __device__ __forceinline__ int share_owner(int64_t total, int n, int64_t u) {
 
 // Run by one whole warp.
 template <int BK>
-__device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int TT, int window,
-                                            int cta, int grid, int least, bool whole) {
+__device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, const Tiling &tl,
+                                            int cta, int grid, int least) {
     const int lane = threadIdx.x & 31;
     Share sh;
     SeqView s{0, 0, 0, 0};
@@ -197,55 +212,50 @@ __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, int 
     for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
         s = SeqView{0, 0, 0, 0};
         if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
-        head = entry_blocks_warp<BK>(s, TT, window, whole);
+        head = entry_units_warp<BK>(s, tl);
         total += head;
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     sh.total = total * n_kv;
     sh.n = sharers(sh.total, grid, least);
-    sh.first = 0;
-    sh.c = Cursor{0, 0, 0, 0, 0, SeqView{0, 0, 0, 0}};
+    sh.c = Cursor{0, 0, 0, 0, 0, 0, SeqView{0, 0, 0, 0}};
     if (sh.total == 0 || cta >= sh.n) return sh;
-    sh.first = share_start(sh.total, sh.n, cta);
-    sh.c.left = share_start(sh.total, sh.n, cta + 1) - sh.first;
+    Cursor &c = sh.c;
+    c.at = share_start(sh.total, sh.n, cta);
+    c.left = share_start(sh.total, sh.n, cta + 1) - c.at;
     int64_t before = 0;
     for (int b0 = 0; b0 < pb.n_seqs; b0 += 32) {
         if (pb.n_seqs > 32) {  // (else the first pass left them)
             s = SeqView{0, 0, 0, 0};
             if (b0 + lane < pb.n_seqs) s = seq_view(pb, b0 + lane);
-            head = entry_blocks_warp<BK>(s, TT, window, whole);
+            head = entry_units_warp<BK>(s, tl);
         }
         const int64_t end = before + warp_inclusive(head * n_kv);
-        const unsigned past = __ballot_sync(0xffffffffu, end > sh.first);
+        const unsigned past = __ballot_sync(0xffffffffu, end > c.at);
         if (past) {
             const int src = __ffs(past) - 1;
-            Cursor &c = sh.c;
             c.b = b0 + src;
             c.s.row = __shfl_sync(0xffffffffu, s.row, src);
             c.s.q0 = __shfl_sync(0xffffffffu, s.q0, src);
             c.s.n = __shfl_sync(0xffffffffu, s.n, src);
             c.s.len = __shfl_sync(0xffffffffu, s.len, src);
             const int64_t per = __shfl_sync(0xffffffffu, head, src);
-            int64_t at = sh.first - (__shfl_sync(0xffffffffu, end, src) - per * n_kv);
+            int64_t at = c.at - (__shfl_sync(0xffffffffu, end, src) - per * n_kv);
             c.h = (int)mul_div(at, 1, per);
             at -= c.h * per;
-            const int tiles = (c.s.n + TT - 1) / TT;
+            const int tiles = (c.s.n + tl.TT - 1) / tl.TT;
             int64_t seen = 0;
             for (int i0 = 0; i0 < tiles; i0 += 32) {
-                int64_t nb = 0;
-                if (whole) {
-                    nb = i0 + lane < tiles;
-                } else if (i0 + lane < tiles) {
-                    const int t = tile_at(i0 + lane, tiles);
-                    nb = key_range<BK>(c.s, t * TT, min((t + 1) * TT, c.s.n), window).nb;
-                }
-                const int64_t e = seen + warp_inclusive(nb);
+                int64_t u = 0;
+                if (i0 + lane < tiles)
+                    u = tl.whole ? 1 : tile_units<BK>(c.s, tl, i0 + lane, tiles);
+                const int64_t e = seen + warp_inclusive(u);
                 const unsigned over = __ballot_sync(0xffffffffu, e > at);
                 if (over) {
                     const int l = __ffs(over) - 1;
                     c.t = i0 + l;
-                    c.off = (int)(at - __shfl_sync(0xffffffffu, e - nb, l));
+                    c.off = (int)(at - __shfl_sync(0xffffffffu, e - u, l));
                     break;
                 }
                 seen = __shfl_sync(0xffffffffu, e, 31);
@@ -263,39 +273,56 @@ struct Piece {
     SeqView s;
     int h, t0, t1;     // key head; new tokens [t0, t1)
     int lo, k0, k1, nb;
+    int parts;         // of a tile that this piece begins and does not finish; else 0
 };
 
-// Takes the next piece of the cursor and steps past it; false when done.
-// (Any thread: no warp-wide step.)
+// Takes the next piece of a share and steps past it; false when done.  (Any
+// thread: no warp-wide step.)
 template <int BK>
-__device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, int TT, int window,
-                                           bool whole, Cursor &c, Piece &p) {
-    if (c.left <= 0) return false;
-    p.s = c.s;
-    p.h = c.h;
-    const int tiles = (c.s.n + TT - 1) / TT;
-    p.t0 = tile_at(c.t, tiles) * TT;
-    p.t1 = min(p.t0 + TT, c.s.n);
-    const KeyRange r = key_range<BK>(c.s, p.t0, p.t1, window);
-    p.lo = r.lo;
-    p.nb = r.nb;
-    p.k0 = c.off;
-    p.k1 = whole ? r.nb : (int)min((int64_t)r.nb, c.off + c.left);
-    c.left -= whole ? 1 : p.k1 - p.k0;
-    c.off = p.k1;
-    if (p.k1 == r.nb && c.left > 0) {
-        c.off = 0;
-        if (++c.t == tiles) {
-            c.t = 0;
-            if (++c.h == n_kv) {
-                c.h = 0;
-                do {
-                    c.s = seq_view(pb, ++c.b);
-                } while (c.s.n == 0);
+__device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, const Tiling &tl,
+                                           Share &sh, int cta, Piece &p) {
+    Cursor &c = sh.c;
+    while (c.left > 0) {
+        p.s = c.s;
+        p.h = c.h;
+        const int tiles = (c.s.n + tl.TT - 1) / tl.TT;
+        p.t0 = tile_at(c.t, tiles) * tl.TT;
+        p.t1 = min(p.t0 + tl.TT, c.s.n);
+        const KeyRange r = key_range<BK>(c.s, p.t0, p.t1, tl.window);
+        p.lo = r.lo;
+        p.nb = r.nb;
+        p.k0 = 0;
+        p.k1 = r.nb;
+        p.parts = 0;
+        int end = 1, off = 1;  // the tile's units, and those before the next piece
+        if (!tl.whole) {
+            const int w = tl.weight(p.t0, p.t1);
+            end = r.nb * w;
+            off = (int)min((int64_t)end, c.off + c.left);
+            p.k0 = (c.off + w - 1) / w;
+            p.k1 = (off + w - 1) / w;
+            if (p.k0 == 0 && p.k1 < r.nb)
+                p.parts = share_owner(sh.total, sh.n, c.at - c.off + end - w) - cta + 1;
+        }
+        const int took = off - c.off;
+        c.left -= took;
+        c.at += took;
+        c.off = off;
+        if (off == end) {
+            c.off = 0;
+            if (c.left > 0 && ++c.t == tiles) {
+                c.t = 0;
+                if (++c.h == n_kv) {
+                    c.h = 0;
+                    do {
+                        c.s = seq_view(pb, ++c.b);
+                    } while (c.s.n == 0);
+                }
             }
         }
+        if (p.k0 < p.k1) return true;
     }
-    return true;
+    return false;
 }
 
 // page of key `key` of table row `row`; n_pages (whose reads give zeros) when
@@ -322,7 +349,7 @@ struct PagedAttnArgs {
     int64_t q_ld, out_ld;
     int n_heads, n_kv, window;
     int box, box_cols;   // keys and columns of 64 dims per TMA box
-    int least;           // fewest key blocks (tiles, when whole) of a CTA's share
+    int least;           // fewest units of a CTA's share
     bool whole;          // tiles are not cut
     float scale;
     SplitNote *notes;    // [CTAs]
