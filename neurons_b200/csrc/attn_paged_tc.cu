@@ -222,8 +222,8 @@ __device__ __forceinline__ Place box_place(const PagedAttnArgs &a, int row, int 
 
 template <int HD, bool F16>
 __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
-    const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-    const PagedAttnArgs a) {
+    const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+    const __grid_constant__ CUtensorMap mv, const PagedAttnArgs a) {
     using T = Tc<HD>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *qs = smem, *ring_k = smem + T::kGroups * T::kQBytes;
@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         mbar_init(&pv_done, 1);
         abort_flag = 0;
         fence_barrier_init();
+        prefetch_tmap(&mq);
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
     }
@@ -447,37 +448,24 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         __syncwarp();
     } else if (warp == T::kQueryWarp) {
         // ---------------------------------------------------------- query rows
-        constexpr int kLanes = HD / 8, kStep = 32 / kLanes;  // lanes per row, rows at a time
-        const uint32_t inv_g = (65535 + G) / G;  // r / G = r * inv_g >> 16 for r < 128
-        for (int pieces = 0;; ++pieces) {
+        // G heads of tok tokens are a tile's rows in their order; the rows of a tile's
+        // missing tokens hold another sequence's, or zeros: their scores are masked.
+        for (int pieces = 0; lane == 0; ++pieces) {
             const int slot = pieces & 1;
-            if (!mbar_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort, a.pb.err))
+            if (!mbar_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort, a.pb.err) ||
+                jobs[slot].n == 0)
                 break;
-            if (jobs[slot].n == 0) break;
-            const Piece p = jobs[slot].p;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&job_empty[slot]);
+            const int row = jobs[slot].p.s.q0 + jobs[slot].p.t0, h = jobs[slot].p.h * G;
+            const int subs = Plan<HD>(jobs[slot].p, tok).two ? 2 : 1;
+            mbar_arrive(&job_empty[slot]);
             if (!mbar_wait_or_abort(&q_empty, (uint32_t)(pieces + 1) & 1u, abort, a.pb.err)) break;
-            const bool two = T::kGroups == 2 && p.t1 - p.t0 > tok;
-            for (int sub = 0; sub <= (two ? 1 : 0); ++sub) {
-                const int t0 = p.t0 + sub * tok, valid = (min(t0 + tok, p.t1) - t0) * G;
-                const int ch = lane % kLanes;
-                // the K-major layout with 128-byte swizzle, columns of 64 dims
-                uint8_t *dst = qs + sub * T::kQBytes + (ch >> 3) * (kBlock * 128);
-#pragma unroll 4
-                for (int r = lane / kLanes; r < kBlock; r += kStep) {
-                    const int t = (int)((uint32_t)r * inv_g >> 16), g = r - t * G;
-                    const uint16_t *src = a.q + (int64_t)(p.s.q0 + t0 + (r < valid ? t : 0)) * a.q_ld +
-                                          (int64_t)(p.h * G + (r < valid ? g : 0)) * HD + ch * 8;
-                    cp_async16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, r < valid ? 16 : 0);
-                }
-            }
-            cp_async_commit();
-            cp_async_wait_group<0>();
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full);
+            mbar_expect_tx(&q_full, subs * (HD / 64) * tok * G * 128);
+            for (int sub = 0; sub < subs; ++sub)
+                for (int col = 0; col < HD / 64; ++col)
+                    tma_load_4d(qs + sub * T::kQBytes + col * (kBlock * 128), &mq, &q_full, 0, h,
+                                row + sub * tok, col);
         }
+        __syncwarp();
     }
     } else {
         // ---------------------------------------------------------- softmax
@@ -749,12 +737,16 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
 template <int HD, bool F16>
 cudaError_t run_tiles(const PagedAttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
                       cudaStream_t st) {
+    const int G = a.n_heads / a.n_kv;
+    CUtensorMap mq;
+    if (!make_map_rows(&mq, F16, a.q, HD, a.n_heads, a.pb.n_tokens, a.q_ld, G, kBlock / G))
+        return cudaErrorInvalidValue;
     auto kern = paged_tiles_kernel<HD, F16>;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(kern, Tc<HD>::kSmem, allowed);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kern, dim3((unsigned)sm_count()), Tc<HD>::kThreads, Tc<HD>::kSmem, st, mk, mv,
-                      a);
+    return launch_pdl(kern, dim3((unsigned)sm_count()), Tc<HD>::kThreads, Tc<HD>::kSmem, st, mq, mk,
+                      mv, a);
 }
 
 }  // namespace

@@ -1016,6 +1016,21 @@ bool make_map_pages(CUtensorMap *m, bool f16, const void *base, int head_dim, in
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_map_rows(CUtensorMap *m, bool f16, const void *base, int head_dim, int n_heads,
+                   int n_tokens, int64_t ld, int box_heads, int box_tokens) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[4] = {64, (cuuint64_t)n_heads, (cuuint64_t)n_tokens, (cuuint64_t)head_dim / 64};
+    cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)ld * 2, 128};
+    cuuint32_t boxes[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+              const_cast<void *>(base), dims, strides, boxes, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool tensor_maps_available() { return encode_fn() != nullptr; }
 
 bool tc_gemm_supported(const TcGemmArgs &a) {

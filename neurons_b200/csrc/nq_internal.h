@@ -138,6 +138,12 @@ int tc_gemm_launches(const TcGemmArgs &a);
 bool make_map_pages(CUtensorMap *m, bool f16, const void *base, int head_dim, int page_size,
                     int n_kv, int n_pages, int64_t page_stride, int box, int cols);
 
+// Query rows [n_tokens][ld] of n_heads x head_dim as a tensor (64 dims, heads,
+// tokens, head_dim / 64) with 128-byte swizzle; a box is 64 dims of box_heads
+// heads of box_tokens tokens, token by token.
+bool make_map_rows(CUtensorMap *m, bool f16, const void *base, int head_dim, int n_heads,
+                   int n_tokens, int64_t ld, int box_heads, int box_tokens);
+
 // True when cuTensorMapEncodeTiled could be resolved from the driver.
 bool tensor_maps_available();
 

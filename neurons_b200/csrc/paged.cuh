@@ -411,6 +411,14 @@ cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, unsigned threads, size_t s
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+__device__ __forceinline__ void tma_load_4d(void *smem_dst, const void *tmap, uint64_t *bar,
+                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
 __device__ __forceinline__ void tma_load_5d(void *smem_dst, const void *tmap, uint64_t *bar,
                                             int32_t c0, int32_t c1, int32_t c2, int32_t c3,
                                             int32_t c4) {
