@@ -529,8 +529,9 @@ __global__ void __launch_bounds__(128) paged_merge_rows_kernel(const PagedAttnAr
 }
 
 // The same for paged_tiles_kernel's parts, [dim / 4][row][4] (its threads have a
-// row each), many rows in few parts: one thread takes 16 dims of a row, so that
-// a warp reads 512 bytes in one piece.
+// row each), many rows in few parts: one thread takes 8 dims of a row, so that
+// a warp reads 512 bytes in one piece, and goes through the parts once with a
+// running maximum, four parts' loads under way.
 template <int HD, bool F16>
 __global__ void __launch_bounds__(128) paged_merge_tiles_kernel(const PagedAttnArgs a, int rows) {
     pdl_launch_dependents();
@@ -538,46 +539,45 @@ __global__ void __launch_bounds__(128) paged_merge_tiles_kernel(const PagedAttnA
     const SplitNote note = a.notes[blockIdx.x];
     if (note.parts == 0) return;
     const int G = a.n_heads / a.n_kv;
-    const int r = blockIdx.z * 128 + threadIdx.x, d0 = blockIdx.y * 16;
+    const int r = blockIdx.z * 128 + threadIdx.x, d0 = blockIdx.y * 8;
     if (r >= note.tokens * G) return;
-    float M = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < note.parts; ++i) {
-        const float2 ml = *reinterpret_cast<const float2 *>(
-            a.part_ml + (part_slot(blockIdx.x, i) * rows + r) * 2);
-        if (ml.y != 0.f) M = fmaxf(M, ml.x);
-    }
-    float L = 0.f, acc[16];
+    float M = -INFINITY, L = 0.f, acc[8];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < note.parts; ++i) {
-        const int64_t at = part_slot(blockIdx.x, i) * rows;
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (at + r) * 2);
-        const float *po = a.part_o + at * HD + ((d0 >> 2) * rows + r) * 4;
-        float4 v[4];
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    constexpr int kAhead = 4;
+    for (int i0 = 0; i0 < note.parts; i0 += kAhead) {
+        float2 ml[kAhead];
+        float4 v[kAhead][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4 *>(po + j * rows * 4);
-        const float f = ml.y != 0.f ? ex2(ml.x - M) : 0.f;
-        L += ml.y * f;
+        for (int e = 0; e < kAhead; ++e) {
+            if (i0 + e >= note.parts) break;
+            const int64_t at = part_slot(blockIdx.x, i0 + e) * rows;
+            ml[e] = *reinterpret_cast<const float2 *>(a.part_ml + (at + r) * 2);
+            const float *po = a.part_o + at * HD + ((d0 >> 2) * rows + r) * 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc[4 * j] = fmaf(v[j].x, f, acc[4 * j]);
-            acc[4 * j + 1] = fmaf(v[j].y, f, acc[4 * j + 1]);
-            acc[4 * j + 2] = fmaf(v[j].z, f, acc[4 * j + 2]);
-            acc[4 * j + 3] = fmaf(v[j].w, f, acc[4 * j + 3]);
+            for (int j = 0; j < 2; ++j) v[e][j] = *reinterpret_cast<const float4 *>(po + j * rows * 4);
+        }
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            if (i0 + e >= note.parts || ml[e].y == 0.f) continue;
+            const float mn = fmaxf(M, ml[e].x);
+            const float f = M == -INFINITY ? 0.f : ex2(M - mn), g = ex2(ml[e].x - mn);
+            M = mn;
+            L = fmaf(L, f, ml[e].y * g);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                acc[4 * j] = fmaf(acc[4 * j], f, v[e][j].x * g);
+                acc[4 * j + 1] = fmaf(acc[4 * j + 1], f, v[e][j].y * g);
+                acc[4 * j + 2] = fmaf(acc[4 * j + 2], f, v[e][j].z * g);
+                acc[4 * j + 3] = fmaf(acc[4 * j + 3], f, v[e][j].w * g);
+            }
         }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    uint16_t *op = a.out + (int64_t)(note.q_row + r / G) * a.out_ld +
-                   (int64_t)(note.heads0 + r % G) * HD + d0;
-#pragma unroll
-    for (int j = 0; j < 16; j += 8)
-        *reinterpret_cast<uint4 *>(op + j) =
-            make_uint4(pack_t2<F16>(acc[j] * inv, acc[j + 1] * inv),
-                       pack_t2<F16>(acc[j + 2] * inv, acc[j + 3] * inv),
-                       pack_t2<F16>(acc[j + 4] * inv, acc[j + 5] * inv),
-                       pack_t2<F16>(acc[j + 6] * inv, acc[j + 7] * inv));
+    *reinterpret_cast<uint4 *>(a.out + (int64_t)(note.q_row + r / G) * a.out_ld +
+                               (int64_t)(note.heads0 + r % G) * HD + d0) =
+        make_uint4(pack_t2<F16>(acc[0] * inv, acc[1] * inv), pack_t2<F16>(acc[2] * inv, acc[3] * inv),
+                   pack_t2<F16>(acc[4] * inv, acc[5] * inv), pack_t2<F16>(acc[6] * inv, acc[7] * inv));
 }
 
 // CTAs of paged_rows_kernel: as many as fit at once
@@ -624,7 +624,7 @@ cudaError_t run_attention(const PagedAttnArgs &a, const CUtensorMap &mk, const C
     if (e != cudaSuccess || s.whole) return e;
     if (s.tiles)
         return launch_pdl(paged_merge_tiles_kernel<HD, F16>,
-                          dim3((unsigned)s.grid, HD / 16, (unsigned)s.rows / 128), 128, 0, st, a,
+                          dim3((unsigned)s.grid, HD / 8, (unsigned)s.rows / 128), 128, 0, st, a,
                           s.rows);
     // (a caller's max_q may be too small: every row of a tile has its CTA)
     return launch_pdl(paged_merge_rows_kernel<HD, F16>, dim3((unsigned)s.grid, rows <= 8 ? 8u : 16u),
