@@ -317,8 +317,8 @@ int nq_llama_reset(nq_llama_t dec, void *stream);
  * the step's logits and argmax. */
 int nq_llama_step(nq_llama_t dec, const int32_t *token, float *logits,
                   int32_t *next_token, void *stream);
-/* n steps over the prompt tokens[0..n) (device); logits (optional) gets the
- * last position's.  Afterwards the decoder's next input is the argmax of the
+/* n steps over the prompt tokens[0..n) (device), or steps of a chunk each
+ * after nq_llama_set_prefill_chunk; logits (optional) gets the last position's.  Afterwards the decoder's next input is the argmax of the
  * last position (the first generated token). */
 int nq_llama_prefill(nq_llama_t dec, const int32_t *tokens, int64_t n,
                      float *logits, void *stream);
@@ -448,6 +448,30 @@ int nq_pages_compact(const nq_page_table_t *table, const nq_page_pool_t *pool, v
  * refused (that move alone). */
 int nq_pages_copy(const nq_page_pool_t *pool, const int32_t *src, const int32_t *dst, int64_t n,
                   void *stream);
+
+/* ---- Llama over a paged cache ----
+ * Prompts in chunks: nq_llama_prefill passes up to `chunk` tokens through the
+ * layers at a time (M-row quantized matmuls, nq_paged_attention over the
+ * decoder's cache) instead of one (0, the default).  The results differ from the
+ * one-token steps' by the order of the sums.  Allocates the chunk's workspace;
+ * not to be called while calls on the decoder are under way. */
+int nq_llama_set_prefill_chunk(nq_llama_t dec, int64_t chunk);
+
+/* The batch's new tokens (tokens: device int32 [batch->n_tokens]) through the
+ * decoder's layers over a paged cache of the caller's (bf16; `cache` describes
+ * layer 0, layer l's keys and values lie l * layer_stride elements on); the
+ * decoder's own cache and position are not touched.  Row rows[i] of the batch
+ * (device int32 [n_out]; negative: left out, its outputs are not meaningful)
+ * yields logits [n_out][vocab] (fp32, optional) and next_tokens [n_out] (int32
+ * argmax, optional).  max_q as in nq_paged_attention.  The pages for the new
+ * tokens are the caller's to reserve.  workspace: nq_llama_forward_workspace_
+ * size() bytes (max_keys = table_width * page_size), 256-byte aligned. */
+size_t nq_llama_forward_workspace_size(nq_llama_t dec, int64_t n_tokens, int64_t n_out, int64_t max_q,
+                                       int64_t max_keys);
+int nq_llama_forward(nq_llama_t dec, const int32_t *tokens, const nq_paged_cache_t *cache,
+                     int64_t layer_stride, const nq_paged_batch_t *batch, int64_t max_q,
+                     const int32_t *rows, int64_t n_out, float *logits, int32_t *next_tokens,
+                     void *workspace, size_t workspace_bytes, void *stream);
 
 /* nq_moe_switch without a workspace argument, for callers that cannot
  * allocate device memory themselves (an FFI host or a runtime that only

@@ -47,6 +47,9 @@ SIGNATURES = {
                                   P, P, I, I, P, U64, P, P]),
     "nq_moe_switch_partial_push": (I, [P, I64, I64, I64, I64, I64, P, P, I64, I64, P, P, P, P, P, P,
                                        P, P, P, I, I, P, U64, P, P]),
+    "nq_llama_set_prefill_chunk": (I, [P, I64]),
+    "nq_llama_forward_workspace_size": (U64, [P, I64, I64, I64, I64]),
+    "nq_llama_forward": (I, [P, P, P, I64, P, I64, P, I64, P, P, P, U64, P]),
     "nq_paged_attention_workspace_size": (U64, [I, I, I, I64, I64]),
     "nq_paged_attention": (I, [P, I64, I, P, P, I64, F32, I64, P, U64, P, I64, P]),
     "nq_paged_append": (I, [P, I64, P, I64, P, I64, I, P, P, P, I, P, I64, P]),

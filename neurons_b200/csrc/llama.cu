@@ -21,6 +21,12 @@
 // in the GEMVs' stores (launch_rows_fused).  Five launches per
 // layer: qkv, attention, o, gate/up, down; then the final norm, the LM head
 // and the argmax.
+//
+// llama_forward runs the same layers for the new tokens of a batch of sequences
+// over a paged cache (nq_paged_append, nq_paged_attention), with the M-row
+// quantized matmuls and one elementwise kernel between them; a prompt's chunks
+// (set_prefill_chunk) are that call on the decoder's own cache, which is a
+// paged cache of one page.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -110,13 +116,13 @@ __device__ __forceinline__ float rope_elem(const uint16_t *head, int e, int hd, 
 
 struct AttnArgs {
     const uint16_t *qkv;        // [n_heads + 2 n_kv][hd] bf16: q heads, k heads, v heads
-    uint16_t *kc, *vc;          // this layer's caches [n_kv][max_ctx][hd]
+    uint16_t *kc, *vc;          // this layer's caches [n_kv][ctx_ld][hd]
     float *pm, *pl, *pacc;      // partials [n_heads][splits] (+ [hd] for pacc)
     int32_t *counter;           // [n_heads], zero between steps
     uint16_t *out;              // [n_heads][hd]
     const int32_t *pos;         // this step's position
     unsigned *err;
-    int n_heads, n_kv, hd, max_ctx, splits;
+    int n_heads, n_kv, hd, max_ctx, ctx_ld, splits;  // ctx_ld: positions a cache has room for
     float log2_base, scale;
 };
 
@@ -186,8 +192,8 @@ __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
         qs[d] = rope_elem(qraw, d, HD, fpos, a.log2_base);
         if (has_new) kn[d] = rope_elem(kraw, d, HD, fpos, a.log2_base);
     }
-    uint16_t *kc = a.kc + (size_t)j * a.max_ctx * HD;
-    uint16_t *vc = a.vc + (size_t)j * a.max_ctx * HD;
+    uint16_t *kc = a.kc + (size_t)j * a.ctx_ld * HD;
+    uint16_t *vc = a.vc + (size_t)j * a.ctx_ld * HD;
     __syncthreads();
     if (has_new && hq % group == 0) {
         for (int d = tid; d < HD; d += kAttnThreads) {
@@ -434,13 +440,19 @@ struct LlamaDecoder {
     nq_qweight_t embed{}, head{};
     const uint16_t *embed_dense = nullptr;
     // device state
-    uint16_t *kc = nullptr, *vc = nullptr;  // [layers][n_kv][max_ctx][hd]
+    int ctx_ld = 0;                         // max_context rounded up to a page's 16 keys
+    uint16_t *kc = nullptr, *vc = nullptr;  // [layers][n_kv][ctx_ld][hd]
     uint16_t *h = nullptr, *qkv = nullptr, *attn = nullptr, *gu = nullptr, *logits = nullptr;
     uint16_t *xn = nullptr;  // the final norm's output (LM head input)
     float *pm = nullptr, *pl = nullptr, *pacc = nullptr;
     int32_t *counter = nullptr, *pos = nullptr, *tok = nullptr;
     float *part_v = nullptr;  // argmax partials [kArgmaxBlocks]
     int32_t *part_i = nullptr, *amax_counter = nullptr;
+    float *freqs = nullptr;      // [hd / 2] radians per position
+    int32_t *one_seq = nullptr;  // page table {0}, length, {0, tokens}, last row of a chunk
+    int64_t chunk = 0;           // tokens per step of a prompt (0: one, by the decode step)
+    void *chunk_ws = nullptr;
+    size_t chunk_ws_bytes = 0;
     int splits = 1;
     int64_t host_pos = 0;  // steps enqueued since the last reset
     std::vector<void *> owned;
@@ -572,10 +584,11 @@ cudaError_t llama_step(LlamaDecoder &d, const int32_t *tok_src, float *logits_f3
     aa.n_kv = c.n_kv_heads;
     aa.hd = c.head_dim;
     aa.max_ctx = c.max_context;
+    aa.ctx_ld = d.ctx_ld;
     aa.splits = d.splits;
     aa.log2_base = log2f(c.rope_theta);
     aa.scale = 1.0f / sqrtf((float)c.head_dim);
-    const size_t layer_cache = (size_t)c.n_kv_heads * c.max_context * hd;
+    const size_t layer_cache = (size_t)c.n_kv_heads * d.ctx_ld * hd;
     for (int l = 0; l < c.n_layers; ++l) {
         const auto &L = d.layers[l];
         if ((e = gemv(d, d.h, H, L.qkv_w, L.qkv_s, L.qkv_b, nq_ + 2 * nkv, H, d.qkv, 1, L.in_norm,
@@ -679,7 +692,8 @@ cudaError_t llama_create(LlamaDecoder &d, const nq_llama_config_t &c,
         L.d_b = s.down.biases;
     }
     d.splits = (c.max_context + kAttnChunk - 1) / kAttnChunk;
-    const size_t cache = (size_t)c.n_layers * c.n_kv_heads * c.max_context * hd;
+    d.ctx_ld = (c.max_context + 15) / 16 * 16;
+    const size_t cache = (size_t)c.n_layers * c.n_kv_heads * d.ctx_ld * hd;
     if ((e = d.alloc(&d.kc, cache)) || (e = d.alloc(&d.vc, cache)) || (e = d.alloc(&d.h, H)) ||
         (e = d.alloc(&d.xn, H)) ||
         (e = d.alloc(&d.qkv, nq_ + 2 * nkv)) || (e = d.alloc(&d.attn, nq_)) ||
@@ -689,13 +703,320 @@ cudaError_t llama_create(LlamaDecoder &d, const nq_llama_config_t &c,
         (e = d.alloc(&d.pacc, (size_t)c.n_heads * d.splits * hd)) ||
         (e = d.alloc(&d.counter, (size_t)c.n_heads)) || (e = d.alloc(&d.pos, 1)) ||
         (e = d.alloc(&d.tok, 1)) || (e = d.alloc(&d.part_v, kArgmaxBlocks)) ||
-        (e = d.alloc(&d.part_i, kArgmaxBlocks)) || (e = d.alloc(&d.amax_counter, 1)))
+        (e = d.alloc(&d.part_i, kArgmaxBlocks)) || (e = d.alloc(&d.amax_counter, 1)) ||
+        (e = d.alloc(&d.freqs, hd / 2)) || (e = d.alloc(&d.one_seq, 8)))
+        return e;
+    std::vector<float> freqs(hd / 2);
+    for (size_t i = 0; i < freqs.size(); ++i)
+        freqs[i] = (float)std::pow((double)c.rope_theta, -2.0 * (double)i / (double)hd);
+    if ((e = cudaMemcpy(d.freqs, freqs.data(), freqs.size() * sizeof(float),
+                        cudaMemcpyHostToDevice)) ||
+        (e = cudaMemset(d.one_seq, 0, 8 * sizeof(int32_t))))
         return e;
     if ((e = cudaMemset(d.amax_counter, 0, sizeof(int32_t)))) return e;
     if ((e = cudaMemset(d.counter, 0, sizeof(int32_t) * c.n_heads)) ||
         (e = cudaMemset(d.pos, 0, sizeof(int32_t))) || (e = cudaMemset(d.tok, 0, sizeof(int32_t))))
         return e;
     return cudaDeviceSynchronize();
+}
+
+namespace {
+
+// ------------------------------------------------- a batch's new tokens
+// h[t] = row tokens[t] of the embedding, as embed_kernel
+__global__ void __launch_bounds__(256) embed_rows_kernel(const int32_t *tokens, const uint32_t *ew,
+                                                         const uint16_t *es, const uint16_t *eb,
+                                                         const uint16_t *dense, int64_t hidden,
+                                                         int bits, int gs, int64_t vocab,
+                                                         uint16_t *h, unsigned *err) {
+    pdl_launch_dependents();
+    pdl_wait();
+    int64_t t = tokens[blockIdx.x];
+    if (t < 0 || t >= vocab) {
+        if (threadIdx.x == 0) atomicOr(err, kErrBadIndex);
+        t = 0;
+    }
+    uint16_t *dst = h + (int64_t)blockIdx.x * hidden;
+    const int per = 32 / bits;
+    for (int64_t k = threadIdx.x; k < hidden; k += blockDim.x) {
+        if (dense) {
+            dst[k] = dense[t * hidden + k];
+            continue;
+        }
+        const uint32_t word = ew[t * (hidden / per) + k / per];
+        const uint32_t q = (word >> (bits * (k % per))) & ((1u << bits) - 1u);
+        const int64_t g = t * (hidden / gs) + k / gs;
+        dst[k] = dq_value(q, es[g], eb[g]);
+    }
+}
+
+// One CTA per row r (of h: rows[r] when rows != nullptr, a negative one left
+// out): h += y (rounded, when y != nullptr; with rows, whose entries may repeat,
+// the sum is not kept), x = rms_norm(h) with rmsnorm_kernel's roundings.
+// hidden % 8 == 0.
+__global__ void __launch_bounds__(256) add_norm_rows_kernel(uint16_t *h, const uint16_t *y,
+                                                            const int32_t *rows, int64_t n_h,
+                                                            const uint16_t *w, int64_t hidden,
+                                                            float eps, uint16_t *x, unsigned *err) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float part[8];
+    int64_t r = blockIdx.x;
+    if (rows) {
+        r = rows[r];
+        if (r < 0) return;
+        if (r >= n_h) {
+            if (threadIdx.x == 0) atomicOr(err, kErrBadIndex);
+            return;
+        }
+    }
+    uint4 *hr = reinterpret_cast<uint4 *>(h + r * hidden);
+    const uint4 *yr = reinterpret_cast<const uint4 *>(y + r * hidden);
+    const int n = (int)(hidden / 8);
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const uint4 hv = hr[i];
+        uint32_t a[4] = {hv.x, hv.y, hv.z, hv.w};
+        if (y) {
+            const uint4 yv = yr[i];
+            const uint32_t b[4] = {yv.x, yv.y, yv.z, yv.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = bf2_add(a[j], b[j]);
+            if (!rows) hr[i] = make_uint4(a[0], a[1], a[2], a[3]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float u = bf16_to_f32((uint16_t)a[j]), v = bf16_to_f32((uint16_t)(a[j] >> 16));
+            ss = fmaf(u, u, fmaf(v, v, ss));
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
+    __syncthreads();
+    float tot = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) tot += part[i];
+    const float inv = 1.0f / sqrtf(tot / (float)hidden + eps);
+    uint4 *xr = reinterpret_cast<uint4 *>(x + (int64_t)blockIdx.x * hidden);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const uint4 hv = hr[i];  // (this thread's own values)
+        const uint4 wv = reinterpret_cast<const uint4 *>(w)[i];
+        uint32_t a[4] = {hv.x, hv.y, hv.z, hv.w};
+        if (y && rows) {
+            const uint4 yv = yr[i];
+            const uint32_t b[4] = {yv.x, yv.y, yv.z, yv.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = bf2_add(a[j], b[j]);
+        }
+        const uint32_t b[4] = {wv.x, wv.y, wv.z, wv.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float u = bf16_to_f32(f32_to_bf16(bf16_to_f32((uint16_t)a[j]) * inv));
+            const float v = bf16_to_f32(f32_to_bf16(bf16_to_f32((uint16_t)(a[j] >> 16)) * inv));
+            o[j] = pack_bf2(bf16_to_f32((uint16_t)b[j]) * u, bf16_to_f32((uint16_t)(b[j] >> 16)) * v);
+        }
+        xr[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+__device__ __forceinline__ float swiglu_bf16(float g, float u) {
+    const float s = bf16_to_f32(f32_to_bf16(1.f / (1.f + expf(-g))));
+    return bf16_to_f32(f32_to_bf16(s * g)) * u;
+}
+
+// act[i] = bf16(bf16(bf16(sigmoid(g)) g) u) for gu in groups of 8 gate values and
+// the 8 matching up values (the interleaved weights' order)
+__global__ void __launch_bounds__(256) swiglu_rows_kernel(const uint4 *gu, int64_t n, uint4 *act) {
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const uint4 g = gu[2 * i], u = gu[2 * i + 1];
+        const uint32_t a[4] = {g.x, g.y, g.z, g.w}, b[4] = {u.x, u.y, u.z, u.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            o[j] = pack_bf2(
+                swiglu_bf16(bf16_to_f32((uint16_t)a[j]), bf16_to_f32((uint16_t)b[j])),
+                swiglu_bf16(bf16_to_f32((uint16_t)(a[j] >> 16)), bf16_to_f32((uint16_t)(b[j] >> 16))));
+        act[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// One CTA per row: the argmax of its logits (first index of the maximum; token 0
+// without a finite one) and their fp32 copy.
+__global__ void __launch_bounds__(1024) argmax_rows_kernel(const uint16_t *logits, int64_t vocab,
+                                                           float *logits_f32, int32_t *next) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float wv[32];
+    __shared__ int64_t wi[32];
+    const uint16_t *row = logits + (int64_t)blockIdx.x * vocab;
+    float best = -INFINITY;
+    int64_t besti = vocab;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < vocab; i += blockDim.x) {
+        const float v = bf16_to_f32(row[i]);
+        if (logits_f32) logits_f32[(int64_t)blockIdx.x * vocab + i] = v;
+        if (v > best) {
+            best = v;
+            besti = i;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        better(best, besti, __shfl_xor_sync(0xffffffffu, best, o),
+               __shfl_xor_sync(0xffffffffu, besti, o));
+    if ((threadIdx.x & 31) == 0) {
+        wv[threadIdx.x >> 5] = best;
+        wi[threadIdx.x >> 5] = besti;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && next) {
+        for (int w = 1; w < 32; ++w) better(best, besti, wv[w], wi[w]);
+        next[blockIdx.x] = besti < vocab ? (int32_t)besti : 0;
+    }
+}
+
+// a chunk of the decoder's own sequence: {page 0}, length with the chunk's T
+// tokens, {0, T}, last row; then the position behind it
+__global__ void chunk_begin_kernel(int32_t *one, const int32_t *pos, int T) {
+    pdl_launch_dependents();
+    pdl_wait();
+    one[0] = 0;
+    one[1] = *pos + T;
+    one[2] = 0;
+    one[3] = T;
+    one[4] = T - 1;
+}
+__global__ void chunk_end_kernel(int32_t *pos, int T) {
+    pdl_launch_dependents();
+    pdl_wait();
+    *pos += T;
+}
+
+// the forward call's workspace
+struct ForwardSpace {
+    uint16_t *h, *x, *y, *qkv, *attn, *gu, *act, *logits;
+    void *attn_ws;
+    size_t attn_ws_bytes, total;
+};
+
+ForwardSpace forward_space(const LlamaDecoder &d, int64_t T, int64_t n_out, int64_t max_q,
+                           int64_t max_keys, void *ws) {
+    const auto &c = d.c;
+    const int64_t H = c.hidden, nq_ = (int64_t)c.n_heads * c.head_dim,
+                  nkv = (int64_t)c.n_kv_heads * c.head_dim, I = c.intermediate;
+    ForwardSpace f{};
+    uint8_t *p = static_cast<uint8_t *>(ws);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *q = p ? p + at : nullptr;
+        at += (bytes + 255) / 256 * 256;
+        return q;
+    };
+    auto rows = [&](int64_t n, int64_t width) {
+        return reinterpret_cast<uint16_t *>(take((size_t)n * width * 2));
+    };
+    f.h = rows(T, H);
+    f.x = rows(std::max(T, n_out), H);
+    f.y = rows(T, H);
+    f.qkv = rows(T, nq_ + 2 * nkv);
+    f.attn = rows(T, nq_);
+    f.gu = rows(T, 2 * I);
+    f.act = rows(T, I);
+    f.logits = rows(n_out, c.vocab);
+    f.attn_ws_bytes = nq_paged_attention_workspace_size(c.n_heads, c.n_kv_heads, c.head_dim, max_q,
+                                                        max_keys);
+    f.attn_ws = take(f.attn_ws_bytes);
+    f.total = at;
+    return f;
+}
+
+int fwd_cuda(cudaError_t e) {
+    if (e == cudaSuccess) return NQ_SUCCESS;
+    cudaGetLastError();
+    set_error(std::string("nq_llama_forward: ") + cudaGetErrorString(e));
+    return NQ_COMPUTE_ERROR;
+}
+
+}  // namespace
+
+// The batch's tokens through all layers, then the logits of `n_out` of their rows
+// (rows: device, negative ones left out).
+int llama_forward(LlamaDecoder &d, const int32_t *tokens, const nq_paged_cache_t &cache,
+                  int64_t layer_stride, const nq_paged_batch_t &batch, int64_t max_q,
+                  const int32_t *rows, int64_t n_out, float *logits, int32_t *next,
+                  const ForwardSpace &f, cudaStream_t st) {
+    const auto &c = d.c;
+    const int64_t T = batch.n_tokens, H = c.hidden, hd = c.head_dim,
+                  nq_ = (int64_t)c.n_heads * hd, nkv = (int64_t)c.n_kv_heads * hd, I = c.intermediate,
+                  Nqkv = nq_ + 2 * nkv;
+    unsigned *err = device_error_word();
+    const float scale = 1.0f / sqrtf((float)c.head_dim);
+    int rc;
+    auto norm = [&](const uint16_t *y, const int32_t *which, int64_t n, const uint16_t *w) {
+        return fwd_cuda(launch_pdl_ll(add_norm_rows_kernel, dim3((unsigned)n), 256, 0, st, f.h, y,
+                                      which, T, w, H, c.rms_eps, f.x, err));
+    };
+    auto mm = [&](const uint16_t *x, int64_t M, const uint32_t *w, const uint16_t *s,
+                  const uint16_t *b, int64_t N, int64_t K, uint16_t *y) {
+        return nq_quantized_matmul(x, M, w, s, b, N, K, c.bits, c.group_size, y, st);
+    };
+    if ((rc = fwd_cuda(launch_pdl_ll(embed_rows_kernel, dim3((unsigned)T), 256, 0, st, tokens,
+                                     d.embed.w, d.embed.scales, d.embed.biases, d.embed_dense, H,
+                                     c.bits, c.group_size, (int64_t)c.vocab, f.h, err))))
+        return rc;
+    for (int l = 0; l < c.n_layers; ++l) {
+        const auto &L = d.layers[l];
+        nq_paged_cache_t lc = cache;
+        lc.k = static_cast<uint16_t *>(cache.k) + l * layer_stride;
+        lc.v = static_cast<uint16_t *>(cache.v) + l * layer_stride;
+        if ((rc = norm(l ? f.y : nullptr, nullptr, T, L.in_norm)) ||
+            (rc = mm(f.x, T, L.qkv_w, L.qkv_s, L.qkv_b, Nqkv, H, f.qkv)) ||
+            (rc = nq_paged_append(f.qkv, Nqkv, f.qkv + nq_, Nqkv, f.qkv + nq_ + nkv, Nqkv, c.n_heads,
+                                  &lc, &batch, d.freqs, (int)(hd / 2), f.qkv, Nqkv, st)) ||
+            (rc = nq_paged_attention(f.qkv, Nqkv, c.n_heads, &lc, &batch, max_q, scale, 0, f.attn_ws,
+                                     f.attn_ws_bytes, f.attn, nq_, st)) ||
+            (rc = mm(f.attn, T, L.o_w, L.o_s, L.o_b, H, nq_, f.y)) ||
+            (rc = norm(f.y, nullptr, T, L.post_norm)) ||
+            (rc = mm(f.x, T, L.gu_w, L.gu_s, L.gu_b, 2 * I, H, f.gu)))
+            return rc;
+        const int64_t n = T * I / 8;
+        if ((rc = fwd_cuda(launch_pdl_ll(
+                 swiglu_rows_kernel,
+                 dim3((unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)sm_count() * 8)), 256, 0,
+                 st, reinterpret_cast<const uint4 *>(f.gu), n, reinterpret_cast<uint4 *>(f.act)))) ||
+            (rc = mm(f.act, T, L.d_w, L.d_s, L.d_b, H, I, f.y)))
+            return rc;
+    }
+    if (n_out == 0) return NQ_SUCCESS;
+    if ((rc = norm(f.y, rows, n_out, d.final_norm)) ||
+        (rc = mm(f.x, n_out, d.head.w, d.head.scales, d.head.biases, c.vocab, H, f.logits)))
+        return rc;
+    return fwd_cuda(launch_pdl_ll(argmax_rows_kernel, dim3((unsigned)n_out), 1024, 0, st,
+                                  (const uint16_t *)f.logits, (int64_t)c.vocab, logits, next));
+}
+
+// One chunk of T tokens of the decoder's own sequence, which is entry 0 of a
+// table of one page per layer.
+int llama_chunk(LlamaDecoder &d, const int32_t *tokens, int64_t T, bool last, float *logits,
+                cudaStream_t st) {
+    const auto &c = d.c;
+    const int64_t page = (int64_t)c.n_kv_heads * d.ctx_ld * c.head_dim;
+    const nq_paged_cache_t cache{d.kc, d.vc, 1, page, c.n_kv_heads, d.ctx_ld, c.head_dim,
+                                 NQ_DTYPE_BF16};
+    const nq_paged_batch_t batch{d.one_seq, 1, 1, 1, d.one_seq + 1, nullptr, d.one_seq + 2, 1, T};
+    const ForwardSpace f = forward_space(d, T, 1, T, d.ctx_ld, d.chunk_ws);
+    int rc;
+    if ((rc = fwd_cuda(launch_pdl_ll(chunk_begin_kernel, dim3(1), 1, 0, st, d.one_seq,
+                                     (const int32_t *)d.pos, (int)T))) ||
+        (rc = llama_forward(d, tokens, cache, page, batch, T, d.one_seq + 4, last ? 1 : 0, logits,
+                            d.tok, f, st)))
+        return rc;
+    return fwd_cuda(launch_pdl_ll(chunk_end_kernel, dim3(1), 1, 0, st, d.pos, (int)T));
 }
 
 }  // namespace nq
@@ -811,6 +1132,16 @@ int nq_llama_prefill(nq_llama_t dec, const int32_t *tokens, int64_t n, float *lo
     auto &d = dec->d;
     if (d.host_pos + n > d.c.max_context)
         return llama_fail(NQ_INVALID_INPUT, std::string(what) + ": context full");
+    if (d.chunk > 0) {
+        for (int64_t i = 0; i < n; i += d.chunk) {
+            const int64_t T = std::min(d.chunk, n - i);
+            if (int rc = nq::llama_chunk(d, tokens + i, T, i + T == n, logits,
+                                         static_cast<cudaStream_t>(stream)))
+                return rc;
+            d.host_pos += T;
+        }
+        return NQ_SUCCESS;
+    }
     for (int64_t i = 0; i < n; ++i) {
         if (int rc = llama_cuda(nq::llama_step(d, tokens + i, i + 1 == n ? logits : nullptr,
                                                nullptr, static_cast<cudaStream_t>(stream)),
@@ -819,6 +1150,64 @@ int nq_llama_prefill(nq_llama_t dec, const int32_t *tokens, int64_t n, float *lo
         ++d.host_pos;
     }
     return NQ_SUCCESS;
+}
+
+int nq_llama_set_prefill_chunk(nq_llama_t dec, int64_t chunk) {
+    const char *what = "nq_llama_set_prefill_chunk";
+    if (!dec || chunk < 0)
+        return llama_fail(NQ_INVALID_INPUT, std::string(what) + ": need a decoder and chunk >= 0");
+    auto &d = dec->d;
+    chunk = std::min<int64_t>(chunk, d.c.max_context);
+    if (chunk > 0) {
+        // (a shorter chunk may take the attention kernel with the larger workspace)
+        size_t need = 0;
+        for (int64_t T : {chunk, (int64_t)1, std::min<int64_t>(chunk, 16)})
+            need = std::max(need, nq::forward_space(d, chunk, 1, T, d.ctx_ld, nullptr).total);
+        if (need > d.chunk_ws_bytes) {
+            void *p = nullptr;
+            if (int rc = llama_cuda(cudaMalloc(&p, need), what)) return rc;
+            d.owned.push_back(p);  // (an older, smaller one may still be in use)
+            d.chunk_ws = p;
+            d.chunk_ws_bytes = need;
+        }
+    }
+    d.chunk = chunk;
+    return NQ_SUCCESS;
+}
+
+size_t nq_llama_forward_workspace_size(nq_llama_t dec, int64_t n_tokens, int64_t n_out, int64_t max_q,
+                                       int64_t max_keys) {
+    if (!dec || n_tokens < 0 || n_out < 0 || max_q < 0 || max_keys < 0) return 0;
+    return nq::forward_space(dec->d, n_tokens, n_out, max_q, max_keys, nullptr).total;
+}
+
+int nq_llama_forward(nq_llama_t dec, const int32_t *tokens, const nq_paged_cache_t *cache,
+                     int64_t layer_stride, const nq_paged_batch_t *batch, int64_t max_q,
+                     const int32_t *rows, int64_t n_out, float *logits, int32_t *next_tokens,
+                     void *workspace, size_t workspace_bytes, void *stream) {
+    const std::string what = "nq_llama_forward";
+    if (!dec || !cache || !batch)
+        return llama_fail(NQ_INVALID_INPUT, what + ": NULL decoder, cache or batch");
+    auto &d = dec->d;
+    if (cache->dtype != NQ_DTYPE_BF16 || cache->head_dim != d.c.head_dim ||
+        cache->n_kv_heads != d.c.n_kv_heads)
+        return llama_fail(NQ_INVALID_INPUT,
+                          what + ": the cache must be bf16, with the decoder's heads");
+    if (layer_stride < 0 || layer_stride % 8 || max_q < 0 || n_out < 0 || batch->n_tokens < 0 ||
+        batch->n_tokens >= 0x7fffffff || n_out >= 0x7fffffff)
+        return llama_fail(NQ_INVALID_INPUT, what + ": a size is negative or too large");
+    if (batch->n_tokens == 0 || batch->n_seqs == 0) return NQ_SUCCESS;
+    if (!tokens || (n_out > 0 && (!rows || (!logits && !next_tokens))))
+        return llama_fail(NQ_INVALID_INPUT, what + ": NULL tokens, rows or outputs");
+    const int64_t most = !batch->q_starts ? 1 : (max_q == 0 ? batch->n_tokens : max_q);
+    const nq::ForwardSpace f = nq::forward_space(d, batch->n_tokens, n_out, most,
+                                                 batch->table_width * cache->page_size, workspace);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < f.total)
+        return llama_fail(NQ_INVALID_INPUT,
+                          what + ": workspace must be 256-byte aligned and hold "
+                                 "nq_llama_forward_workspace_size() bytes");
+    return nq::llama_forward(d, tokens, *cache, layer_stride, *batch, most, rows, n_out, logits,
+                             next_tokens, f, static_cast<cudaStream_t>(stream));
 }
 
 int nq_llama_generate(nq_llama_t dec, const int32_t *token, int64_t n, int32_t *tokens,

@@ -6,14 +6,22 @@ generation (:713-812) as back-to-back steps that feed each other's token on
 the device.
 
     dec = LlamaDecoder(cfg, weights)      # weights: torch CUDA tensors
+    dec.set_prefill_chunk(512)            # the prompt in chunks (default: by the step)
     dec.prefill(prompt_ids)               # int32 CUDA tensor
     ids = dec.generate(64)                # int32 CUDA tensor of 64 tokens
+
+PagedLlama serves many sequences with the same weights over one page pool:
+
+    srv = PagedLlama(dec, n_pages=4096, page_size=64, max_seqs=64, max_len=8192)
+    logits, tok = srv.step([0, 1], prompts, [len0, len1])   # chunks of any lengths
+    logits, tok = srv.step([0, 1], tok, [1, 1])             # one token each
+    srv.fork(0, [2, 3]); srv.free([1]); srv.compact()
 """
 import ctypes
 
 import torch
 
-from . import ops
+from . import ops, paged
 from ._lib import NQError, check, lib
 
 P = ctypes.c_void_p
@@ -87,6 +95,10 @@ class LlamaDecoder:
     def position(self):
         return int(lib().nq_llama_position(self.handle))
 
+    def set_prefill_chunk(self, chunk):
+        """Prompts in chunks of up to `chunk` tokens (0: one position per step)."""
+        check(lib().nq_llama_set_prefill_chunk(self.handle, int(chunk)))
+
     def reset(self):
         check(lib().nq_llama_reset(self.handle, ops._stream()))
 
@@ -102,7 +114,8 @@ class LlamaDecoder:
 
     def prefill(self, tokens, logits=True):
         """The prompt (int32 CUDA tensor) through the decoder, one position per
-        step; returns the last position's logits (fp32) or None."""
+        step or in chunks (set_prefill_chunk); returns the last position's logits
+        (fp32) or None."""
         if tokens.dtype != torch.int32 or not tokens.is_cuda:
             raise NQError(1, "prefill: tokens must be an int32 CUDA tensor")
         lg = torch.empty(self.vocab, dtype=torch.float32, device="cuda") if logits else None
@@ -118,3 +131,92 @@ class LlamaDecoder:
                                       P(token.data_ptr()) if token is not None else None, n,
                                       P(out.data_ptr()), ops._stream()))
         return out
+
+
+class PagedLlama:
+    """Continuous batching over a LlamaDecoder's weights: sequences 0 .. max_seqs - 1 of up
+    to max_len tokens in a pool of n_pages pages.  The page table, lengths and
+    reference counts live on the device; the host keeps the lengths beside them."""
+
+    def __init__(self, decoder, n_pages, page_size=64, max_seqs=64, max_len=4096):
+        c = decoder.cfg
+        if n_pages <= 0 or page_size <= 0 or page_size % 16 or max_seqs <= 0 or max_len <= 0:
+            raise NQError(1, "PagedLlama: sizes must be positive, page_size a multiple of 16")
+        self.decoder, self.max_len = decoder, max_len
+        self.pool = torch.empty((c["n_layers"], 2, n_pages, c["n_kv_heads"], page_size,
+                                 c["head_dim"]), dtype=torch.bfloat16, device="cuda")
+        width = -(-max_len // page_size)
+        self.refs = torch.zeros(n_pages, dtype=torch.int32, device="cuda")
+        self.table = torch.full((max_seqs, width), -1, dtype=torch.int32, device="cuda")
+        self.lens = torch.zeros(max_seqs, dtype=torch.int32, device="cuda")
+        self.host_lens = [0] * max_seqs
+
+    def _ids(self, x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+    def _check(self, seqs):
+        if any(s < 0 or s >= len(self.host_lens) for s in seqs) or len(set(seqs)) < len(seqs):
+            raise NQError(1, f"sequences must be different numbers below {len(self.host_lens)}")
+
+    def step(self, seqs, tokens, news, logits=True):
+        """news[i] new tokens of sequence seqs[i], one sequence after another in `tokens`
+        (int32 CUDA tensor).  Returns the last positions' logits (fp32 [n, vocab], or None)
+        and argmax (int32 [n]).  Too few free pages leave the sequences as they were and
+        raise bit 2 of take_device_error(); the step's outputs mean nothing then, and
+        lengths() tells the sequences' lengths."""
+        self._check(seqs)
+        n, total = len(seqs), sum(news)
+        if len(news) != n or n == 0 or min(news) < 1 or tokens.dtype != torch.int32 or \
+                not tokens.is_cuda or not tokens.is_contiguous() or tokens.numel() != total:
+            raise NQError(1, "step: tokens must be int32 CUDA, news[i] >= 1 of them for each sequence")
+        new_lens = [self.host_lens[s] + m for s, m in zip(seqs, news)]
+        if max(new_lens) > self.max_len:
+            raise NQError(1, f"step: a sequence would pass max_len {self.max_len}")
+        starts = [0]
+        for m in news:
+            starts.append(starts[-1] + m)
+        meta = self._ids(list(seqs) + new_lens + starts + [e - 1 for e in starts[1:]])
+        ids, lens, q_starts, rows = meta.split([n, n, n + 1, n])
+        paged.pages_reserve(self.pool, self.refs, self.table, self.lens, ids, lens)
+        cache = paged._cache(self.pool[0, 0], self.pool[0, 1])[0]
+        batch = paged._batch(self.table, self.lens, ids, q_starts, total, self.pool.get_device())
+        d = self.decoder
+        lg = torch.empty((n, d.vocab), dtype=torch.float32, device="cuda") if logits else None
+        nxt = torch.empty(n, dtype=torch.int32, device="cuda")
+        most = max(news)
+        f = lib()
+        need = f.nq_llama_forward_workspace_size(d.handle, total, n, most,
+                                                 self.table.shape[1] * self.pool.shape[-2])
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        check(f.nq_llama_forward(d.handle, tokens.data_ptr(), ctypes.byref(cache),
+                                 self.pool.stride(0), ctypes.byref(batch), most, rows.data_ptr(), n,
+                                 lg.data_ptr() if logits else None, nxt.data_ptr(), ws.data_ptr(),
+                                 need, ops._stream()))
+        for s, m in zip(seqs, new_lens):
+            self.host_lens[s] = m
+        return lg, nxt
+
+    def fork(self, parent, children):
+        """children (empty so far) continue from parent's tokens, sharing its pages."""
+        self._check([parent] + list(children))
+        if any(self.host_lens[c] for c in children):
+            raise NQError(1, "fork: a child has tokens")
+        paged.pages_fork(self.refs, self.table, self.lens, self._ids([parent] * len(children)),
+                         self._ids(list(children)))
+        for c in children:
+            self.host_lens[c] = self.host_lens[parent]
+
+    def free(self, seqs):
+        self._check(seqs)
+        paged.pages_free(self.refs, self.table, self.lens, self._ids(list(seqs)))
+        for s in seqs:
+            self.host_lens[s] = 0
+
+    def compact(self):
+        """The used pages move to the pool's low end."""
+        paged.pages_compact(self.pool, self.refs, self.table)
+
+    def lengths(self):
+        """The lengths as the device has them (waits for it); the host's copy follows."""
+        self.host_lens = self.lens.tolist()
+        return list(self.host_lens)

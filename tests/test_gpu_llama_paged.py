@@ -1,0 +1,176 @@
+"""GPU parity of the Llama paths over a paged cache: prompts in chunks against the
+oracle's decode function (oracle/llama_oracle.py), and PagedLlama's batched steps, forks,
+frees and compaction against one decoder per sequence.  Logits: normwise error <= 1e-2,
+as for the decode step (tests/test_gpu_llama.py): each step's inputs differ only through
+earlier bf16 rounding flips."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import neurons_b200 as nb
+from neurons_b200._lib import lib
+from neurons_b200.llama import LlamaDecoder, PagedLlama
+from test_gpu_llama import SMALL, check_logits, make_model
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def model(oracle):
+    return make_model(oracle, dict(SMALL, max_context=650), 21)
+
+
+def cfg():
+    return dict(SMALL, max_context=650)  # (not a multiple of a page's 16 keys)
+
+
+@pytest.mark.parametrize("chunk", [1, 7, 64, 300, 1000])
+def test_chunked_prompt_matches_the_oracle(oracle, nqlib, model, chunk):
+    from oracle.llama_oracle import LlamaOracle
+    host, dev = model
+    dec, ora = LlamaDecoder(cfg(), dev), LlamaOracle(cfg(), host)
+    toks = np.random.default_rng(5).integers(0, SMALL["vocab"], 150).astype(np.int32)
+    for t in toks:
+        ref, _ = ora.step(int(t))
+    dec.set_prefill_chunk(chunk)
+    lg = dec.prefill(torch.from_numpy(toks).cuda())
+    torch.cuda.synchronize()
+    check_logits(oracle, lg, ref, f"chunk {chunk}")
+    assert dec.position == 150
+    # the decode step goes on over the chunks' keys, from the prompt's own next token
+    token = int(lg.argmax())
+    for i in range(3):
+        lg, nxt = dec.step(None)
+        ref, _ = ora.step(token)
+        torch.cuda.synchronize()
+        check_logits(oracle, lg, ref, f"chunk {chunk}, step {i}")
+        token = int(nxt.item())
+    assert nb.take_device_error() == 0
+
+
+def test_a_second_prompt_continues_the_first(oracle, nqlib, model):
+    _, dev = model
+    toks = torch.randint(0, SMALL["vocab"], (200,), dtype=torch.int32, device="cuda")
+    one, two = LlamaDecoder(cfg(), dev), LlamaDecoder(cfg(), dev)
+    one.set_prefill_chunk(64)
+    two.set_prefill_chunk(64)
+    a = one.prefill(toks)
+    two.prefill(toks[:100], logits=False)
+    b = two.prefill(toks[100:])
+    assert (a - b).norm() <= 1e-2 * a.norm()
+    two.set_prefill_chunk(0)
+    two.reset()
+    c = two.prefill(toks)  # by the decode step, as before
+    assert (a - c).norm() <= 1e-2 * a.norm()
+
+
+def test_chunked_prompt_in_a_graph(nqlib, model):
+    _, dev = model
+    toks = torch.randint(0, SMALL["vocab"], (90,), dtype=torch.int32, device="cuda")
+    dec = LlamaDecoder(cfg(), dev)
+    dec.set_prefill_chunk(40)
+    want = dec.prefill(toks).clone()
+    dec.reset()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = dec.prefill(toks)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert nb.take_device_error() == 0
+
+
+def close(a, b, what):
+    err = ((a - b).norm() / b.norm()).item()
+    assert err < 1e-2, f"{what}: {err:.3e}"
+
+
+@pytest.mark.parametrize("page_size", [16, 128])
+def test_paged_serving_matches_single_sequences(nqlib, model, page_size):
+    """Prompts of several lengths in one step, a fork, single tokens, a chunk beside them, an
+    end, a compaction: every sequence's logits are those of a decoder of its own."""
+    _, dev = model
+    g = torch.Generator().manual_seed(3)
+    dec = LlamaDecoder(cfg(), dev)
+    srv = PagedLlama(dec, n_pages=2400 // page_size, page_size=page_size, max_seqs=6, max_len=500)
+    said = {}
+
+    def step(seqs, news):
+        toks = [torch.randint(0, SMALL["vocab"], (m,), dtype=torch.int32, generator=g) for m in news]
+        lg, nxt = srv.step(seqs, torch.cat(toks).cuda(), news)
+        for i, (s, t) in enumerate(zip(seqs, toks)):
+            said[s] = torch.cat([said.get(s, t[:0]), t])
+            own = LlamaDecoder(cfg(), dev)
+            own.set_prefill_chunk(600)
+            close(lg[i], own.prefill(said[s].cuda()), f"sequence {s} of {seqs}")
+            assert nxt[i].item() == lg[i].argmax().item()
+            own.close()
+        assert srv.lens.tolist() == srv.host_lens
+        assert nb.take_device_error() == 0
+
+    step([0, 1, 2], [100, 1, 33])
+    step([2, 0], [1, 1])
+    srv.fork(0, [3, 4])
+    said[3], said[4] = said[0], said[0]
+    step([0, 1, 2, 3, 4], [1, 1, 1, 1, 1])
+    step([4, 1, 3], [1, 130, 1])
+    srv.free([0, 2])
+    del said[0], said[2]
+    srv.compact()
+    step([1, 3, 4, 5], [1, 1, 1, 60])
+    assert srv.lengths() == [0, len(said[1]), 0, len(said[3]), len(said[4]), len(said[5])]
+    used = int((srv.refs > 0).sum())
+    assert int(srv.table.max()) < used + 20
+
+
+def test_serving_refusals(nqlib, model):
+    _, dev = model
+    dec = LlamaDecoder(cfg(), dev)
+    srv = PagedLlama(dec, n_pages=6, page_size=16, max_seqs=3, max_len=64)
+    t = lambda n: torch.zeros(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    for call in (lambda: srv.step([0, 0], t(2), [1, 1]), lambda: srv.step([3], t(1), [1]),
+                 lambda: srv.step([0], t(1), [2]), lambda: srv.step([0], t(1).long(), [1]),
+                 lambda: srv.step([0], t(65), [65]), lambda: srv.step([], t(0), []),
+                 lambda: srv.step([0], t(0), [0]), lambda: srv.fork(0, [3]),
+                 lambda: srv.free([1, 1]), lambda: PagedLlama(dec, 4, page_size=24),
+                 lambda: dec.set_prefill_chunk(-1)):
+        with pytest.raises(nb.NQError):
+            call()
+    srv.step([0, 1], t(80), [40, 40])  # six pages
+    with pytest.raises(nb.NQError):
+        srv.fork(0, [1])
+    assert nb.take_device_error() == 0
+    srv.step([2], t(16), [16])  # no page left: the device refuses
+    assert nb.take_device_error() & 4
+    assert srv.lengths() == [40, 40, 0]
+    srv.free([0])
+    srv.step([2], t(16), [16])
+    assert nb.take_device_error() == 0 and srv.lengths() == [0, 40, 16]
+
+
+def test_forward_refusals(nqlib, model):
+    _, dev = model
+    dec = LlamaDecoder(cfg(), dev)
+    from neurons_b200.paged import _Batch, _Cache
+    z = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda").data_ptr()
+    ok = dict(tokens=z, cache=_Cache(z, z, 2, 2 * 16 * 128, 2, 16, 128, 1), stride=1 << 14,
+              batch=_Batch(z, 1, 1, 1, z, None, None, 1, 1), max_q=1, rows=z, n_out=1, logits=z,
+              ws=z, ws_bytes=16)
+
+    def call(**kw):
+        d = {**ok, **kw}
+        return lib().nq_llama_forward(dec.handle, d["tokens"], ctypes.byref(d["cache"]), d["stride"],
+                                      ctypes.byref(d["batch"]), d["max_q"], d["rows"], d["n_out"],
+                                      d["logits"], None, d["ws"], d["ws_bytes"], None)
+
+    for kw in (dict(), dict(tokens=None), dict(ws=None), dict(rows=None), dict(logits=None),
+               dict(max_q=-1), dict(n_out=-1), dict(stride=4), dict(stride=-8),
+               dict(cache=_Cache(z, z, 2, 4096, 2, 16, 128, 2)),
+               dict(cache=_Cache(z, z, 2, 4096, 1, 16, 128, 1)),
+               dict(cache=_Cache(z, z, 2, 4096, 2, 16, 64, 1))):
+        assert call(**kw) == 1, kw
+    assert call(batch=_Batch(z, 1, 1, 1, z, None, None, 0, 0)) == 0

@@ -153,3 +153,12 @@ def test_page_lists_and_counts_are_checked(nqlib):
     assert nqlib.nq_pages_free(t_, None, 0, None) == 0
     assert nqlib.nq_pages_fork(t_, None, None, 0, None) == 0
     assert nqlib.nq_pages_copy(p_, None, None, 0, None) == 0
+
+
+def test_llama_paged_entry_points_refuse_null(nqlib):
+    c, b = cache(), batch()
+    assert nqlib.nq_llama_set_prefill_chunk(None, 16) == 1
+    assert nqlib.nq_llama_forward_workspace_size(None, 1, 1, 1, 16) == 0
+    assert nqlib.nq_llama_forward(None, A, ctypes.byref(c), 0, ctypes.byref(b), 1, A, 1, A, A, A,
+                                  1 << 30, None) == 1
+    assert nqlib.nq_last_error()
