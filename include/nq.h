@@ -374,7 +374,7 @@ typedef struct nq_paged_batch {
  * unknown).  Softmax and sums in fp32; the weights are rounded to the cache's type
  * for the second product, the result once.  workspace: nq_paged_attention_
  * workspace_size() bytes for this max_q and max_keys = table_width *
- * page_size (0 for short tables), 256-byte aligned, contents irrelevant; two
+ * page_size (0: none is needed), 256-byte aligned, contents irrelevant; two
  * calls that overlap on the GPU need one each. */
 size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q,
                                          int64_t max_keys);

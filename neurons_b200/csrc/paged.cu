@@ -46,49 +46,80 @@ __device__ __forceinline__ int entry_of(const PagedBatch &pb, int i) {
     return -1;
 }
 
+constexpr int kAppendThreads = 128;
+
 // (x_i, x_{i + half}) turned by pos * freqs[i], for the first 2 * half dims of
 // each head of q and k; the rest, and v, as they are.  k and v go to their
 // page.  One CTA per token: its angles are computed once for all heads, in
 // 64 bits (pos * freq of a 24-bit position and a 32-bit frequency is exact
 // there; in 32 bits the angle of position 100000 would be off by up to 0.004)
 // and reduced to a part of a turn before sine and cosine are taken in 32.
+// Memory bounds it: the first three vector pairs and one value vector of a thread
+// (all there are for 40 turned heads of 128 dims) are under way before the token's
+// entry, page and angles are looked up.
 template <bool F16>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     __shared__ float2 turn[128];  // cosine, sine
-    const int i = blockIdx.x;
-    const int b = entry_of(a.pb, i);
+    const int64_t i = blockIdx.x;
+    const int tid = threadIdx.x;
+    const int per = a.half / 8, heads = a.n_heads + a.n_kv, pairs = heads * per;
+    const int vper = a.hd / 8, values = a.n_kv * vper;
+    // vector pair w of the token: its first half (the second is a.half on)
+    auto source = [&](int w) {
+        const int h = w / per, f = (w - h * per) * 8;
+        return (h < a.n_heads ? a.q + i * a.q_ld + (int64_t)h * a.hd
+                              : a.k + i * a.k_ld + (int64_t)(h - a.n_heads) * a.hd) +
+               f;
+    };
+    auto value = [&](int w) {
+        const int h = w / vper;
+        return a.v + i * a.v_ld + (int64_t)h * a.hd + (w - h * vper) * 8;
+    };
+    constexpr int kFirst = 3;
+    uint4 x[kFirst], y[kFirst], vv = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j) {
+        const int w = tid + j * kAppendThreads;
+        if (w < pairs) {
+            const uint16_t *src = source(w);
+            x[j] = *reinterpret_cast<const uint4 *>(src);
+            y[j] = *reinterpret_cast<const uint4 *>(src + a.half);
+        }
+    }
+    if (tid < values) vv = *reinterpret_cast<const uint4 *>(value(tid));
+
+    const int b = entry_of(a.pb, (int)i);
     if (b < 0) return;
     const SeqView s = seq_view(a.pb, b);
-    const int t = i - s.q0;
+    const int t = (int)i - s.q0;
     if (t < 0 || t >= s.n) return;  // behind the last sequence, or padding
     const int pos = s.len - s.n + t;
+    for (int f = tid; f < a.half; f += kAppendThreads) {
+        const double u = (double)pos * (double)a.freqs[f] * 0.15915494309189535;  // 1 / 2 pi
+        float sn, cs;
+        sincospif((float)(2.0 * (u - rint(u))), &sn, &cs);
+        turn[f] = make_float2(cs, sn);
+    }
     int page = a.pb.n_pages;
     if (pos >= 0)
         page = page_of(a.pb, s.row, pos);
-    else if (threadIdx.x == 0)
+    else if (tid == 0)
         atomicOr(a.pb.err, kErrBadIndex);  // more new tokens than the length
-    for (int f = threadIdx.x; f < a.half; f += blockDim.x) {
-        const double x = (double)pos * (double)a.freqs[f] * 0.15915494309189535;  // 1 / 2 pi
-        float sn, cs;
-        sincospif((float)(2.0 * (x - rint(x))), &sn, &cs);
-        turn[f] = make_float2(cs, sn);
-    }
     __syncthreads();
     const int64_t place =
         (int64_t)page * a.page_stride + (int64_t)(pos < 0 ? 0 : pos % a.pb.page_size) * a.hd;
     const int64_t head_ld = (int64_t)a.pb.page_size * a.hd;  // next key head's row in a page
     const bool keep = page < a.pb.n_pages;
-    const int per = a.half / 8, heads = a.n_heads + a.n_kv;
-    for (int w = threadIdx.x; w < heads * per; w += blockDim.x) {
+    // where head h of q and k goes (nullptr: nowhere)
+    auto target = [&](int h) -> uint16_t * {
+        if (h < a.n_heads) return a.q_out + i * a.q_out_ld + (int64_t)h * a.hd;
+        return keep ? a.kc + place + (h - a.n_heads) * head_ld : nullptr;
+    };
+    auto put_pair = [&](int w, const uint4 &xv, const uint4 &yv) {
         const int h = w / per, f = (w - h * per) * 8;
-        const bool is_q = h < a.n_heads;
-        const uint16_t *src = is_q ? a.q + i * a.q_ld + (int64_t)h * a.hd
-                                   : a.k + i * a.k_ld + (int64_t)(h - a.n_heads) * a.hd;
-        const uint4 x = *reinterpret_cast<const uint4 *>(src + f);
-        const uint4 y = *reinterpret_cast<const uint4 *>(src + f + a.half);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w}, ys[4] = {yv.x, yv.y, yv.z, yv.w};
         uint32_t u[4], v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -104,29 +135,36 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
             u[j] = pack_t2<F16>(p[0], p[1]);
             v[j] = pack_t2<F16>(r[0], r[1]);
         }
-        if (!is_q && !keep) continue;
-        uint16_t *dst = is_q ? a.q_out + i * a.q_out_ld + (int64_t)h * a.hd
-                             : a.kc + place + (h - a.n_heads) * head_ld;
+        uint16_t *dst = target(h);
+        if (!dst) return;
         *reinterpret_cast<uint4 *>(dst + f) = make_uint4(u[0], u[1], u[2], u[3]);
         *reinterpret_cast<uint4 *>(dst + f + a.half) = make_uint4(v[0], v[1], v[2], v[3]);
+    };
+    auto put_value = [&](int w, const uint4 &v) {
+        const int h = w / vper;
+        if (keep)
+            *reinterpret_cast<uint4 *>(a.vc + place + h * head_ld + (w - h * vper) * 8) = v;
+    };
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j) {
+        const int w = tid + j * kAppendThreads;
+        if (w < pairs) put_pair(w, x[j], y[j]);
     }
+    if (tid < values) put_value(tid, vv);
+    for (int w = tid + kFirst * kAppendThreads; w < pairs; w += kAppendThreads) {
+        const uint16_t *src = source(w);
+        put_pair(w, *reinterpret_cast<const uint4 *>(src),
+                 *reinterpret_cast<const uint4 *>(src + a.half));
+    }
+    for (int w = tid + kAppendThreads; w < values; w += kAppendThreads)
+        put_value(w, *reinterpret_cast<const uint4 *>(value(w)));
     const int rest = (a.hd - 2 * a.half) / 8;  // vectors of a head that are not turned
-    for (int w = threadIdx.x; w < heads * rest; w += blockDim.x) {
+    for (int w = tid; w < heads * rest; w += kAppendThreads) {
         const int h = w / rest, f = 2 * a.half + (w - h * rest) * 8;
-        const bool is_q = h < a.n_heads;
-        if (!is_q && !keep) continue;
-        const uint16_t *src = is_q ? a.q + i * a.q_ld + (int64_t)h * a.hd
-                                   : a.k + i * a.k_ld + (int64_t)(h - a.n_heads) * a.hd;
-        uint16_t *dst = is_q ? a.q_out + i * a.q_out_ld + (int64_t)h * a.hd
-                             : a.kc + place + (h - a.n_heads) * head_ld;
-        *reinterpret_cast<uint4 *>(dst + f) = *reinterpret_cast<const uint4 *>(src + f);
-    }
-    if (!keep) return;
-    const int vper = a.hd / 8;
-    for (int w = threadIdx.x; w < a.n_kv * vper; w += blockDim.x) {
-        const int h = w / vper, f = (w - h * vper) * 8;
-        *reinterpret_cast<uint4 *>(a.vc + place + h * head_ld + f) =
-            *reinterpret_cast<const uint4 *>(a.v + i * a.v_ld + (int64_t)h * a.hd + f);
+        const uint16_t *src = h < a.n_heads ? a.q + i * a.q_ld + (int64_t)h * a.hd
+                                            : a.k + i * a.k_ld + (int64_t)(h - a.n_heads) * a.hd;
+        if (uint16_t *dst = target(h))
+            *reinterpret_cast<uint4 *>(dst + f) = *reinterpret_cast<const uint4 *>(src + f);
     }
 }
 
@@ -687,7 +725,7 @@ int nq_paged_append(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t 
     a.hd = hd;
     a.half = n_freqs;
     auto kern = cache->dtype == NQ_DTYPE_F16 ? paged_append_kernel<true> : paged_append_kernel<false>;
-    return from_cuda(launch_pdl(kern, dim3((unsigned)batch->n_tokens), 256, 0,
+    return from_cuda(launch_pdl(kern, dim3((unsigned)batch->n_tokens), kAppendThreads, 0,
                                 static_cast<cudaStream_t>(stream), a),
                      fn);
 }
