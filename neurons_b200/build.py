@@ -11,6 +11,8 @@ point for TMA descriptors is resolved at run time through
 cudaGetDriverEntryPoint.  `-v` prints ptxas register/spill reports.
 libnq_dist.so (csrc/dist.cu) links libnq.so and the NCCL that ships with
 torch (the same libnccl.so.2 a torch process has already loaded).
+_paged.so (binding/paged_torch.cpp) is the torch binding of the paged cache's
+calls; it links libnq.so and the installed torch.
 """
 import os
 import subprocess
@@ -32,6 +34,10 @@ HEADERS = ["nq_common.cuh", "nq_internal.h", "paged.cuh", "cuda_backend.h", "ifa
 # The reference's interface headers, restated, for building libnq on its own
 # (inside the reference tree its own core/ headers take their place).
 IFACE = os.path.join(CSRC, "iface")
+
+# The torch binding of the paged cache's calls (a CPython module).
+PAGED_LIB = os.path.join(HERE, "_paged.so")
+PAGED_SOURCE = os.path.join(HERE, "binding", "paged_torch.cpp")
 
 DIST_LIB = os.path.join(HERE, "libnq_dist.so")
 DIST_SOURCE = "dist.cu"
@@ -87,7 +93,31 @@ def build(force: bool = False, verbose: bool = False) -> str:
                        check=True)
         os.replace(tmp, LIB)
     build_dist(force, verbose)
+    build_paged(force)
     return LIB
+
+
+def build_paged(force: bool = False) -> str:
+    """neurons_b200/_paged.so against the installed torch's headers and libraries."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    s = PAGED_SOURCE
+    o = os.path.join(BUILD, os.path.basename(s) + ".o")
+    if force or _newer(o, [s, os.path.join(INCLUDE, "nq.h")]):
+        inc = cpp_extension.include_paths() + [os.path.join(CUDA_HOME, "include"),
+                                               sysconfig.get_paths()["include"], INCLUDE]
+        subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-DNDEBUG",
+                        "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI] +
+                       [a for d in inc for a in ("-isystem" if d != INCLUDE else "-I", d)] +
+                       ["-c", s, "-o", o], check=True)
+    if force or _newer(PAGED_LIB, [o, LIB]):
+        tmp = PAGED_LIB + ".tmp%d" % os.getpid()
+        libs = [a for d in cpp_extension.library_paths() for a in ("-L" + d, "-Wl,-rpath," + d)]
+        subprocess.run(["g++", "-shared", "-o", tmp, o, "-L" + HERE, "-lnq", "-Wl,-rpath,$ORIGIN"] +
+                       libs + ["-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"], check=True)
+        os.replace(tmp, PAGED_LIB)
+    return PAGED_LIB
 
 
 def build_dist(force: bool = False, verbose: bool = False) -> str:

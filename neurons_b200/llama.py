@@ -178,18 +178,20 @@ class PagedLlama:
         meta = self._ids(list(seqs) + new_lens + starts + [e - 1 for e in starts[1:]])
         ids, lens, q_starts, rows = meta.split([n, n, n + 1, n])
         paged.pages_reserve(self.pool, self.refs, self.table, self.lens, ids, lens)
-        cache = paged._cache(self.pool[0, 0], self.pool[0, 1])[0]
-        batch = paged._batch(self.table, self.lens, ids, q_starts, total, self.pool.get_device())
-        d = self.decoder
+        d, pool, table = self.decoder, self.pool, self.table
+        cache = paged.Cache(pool.data_ptr(), pool[0, 1].data_ptr(), pool.shape[2], pool.stride(2),
+                            *pool.shape[3:], 1)
+        batch = paged.Batch(table.data_ptr(), table.shape[1], table.shape[1], table.shape[0],
+                            self.lens.data_ptr(), ids.data_ptr(), q_starts.data_ptr(), n, total)
         lg = torch.empty((n, d.vocab), dtype=torch.float32, device="cuda") if logits else None
         nxt = torch.empty(n, dtype=torch.int32, device="cuda")
         most = max(news)
         f = lib()
         need = f.nq_llama_forward_workspace_size(d.handle, total, n, most,
-                                                 self.table.shape[1] * self.pool.shape[-2])
+                                                 table.shape[1] * pool.shape[-2])
         ws = torch.empty(need, dtype=torch.uint8, device="cuda")
         check(f.nq_llama_forward(d.handle, tokens.data_ptr(), ctypes.byref(cache),
-                                 self.pool.stride(0), ctypes.byref(batch), most, rows.data_ptr(), n,
+                                 pool.stride(0), ctypes.byref(batch), most, rows.data_ptr(), n,
                                  lg.data_ptr() if logits else None, nxt.data_ptr(), ws.data_ptr(),
                                  need, ops._stream()))
         for s, m in zip(seqs, new_lens):

@@ -155,10 +155,10 @@ def test_serving_refusals(nqlib, model):
 def test_forward_refusals(nqlib, model):
     _, dev = model
     dec = LlamaDecoder(cfg(), dev)
-    from neurons_b200.paged import _Batch, _Cache
+    from neurons_b200.paged import Batch, Cache
     z = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda").data_ptr()
-    ok = dict(tokens=z, cache=_Cache(z, z, 2, 2 * 16 * 128, 2, 16, 128, 1), stride=1 << 14,
-              batch=_Batch(z, 1, 1, 1, z, None, None, 1, 1), max_q=1, rows=z, n_out=1, logits=z,
+    ok = dict(tokens=z, cache=Cache(z, z, 2, 2 * 16 * 128, 2, 16, 128, 1), stride=1 << 14,
+              batch=Batch(z, 1, 1, 1, z, None, None, 1, 1), max_q=1, rows=z, n_out=1, logits=z,
               ws=z, ws_bytes=16)
 
     def call(**kw):
@@ -169,8 +169,8 @@ def test_forward_refusals(nqlib, model):
 
     for kw in (dict(), dict(tokens=None), dict(ws=None), dict(rows=None), dict(logits=None),
                dict(max_q=-1), dict(n_out=-1), dict(stride=4), dict(stride=-8),
-               dict(cache=_Cache(z, z, 2, 4096, 2, 16, 128, 2)),
-               dict(cache=_Cache(z, z, 2, 4096, 1, 16, 128, 1)),
-               dict(cache=_Cache(z, z, 2, 4096, 2, 16, 64, 1))):
+               dict(cache=Cache(z, z, 2, 4096, 2, 16, 128, 2)),
+               dict(cache=Cache(z, z, 2, 4096, 1, 16, 128, 1)),
+               dict(cache=Cache(z, z, 2, 4096, 2, 16, 64, 1))):
         assert call(**kw) == 1, kw
-    assert call(batch=_Batch(z, 1, 1, 1, z, None, None, 0, 0)) == 0
+    assert call(batch=Batch(z, 1, 1, 1, z, None, None, 0, 0)) == 0

@@ -4,7 +4,7 @@ import ctypes
 
 import pytest
 
-from neurons_b200.paged import _Batch, _Cache, _Pool, _Table
+from neurons_b200.paged import Batch, Cache, PagePool, PageTable
 
 A = 1 << 20  # an aligned address that validation never reads
 
@@ -13,14 +13,14 @@ def cache(**kw):
     d = dict(k=A, v=A, n_pages=8, page_stride=2 * 16 * 64, n_kv_heads=2, page_size=16, head_dim=64,
              dtype=1)
     d.update(kw)
-    return _Cache(**d)
+    return Cache(**d)
 
 
 def batch(**kw):
     d = dict(table=A, table_ld=4, table_width=4, n_rows=2, kv_lens=A, seqs=None, q_starts=A,
              n_seqs=2, n_tokens=6)
     d.update(kw)
-    return _Batch(**d)
+    return Batch(**d)
 
 
 def attend(lib, c=None, b=None, heads=4, q=A, q_ld=256, max_q=4, scale=0.1, window=0, ws=A,
@@ -105,13 +105,13 @@ def test_workspace_size_of_bad_shapes_is_zero(nqlib):
 def table(**kw):
     d = dict(refs=A, table=A, lens=A, n_pages=8, n_rows=4, table_ld=4, table_width=4, page_size=16)
     d.update(kw)
-    return _Table(**d)
+    return PageTable(**d)
 
 
 def pool(**kw):
     d = dict(data=A, outer=2, n_pages=8, page_bytes=64)
     d.update(kw)
-    return _Pool(**d)
+    return PagePool(**d)
 
 
 BAD_TABLES = [dict(refs=None), dict(table=None), dict(lens=None), dict(n_pages=0), dict(n_rows=0),
