@@ -682,7 +682,8 @@ int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_pa
     c.n_heads = n_heads;
     c.n_kv = cache->n_kv_heads;
     c.head_dim = cache->head_dim;
-    c.window = (int)std::min<int64_t>(window, kMaxInt);
+    // (a window as long as the table hides nothing)
+    c.window = window < (int64_t)c.pb.table_width * c.pb.page_size ? (int)window : 0;
     c.f16 = cache->dtype == NQ_DTYPE_F16;
     c.scale = scale;
     c.ws = workspace;

@@ -130,6 +130,52 @@ def test_padding_entries_are_skipped(news):
     assert nb.take_device_error() == 0
 
 
+@pytest.mark.parametrize("window", [1 << 20, 1 << 31, 1 << 62])
+@pytest.mark.parametrize("news", [[1, 1], [40, 9]])
+def test_a_window_longer_than_the_table(window, news):
+    b = Batch([300, 9], news, 8, 2, 128, 16, BF, seed=14)
+    assert torch.equal(b.call(nb, window=window), b.call(nb))
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [70, 1, 9]])
+def test_strided_table_rows_and_queries(news):
+    """A table that is a part of a wider one, queries and results in rows of others."""
+    b = Batch([200, 90, 700], news, 8, 2, 64, 32, HF, seed=15)
+    wide = torch.full((b.table.shape[0], b.table.shape[1] + 5), 1 << 20, dtype=torch.int32,
+                      device="cuda")
+    wide[:, :b.table.shape[1]] = b.table
+    want = b.call(nb)
+    room = torch.full((b.tokens, 3, 8, 64), 2.0, dtype=HF, device="cuda")
+    got = nb.paged_attention(b.q, b.k, b.v, wide[:, :b.table.shape[1]], b.row_lens,
+                             q_starts=b.starts, seqs=b.seqs, out=room[:, 1])
+    assert torch.equal(got, want)
+    assert (room[:, 0] == 2).all() and (room[:, 2] == 2).all()
+    assert nb.take_device_error() == 0
+
+
+def test_a_long_prompt_beside_many_steps():
+    """More than 32 sequences, a prompt of several tiles among them."""
+    lens = [700] + [17 * i % 600 + 1 for i in range(70)]
+    b = Batch(lens, [700] + [1] * 70, 4, 2, 64, 32, BF, seed=16)
+    check_attention(b.call(nb, max_q=700), b)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams whose workspaces are torch's: each gets its own result."""
+    bs = [Batch([3000, 40], [n, 1], 8, 2, 128, 16, BF, seed=17 + n) for n in (1, 50)]
+    want = [b.call(nb).clone() for b in bs]
+    streams = [torch.cuda.Stream() for _ in bs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (b, s) in enumerate(zip(bs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(b.call(nb))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+
+
 def test_without_q_starts_and_seqs():
     b = Batch([90, 300, 200], [1, 1, 1], 8, 2, 128, 16, BF, seed=9)
     q = torch.empty_like(b.q)
