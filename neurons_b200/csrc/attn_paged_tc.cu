@@ -37,20 +37,26 @@ namespace nq {
 namespace {
 
 constexpr int kBlock = 128;  // keys per block, rows per query tile
-// The weights of a block's first kMost keys are handed over early, so that most
-// of P V runs while the rest are still being made.
-constexpr int kMost = 96;
 
 template <int HD>
 struct Tc {
     static constexpr int kGroups = HD == 256 ? 1 : 2;       // softmax warpgroups
     static constexpr int kMmaWarp = 4 * kGroups, kKeyWarp = kMmaWarp + 1;
     static constexpr int kValueWarp = kKeyWarp + 1, kQueryWarp = kValueWarp + 1;
-    // A third (second) warpgroup of MMA, key, value and query warp.  With
+    // The last warpgroup is one MMA, one key, one value and one query warp.  With
     // two softmax warpgroups registers are moved between them: 168 each at launch
     // (all of the SM's 64 K), then 208 for a softmax thread, which holds a row of 128
     // scores, and 88 for the others; 2 * 208 + 88 = 3 * 168.
     static constexpr int kThreads = 128 * (kGroups + 1);
+    // S in TMEM per group, beside O.  One each for two groups: 64 keys in two S each
+    // would have the next S ready when a softmax is done, but an MMA of 64 columns
+    // takes 68 cycles where one of 128 takes 83 (its 128 query rows come from shared
+    // memory either way), and a prompt of 8192 tokens 556 us instead of 496.
+    static constexpr int kBufs = kGroups == 2 ? 1 : 2;
+    // The weights of a step's first kMost keys are handed over early, so that most of
+    // P V runs while the rest are still being made (96 of 128: a prompt of 8192 tokens
+    // 519 -> 492 us; with 256 dims, where the MMAs are the bound, 440 -> 475).
+    static constexpr int kMost = kGroups == 2 ? 96 : kBlock;
     // a ring stage: 128 keys (or values) x kUnitDims dims
     static constexpr int kUnitDims = HD < 128 ? HD : 128;
     static constexpr int kUnits = HD / kUnitDims;
@@ -185,17 +191,19 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
         "r"(r[29]), "r"(r[30]), "r"(r[31]));
 }
 
-// The blocks of a piece as steps: step i works on S buffer i % 2.
+// The blocks of a piece as the groups' steps; step i works on the group's S
+// buffer i % kBufs.
 template <int HD>
 struct Plan {
-    bool two;    // two query tiles: steps 2b and 2b + 1 are block b
+    bool two;    // two query tiles, a group each; else the groups take the blocks in turn
     int n;       // blocks
-    int tok;     // tokens per query tile
-    __device__ __forceinline__ Plan(const Piece &p, int tok_)
-        : two(Tc<HD>::kGroups == 2 && p.t1 - p.t0 > tok_), n(p.k1 - p.k0), tok(tok_) {}
-    __device__ __forceinline__ int steps() const { return two ? 2 * n : n; }
-    __device__ __forceinline__ int block(int i) const { return two ? i >> 1 : i; }
-    __device__ __forceinline__ bool last_use(int i) const { return !two || (i & 1); }
+    __device__ __forceinline__ Plan(const Piece &p, int tok)
+        : two(Tc<HD>::kGroups == 2 && p.t1 - p.t0 > tok), n(p.k1 - p.k0) {}
+    __device__ __forceinline__ bool turns() const { return Tc<HD>::kGroups == 2 && !two; }
+    __device__ __forceinline__ int steps(int w) const { return turns() ? (n + 1 - w) / 2 : n; }
+    __device__ __forceinline__ int block(int w, int i) const { return turns() ? 2 * i + w : i; }
+    // whether group w is the last that uses a block's keys and values
+    __device__ __forceinline__ bool last_use(int w) const { return !two || w == 1; }
 };
 
 // A piece as the key warp, which alone walks the list, hands it to the others
@@ -232,9 +240,9 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     // a ring of keys and one of values: a ring has one producer, or its waits would be
     // ambiguous
     __shared__ __align__(8) uint64_t full_k[T::kStages], empty_k[T::kStages];
-    __shared__ __align__(8) uint64_t full_v[T::kStages], empty_v[T::kStages], s_full[2];
-    __shared__ __align__(8) uint64_t p_most[2], p_rest[2];
-    __shared__ __align__(8) uint64_t q_full, q_empty, o_full, pv_done;
+    __shared__ __align__(8) uint64_t full_v[T::kStages], empty_v[T::kStages];
+    __shared__ __align__(8) uint64_t s_full[2], p_most[2], p_ready[2];  // per S
+    __shared__ __align__(8) uint64_t q_full, q_empty, o_full, pv_done[T::kGroups];
     __shared__ uint32_t tmem_holder;
     __shared__ int abort_flag;
     __shared__ float2 xml[T::kGroups == 2 ? 2 * kBlock : 1];
@@ -254,17 +262,17 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             mbar_init(&full_v[i], 1);
             mbar_init(&empty_v[i], 1);
         }
+        for (int i = 0; i < T::kGroups; ++i) mbar_init(&pv_done[i], 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_most[i], 4);  // (one arrival per warp)
-            mbar_init(&p_rest[i], 4);
+            mbar_init(&p_ready[i], 4);
             mbar_init(&job_full[i], 1);
             mbar_init(&job_empty[i], 3 + 4 * T::kGroups);  // the other warps
         }
         mbar_init(&q_full, 1);
         mbar_init(&q_empty, 1);
         mbar_init(&o_full, 1);
-        mbar_init(&pv_done, 1);
         abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&mq);
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                        v_lo = desc_mn(smem_u32(ring_v));
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         int blocks = 0, pieces = 0;  // finished
-        uint32_t p_phase = 0;  // bit: parity of that buffer's next p_most and p_rest
+        uint32_t p_phase = 0;        // bit: parity of that S's next p_most and p_ready
         bool ok = true;
         auto wait = [&](uint64_t *bar, uint32_t parity) {
             return __all_sync(0xffffffffu, mbar_poll_or_abort(bar, parity, abort, a.pb.err)) != 0;
@@ -376,13 +384,13 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             pl.n = __shfl_sync(0xffffffffu, jobs[slot].n, 0);
             pl.two = __all_sync(0xffffffffu, pl.two);
             if (pl.n == 0) break;
-            const int steps = pl.steps();
             __syncwarp();
             if (lane == 0) mbar_arrive(&job_empty[slot]);
             ok = wait(&q_full, (uint32_t)pieces & 1u);
-            auto issue_s = [&](int i) {
-                const int b = pl.block(i), buf = i & 1;
-                const uint32_t qd = q_lo + (pl.two && buf ? T::kQBytes >> 4 : 0);
+            int s_left = T::kGroups == 2 ? pl.steps(0) + pl.steps(1) : pl.steps(0);
+            auto issue_s = [&](int w, int i) {
+                const int b = pl.block(w, i), at = w * T::kBufs + i % T::kBufs;
+                const uint32_t qd = q_lo + (pl.two && w ? T::kQBytes >> 4 : 0);
 #pragma unroll
                 for (int u = 0; u < T::kUnits; ++u) {
                     const int g = (blocks + b) * T::kUnits + u;
@@ -394,46 +402,56 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     for (int kk = 0; kk < T::kUnitDims / 16; ++kk) {
                         // 16 dims: 32 bytes on in the swizzled rows; 64: the next column
                         const uint32_t off = ((kk >> 2) * (kBlock * 128) + (kk & 3) * 32) >> 4;
-                        mma_ss(tm + buf * 128,
+                        mma_ss(tm + at * kBlock,
                                qd + (u * (T::kUnitDims / 64) * (kBlock * 128) >> 4) + off, kDescHi,
                                kd + off, kDescHi, kIdS, (u > 0 || kk > 0) ? 1u : 0u);
                     }
-                    if (pl.last_use(i)) mma_commit(&empty_k[g % T::kStages]);
+                    if (pl.last_use(w)) mma_commit(&empty_k[g % T::kStages]);
                 }
-                mma_commit(&s_full[buf]);
-                if (i + 1 == steps) mma_commit(&q_empty);
+                mma_commit(&s_full[at]);
+                if (--s_left == 0) mma_commit(&q_empty);
             };
-            if (ok) issue_s(0);
-            if (ok && steps > 1) issue_s(1);
-            for (int i = 0; ok && i < steps; ++i) {
-                const int b = pl.block(i), buf = i & 1;
-                ok = wait(&p_most[buf], (p_phase >> buf) & 1u);
-                if (!ok) break;
-                const uint32_t acc = T::kGroups == 2 ? i > 1 : i > 0;
-                const uint32_t o = tm + T::kO + (T::kGroups == 2 ? buf * HD : 0);
 #pragma unroll
-                for (int u = 0; u < T::kUnits; ++u) {
-                    const int g = (blocks + b) * T::kUnits + u;
-                    wait_stage(full_v, g);
+            for (int i = 0; i < T::kBufs; ++i)
+#pragma unroll
+                for (int w = 0; w < T::kGroups; ++w)
+                    if (ok && i < pl.steps(w)) issue_s(w, i);
+            for (int i = 0; ok && i < pl.steps(0); ++i) {
+                // (not unrolled: all roles' code shares one instruction cache, and two copies
+                // of this one cost a prompt of 8192 tokens 532 us instead of 483)
+#pragma unroll 1
+                for (int w = 0; w < T::kGroups; ++w) {
+                    if (i >= pl.steps(w)) continue;
+                    const int b = pl.block(w, i), at = w * T::kBufs + i % T::kBufs;
+                    ok = ok && wait(T::kMost < kBlock ? &p_most[at] : &p_ready[at],
+                                    (p_phase >> at) & 1u);
                     if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t vd = v_lo + (g % T::kStages) * (T::kUnitBytes >> 4);
+                    const uint32_t o = tm + T::kO + w * HD;
 #pragma unroll
-                    for (int kk = 0; kk < kBlock / 16; ++kk) {
-                        if (u == 0 && kk == kMost / 16) {
-                            ok = wait(&p_rest[buf], (p_phase >> buf) & 1u);
-                            if (!ok) break;
-                            p_phase ^= 1u << buf;
-                            tc_fence_after();
+                    for (int u = 0; u < T::kUnits; ++u) {
+                        const int g = (blocks + b) * T::kUnits + u;
+                        wait_stage(full_v, g);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t vd = v_lo + (g % T::kStages) * (T::kUnitBytes >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < kBlock / 16; ++kk) {
+                            if (u == 0 && kk == T::kMost / 16) {
+                                ok = wait(&p_ready[at], (p_phase >> at) & 1u);
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            mma_ts(o + u * T::kUnitDims, tm + at * kBlock + kk * 8,
+                                   vd + (kk * 16 * 128 >> 4), kDescHi, kIdO,
+                                   (i > 0 || kk > 0) ? 1u : 0u);
                         }
-                        mma_ts(o + u * T::kUnitDims, tm + buf * 128 + kk * 8,
-                               vd + (kk * 16 * 128 >> 4), kDescHi, kIdO, (acc || kk > 0) ? 1u : 0u);
+                        if (!ok) break;
+                        if (pl.last_use(w)) mma_commit(&empty_v[g % T::kStages]);
                     }
-                    if (!ok) break;
-                    if (pl.last_use(i)) mma_commit(&empty_v[g % T::kStages]);
+                    p_phase ^= 1u << at;
+                    mma_commit(&pv_done[w]);
+                    if (ok && i + T::kBufs < pl.steps(w)) issue_s(w, i + T::kBufs);
                 }
-                if (T::kGroups == 1) mma_commit(&pv_done);
-                if (ok && i + 2 < steps) issue_s(i + 2);
             }
             mma_commit(&o_full);
             blocks += pl.n;
@@ -494,42 +512,42 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             if (!ok || job.n == 0) break;
             const Piece &p = job.p;
             const Plan<HD> pl(p, tok);
-            const int steps = pl.steps();
+            const int steps = pl.steps(w);
             const int sub = pl.two ? w : 0;         // which query tile
             const int t0 = p.t0 + sub * tok, t1 = min(t0 + tok, p.t1);
             const int valid = (t1 - t0) * G;
             const int base = p.s.len - p.s.n;
             const int pos = r < valid ? base + t0 + (int)((uint32_t)r * inv_g >> 16) : -1;
-            // steps whose block reaches past the first row's position, or below the last
+            // steps whose keys reach past the first row's position, or below the last
             // row's window, are masked
             const int full_to = base + t0 + 1 - kBlock;
             const int full_from = a.window > 0 ? base + t1 - a.window : 0;
             const int block0 = p.lo + p.k0;
             float m = -INFINITY, l = 0.f;
-            bool first = true;
-            for (int i = T::kGroups == 2 ? w : 0; i < steps; i += T::kGroups) {
-                const int buf = i & 1, b = pl.block(i);
+            for (int i = 0; i < steps; ++i) {
+                const int buf = i % T::kBufs, at = w * T::kBufs + buf, b = pl.block(w, i);
                 ok = ok && !*abort &&
-                     mbar_poll_or_abort(&s_full[buf], (s_phase >> buf) & 1u, abort, a.pb.err);
+                     mbar_poll_or_abort(&s_full[at], (s_phase >> buf) & 1u, abort, a.pb.err);
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
                 }
                 s_phase ^= 1u << buf;
                 tc_fence_after();
-                const uint32_t sc = tmem + lanes + buf * 128;
-                float s[128];
+                const uint32_t sc = tmem + lanes + at * kBlock;
+                float s[kBlock];
                 float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 const int key0 = (block0 + b) * kBlock;
                 const bool masked = key0 > full_to || key0 < full_from;
                 const int hi = pos - key0, lo = a.window > 0 ? hi - a.window + 1 : 0;
+                // (the second half on its way while the first one's maximum is taken)
                 tmem_ld_32x32b_x32(sc, *reinterpret_cast<uint32_t(*)[32]>(s));
                 tmem_ld_32x32b_x32(sc + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
                 tmem_ld_wait();
                 tmem_ld_32x32b_x32(sc + 64, *reinterpret_cast<uint32_t(*)[32]>(s + 64));
                 tmem_ld_32x32b_x32(sc + 96, *reinterpret_cast<uint32_t(*)[32]>(s + 96));
 #pragma unroll
-                for (int c = 0; c < 128; c += 64) {
+                for (int c = 0; c < kBlock; c += 64) {
                     if (c > 0) tmem_ld_wait();
                     if (masked) {
 #pragma unroll
@@ -546,15 +564,13 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 // (m == -inf: the difference is +inf, or NaN when the row has no key yet)
                 if (__any_sync(0xffffffffu, (mn - m) * cs > 8.f)) {
                     const float f = m == -INFINITY ? 0.f : ex2((m - mn) * cs);
-                    if (!first) {
-                        if (T::kGroups == 1) {
-                            // O still takes the last block's product: wait for it
-                            ok = mbar_wait_or_abort(&pv_done, (uint32_t)(pvs + i - 1) & 1u, abort,
-                                                    a.pb.err);
-                            ok = __all_sync(0xffffffffu, ok);
-                            tc_fence_after();
-                        }
-                        const uint32_t oc = tmem + lanes + T::kO + (T::kGroups == 2 ? w * HD : 0);
+                    if (i > 0) {
+                        // O still takes the last step's product: wait for it
+                        ok = mbar_wait_or_abort(&pv_done[w], (uint32_t)(pvs + i - 1) & 1u, abort,
+                                                a.pb.err);
+                        ok = __all_sync(0xffffffffu, ok);
+                        tc_fence_after();
+                        const uint32_t oc = tmem + lanes + T::kO + w * HD;
 #pragma unroll 1
                         for (int j = 0; j < HD; j += 32) {
                             uint32_t v[32];
@@ -569,7 +585,6 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     l *= f;
                     m = mn;
                 }
-                first = false;
                 const int key_hi = p.s.len - p.s.n + p.t1;
                 const int key_lo = a.window > 0 ? p.s.len - p.s.n + p.t0 - a.window + 1 : 0;
                 if (key0 < key_lo || key0 + kBlock > key_hi) {
@@ -580,8 +595,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     // (256 dims: the stage's last values may still be under way, and a wait two
                     // phases ahead would be ambiguous)
                     if (T::kGroups == 1 && i > 0)
-                        ok = ok && mbar_wait_or_abort(&pv_done, (uint32_t)(pvs + i - 1) & 1u, abort,
-                                                      a.pb.err);
+                        ok = ok && mbar_wait_or_abort(&pv_done[w], (uint32_t)(pvs + i - 1) & 1u,
+                                                      abort, a.pb.err);
 #pragma unroll
                     for (int u = 0; u < T::kUnits; ++u) {
                         const int g = (blocks + b) * T::kUnits + u;
@@ -589,7 +604,8 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                                                       (uint32_t)(g / T::kStages) & 1u, abort,
                                                       a.pb.err);
                         if (ok && clear) {
-                            uint8_t *v = ring_v + (g % T::kStages) * T::kUnitBytes + r * 128;
+                            uint8_t *v = ring_v + (g % T::kStages) * T::kUnitBytes +
+                                         r * 128;
 #pragma unroll
                             for (int j = 0; j < T::kUnitDims / 8; ++j)
                                 *reinterpret_cast<uint4 *>(v + (j >> 3) * (kBlock * 128) +
@@ -602,7 +618,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 const float z = m == -INFINITY ? 0.f : m * cs;
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < kBlock / 32; ++j) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -614,17 +630,17 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                         pk[e] = pack_t2<F16>(e0, e1);
                     }
                     tmem_st_32x32b_x16(sc + j * 16, pk);
-                    if (j * 32 + 32 == kMost) {
+                    if (T::kMost < kBlock && j * 32 + 32 == T::kMost) {
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&p_most[buf]);
+                        if (lane == 0) mbar_arrive(&p_most[at]);
                     }
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_rest[buf]);
+                if (lane == 0) mbar_arrive(&p_ready[at]);
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             ok = ok && !*abort &&
@@ -650,7 +666,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                 const float inv = L == 0.f ? 0.f : (whole ? 1.f / L : 1.f);
                 f0 *= inv;
                 f1 *= inv;
-                const bool both = join && steps > 1;
+                const bool both = join && pl.n > 1;  // (else the second has no step)
                 const bool none = L == 0.f;
                 const int slot = 2 * blockIdx.x + (p.k0 == 0 ? 1 : 0);
                 const int row = sub * tok * G + r;
