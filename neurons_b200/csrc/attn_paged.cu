@@ -464,61 +464,67 @@ __device__ __forceinline__ int64_t part_slot(int c, int i) {
 }
 
 // Joins the parts of the tiles that several CTAs shared, in the CTAs' order:
-// paged_rows_kernel's, [row][dim], few rows in many parts.  One CTA per row, its
-// four warps take the parts in turn.
+// paged_rows_kernel's, [row][dim], few rows in many parts.  One CTA per row; its
+// four warps take the parts in turn, once, with running maxima that they join at
+// the end.
 template <int HD, bool F16>
 __global__ void __launch_bounds__(128) paged_merge_rows_kernel(const PagedAttnArgs a, int rows) {
     pdl_launch_dependents();
     pdl_wait();
-    __shared__ float sums[4][HD + 1];
+    __shared__ float sums[4][HD + 2];
     const SplitNote note = a.notes[blockIdx.x];
     if (note.parts == 0) return;
     const int G = a.n_heads / a.n_kv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r = blockIdx.y;
     if (r >= note.tokens * G) return;
-    constexpr int kPer = HD / 32;
-    float M = -INFINITY;
-    for (int i = lane; i < note.parts; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2 *>(
-            a.part_ml + (part_slot(blockIdx.x, i) * rows + r) * 2);
-        if (ml.y != 0.f) M = fmaxf(M, ml.x);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-    float L = 0.f, acc[kPer];
+    constexpr int kPer = HD / 32, kAhead = 4;
+    float M = -INFINITY, L = 0.f, acc[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < note.parts; i += 4) {
-        const int64_t at = part_slot(blockIdx.x, i) * rows + r;
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
-        const float *po = a.part_o + at * HD + lane * kPer;
-        float v[kPer];
+    for (int i0 = warp; i0 < note.parts; i0 += 4 * kAhead) {
+        float2 ml[kAhead], v[kAhead][kPer / 2];
 #pragma unroll
-        for (int j = 0; j < kPer; j += 2) {
-            const float2 w = *reinterpret_cast<const float2 *>(po + j);
-            v[j] = w.x;
-            v[j + 1] = w.y;
+        for (int e = 0; e < kAhead; ++e) {
+            if (i0 + 4 * e >= note.parts) break;
+            const int64_t at = part_slot(blockIdx.x, i0 + 4 * e) * rows + r;
+            ml[e] = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
+#pragma unroll
+            for (int j = 0; j < kPer / 2; ++j)
+                v[e][j] = *reinterpret_cast<const float2 *>(a.part_o + at * HD + lane * kPer + 2 * j);
         }
-        const float f = ml.y != 0.f ? ex2(ml.x - M) : 0.f;
-        L += ml.y * f;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) acc[j] = fmaf(v[j], f, acc[j]);
+        for (int e = 0; e < kAhead; ++e) {
+            if (i0 + 4 * e >= note.parts || ml[e].y == 0.f) continue;
+            const float mn = fmaxf(M, ml[e].x);
+            const float f = M == -INFINITY ? 0.f : ex2(M - mn), g = ex2(ml[e].x - mn);
+            M = mn;
+            L = fmaf(L, f, ml[e].y * g);
+#pragma unroll
+            for (int j = 0; j < kPer / 2; ++j) {
+                acc[2 * j] = fmaf(acc[2 * j], f, v[e][j].x * g);
+                acc[2 * j + 1] = fmaf(acc[2 * j + 1], f, v[e][j].y * g);
+            }
+        }
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sums[warp][lane * kPer + j] = acc[j];
-    if (lane == 0) sums[warp][HD] = L;
+    if (lane == 0) {
+        sums[warp][HD] = L;
+        sums[warp][HD + 1] = M;
+    }
     __syncthreads();
     if (warp > 0) return;
+    M = fmaxf(fmaxf(sums[0][HD + 1], sums[1][HD + 1]), fmaxf(sums[2][HD + 1], sums[3][HD + 1]));
     L = 0.f;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        L += sums[w][HD];
+        const float f = sums[w][HD] == 0.f ? 0.f : ex2(sums[w][HD + 1] - M);
+        L = fmaf(sums[w][HD], f, L);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) acc[j] += sums[w][lane * kPer + j];
+        for (int j = 0; j < kPer; ++j) acc[j] = fmaf(sums[w][lane * kPer + j], f, acc[j]);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     uint16_t *op = a.out + (int64_t)(note.q_row + r / G) * a.out_ld +
