@@ -35,25 +35,29 @@ struct SeqView {
 // Reads entry b.  What the arrays say outside their ranges (a table row, a
 // length past the table's width, token rows past n_tokens) is cut to the range
 // and raises the error word; a padding entry has n == 0.
+// (All loads first: each is a trip to L2, and a call waits for them before its
+// first key.)
 __device__ __forceinline__ SeqView seq_view(const PagedBatch &pb, int b) {
     SeqView s;
-    bool bad = false;
     s.row = pb.seqs ? pb.seqs[b] : b;
+    int end = b + 1;
+    s.q0 = b;
     if (pb.q_starts) {
         s.q0 = pb.q_starts[b];
-        s.n = pb.q_starts[b + 1] - s.q0;
-    } else {
-        s.q0 = b;
-        s.n = 1;
+        end = pb.q_starts[b + 1];
     }
-    if (s.q0 < 0 || s.q0 > pb.n_tokens || s.n < 0) {
+    s.len = pb.lens[min(max(s.row, 0), pb.n_rows - 1)];
+    s.n = end - s.q0;
+    bool bad = false;
+    if (s.q0 < 0 || s.q0 > pb.n_tokens || end < s.q0) {
         bad = true;
         s.q0 = 0;
         s.n = 0;
-    } else if (s.n > pb.n_tokens - s.q0) {
+    } else if (end > pb.n_tokens) {
         bad = true;
         s.n = pb.n_tokens - s.q0;
     }
+    const int64_t most = (int64_t)pb.table_width * pb.page_size;
     if (s.row < 0) {
         s.n = 0;
         s.len = 0;
@@ -61,13 +65,9 @@ __device__ __forceinline__ SeqView seq_view(const PagedBatch &pb, int b) {
         bad = true;
         s.row = 0;
         s.len = 0;
-    } else {
-        s.len = pb.lens[s.row];
-        const int64_t most = (int64_t)pb.table_width * pb.page_size;
-        if (s.len < 0 || s.len > most) {
-            bad = true;
-            s.len = s.len < 0 ? 0 : (int)most;
-        }
+    } else if (s.len < 0 || s.len > most) {
+        bad = true;
+        s.len = s.len < 0 ? 0 : (int)most;
     }
     if (bad) atomicOr(pb.err, kErrBadIndex);
     return s;
