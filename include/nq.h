@@ -371,7 +371,7 @@ typedef struct nq_paged_batch {
  * token's window reaches, may hold anything; the values that the rows of one
  * call see have to be finite.  max_q: no entry has more new tokens than this (it
  * selects the kernel and the workspace's size, results hold for any; 0:
- * unknown).  Softmax and sums in fp32; the weights are rounded to the cache's type
+ * unknown, with the workspace that any would need).  Softmax and sums in fp32; the weights are rounded to the cache's type
  * for the second product, the result once.  workspace: nq_paged_attention_
  * workspace_size() bytes for this max_q and max_keys = table_width *
  * page_size (0: none is needed), 256-byte aligned, contents irrelevant; two
@@ -391,7 +391,9 @@ int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_pa
  * once; dims past 2 * n_freqs stay.  n_freqs is a multiple of 8, at most
  * head_dim / 2; 0 turns nothing.  The queries go to q_out (may be q itself).
  * A token at a negative position or whose page is missing is not stored (error
- * word). */
+ * word).  Two entries of one call must not be the same sequence, nor hold their
+ * new tokens' pages in common (nq_pages_reserve parts such pages): which of their
+ * keys stay is not defined. */
 int nq_paged_append(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t k_ld,
                     const uint16_t *v, int64_t v_ld, int n_heads, const nq_paged_cache_t *cache,
                     const nq_paged_batch_t *batch, const float *freqs, int n_freqs, uint16_t *q_out,
@@ -429,8 +431,8 @@ int nq_pages_fork(const nq_page_table_t *table, const int32_t *parents, const in
  * and has other holders is replaced by a copy, and free pages are added, the
  * lowest first, in the list's order.  All or nothing: too few free pages, a
  * length below the present one or past the table, a row out of range or a
- * sequence listed twice refuse the whole call.  workspace:
- * nq_pages_workspace_size(0, n) bytes, 256-byte aligned. */
+ * sequence listed twice refuse the whole call.  n * table_width < 2^31.
+ * workspace: nq_pages_workspace_size(0, n) bytes, 256-byte aligned. */
 size_t nq_pages_workspace_size(int64_t n_pages, int64_t n);
 int nq_pages_reserve(const nq_page_table_t *table, const nq_page_pool_t *pool, const int32_t *seqs,
                      const int32_t *new_lens, int64_t n, void *workspace, size_t workspace_bytes,

@@ -205,8 +205,9 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int64_t dim = c.c.head_dim;
         const Rows q = rows_of(a[0], "q", -1, dim, c.dtype, c.device);
         const nq_paged_batch_t b = batch_of(a[3], a[4], a[9], a[5], q.tokens, c.device);
-        const int64_t max_q =
-            a[5] == Py_None ? 1 : (a[6] == Py_None ? q.tokens : integer(a[6], "max_q"));
+        int64_t max_q = a[6] == Py_None ? 0 : integer(a[6], "max_q");
+        if (a[5] == Py_None) max_q = 1;
+        if (max_q == 0) max_q = q.tokens;
         const int64_t window = integer(a[7], "window");
         double scale = 1.0 / std::sqrt((double)dim);
         if (a[8] != Py_None) {

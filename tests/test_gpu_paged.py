@@ -77,6 +77,16 @@ def test_any_max_q_gives_the_result(max_q):
     check_attention(b.call(nb, max_q=max_q), b)
 
 
+@pytest.mark.parametrize("news", [[1, 1], [3, 40]])
+def test_an_unknown_max_q_with_the_workspace_of_any(news):
+    b = Batch([700, 1900], news, 8, 2, 128, 16, torch.bfloat16, seed=8)
+    size = nb.paged_attention_workspace_size(8, 2, 128, 0, b.table.shape[1] * b.page)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    check_attention(b.call(nb, max_q=0, workspace=ws), b)
+    check_attention(b.call(nb, max_q=0), b)
+    check_attention(b.call(nb, max_q=1 << 62, workspace=ws), b)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_scale_and_strided_cache(dtype):
     """Keys and values side by side in one tensor; a scale of the caller's."""

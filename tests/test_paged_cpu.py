@@ -102,6 +102,14 @@ def test_workspace_size_of_bad_shapes_is_zero(nqlib):
     assert nqlib.nq_pages_workspace_size(0, 0) > 0
 
 
+def test_workspace_size_without_a_known_max_q_is_the_largest(nqlib):
+    size = nqlib.nq_paged_attention_workspace_size
+    for heads, kv_heads, keys in ((32, 8, 8192), (4, 2, 1024), (64, 1, 512), (8, 8, 16)):
+        most = max(size(heads, kv_heads, 128, q, keys) for q in (1, 2, 4, 16, 17, 129, 4096))
+        assert size(heads, kv_heads, 128, 0, keys) == most
+        assert size(heads, kv_heads, 128, 1 << 62, keys) == size(heads, kv_heads, 128, 4096, keys)
+
+
 def table(**kw):
     d = dict(refs=A, table=A, lens=A, n_pages=8, n_rows=4, table_ld=4, table_width=4, page_size=16)
     d.update(kw)
@@ -139,6 +147,12 @@ def test_bad_pools_are_refused(nqlib, bad):
     assert nqlib.nq_pages_compact(t_, p_, A, 1 << 30, None) == 1
     if "n_pages" not in bad or bad["n_pages"] == 0:
         assert nqlib.nq_pages_copy(p_, A, A, 1, None) == 1
+
+
+def test_a_list_that_could_ask_for_2_31_pages_is_refused(nqlib):
+    t, p = table(table_width=1 << 16, table_ld=1 << 16, n_rows=1 << 16), pool()
+    t_, p_ = ctypes.byref(t), ctypes.byref(p)
+    assert nqlib.nq_pages_reserve(t_, p_, A, A, 1 << 15, A, 1 << 40, None) == 1
 
 
 def test_page_lists_and_counts_are_checked(nqlib):
