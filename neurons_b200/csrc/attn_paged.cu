@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     pdl_wait();  // lengths, tables, q and the cache come from earlier kernels
 
     const Tiling tl{TT, TT, a.window, a.whole};
-    Share sh = find_share<kBlock>(a.pb, a.n_kv, tl, blockIdx.x, gridDim.x, a.least);
+    Share sh = find_share<kBlock>(a.pb, a.n_kv, tl, blockIdx.x, gridDim.x);
     Piece p;
     int it = 0;  // blocks so far: stage it % kStages, parity it / kStages
 
@@ -693,7 +693,6 @@ cudaError_t launch_paged_attention(const PagedAttnCall &c, cudaStream_t st) {
     a.n_kv = c.n_kv;
     a.window = c.window;
     a.scale = c.scale;
-    a.least = s.whole ? 1 : Tiling::kMost;
     a.whole = s.whole;
     // the largest power of two that divides the page size: no box crosses a page
     a.box = std::min(s.block, c.pb.page_size & -c.pb.page_size);

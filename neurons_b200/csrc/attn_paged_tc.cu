@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
     };
     if (warp == T::kKeyWarp) {
         const Tiling tl{TT, T::kGroups == 2 ? tok : TT, a.window, a.whole};
-        Share sh = find_share<kBlock>(a.pb, a.n_kv, tl, blockIdx.x, gridDim.x, a.least);
+        Share sh = find_share<kBlock>(a.pb, a.n_kv, tl, blockIdx.x, gridDim.x);
         Piece p;
         int filled = 0, jobs_out = 0;
         bool ok = true, note_left = false;

@@ -102,14 +102,18 @@ struct Tiling {
     static constexpr int kMost = 4;
     int TT, half, window;
     bool whole;  // a tile counts as one unit and is never cut
+    __device__ __forceinline__ int tiles(int n) const { return n <= TT ? n > 0 : (n + TT - 1) / TT; }
     __device__ __forceinline__ int weight(int t0, int t1) const { return t1 - t0 > half ? 4 : 3; }
 };
 
 // A position in the list of all units of a call: entry b, key head h, place t in
 // the order of the token tiles, and `off` units into that tile; `at` is its
-// number and `left` what the CTA still has to do.
+// number and `left` what the CTA still has to do; done: it stands at the end of
+// tile t.  (The step to the next tile is taken with the next piece: it may wait
+// for memory, which a piece in hand need not.)
 struct Cursor {
     int b, h, t, off;
+    bool done;
     int64_t at, left;
     SeqView s;
 };
@@ -138,7 +142,7 @@ template <int BK>
 __device__ __forceinline__ int64_t entry_units_warp(const SeqView &s, const Tiling &tl) {
     // units of one head of this lane's entry; the lanes sum long entries together
     const int lane = threadIdx.x & 31;
-    const int tiles = (s.n + tl.TT - 1) / tl.TT;
+    const int tiles = tl.tiles(s.n);
     if (tl.whole) return tiles;
     int64_t mine = 0;
     if (tiles == 1) mine = tile_units<BK>(s, tl, 0, 1);
@@ -149,7 +153,7 @@ __device__ __forceinline__ int64_t entry_units_warp(const SeqView &s, const Tili
         SeqView o;
         o.n = __shfl_sync(0xffffffffu, s.n, src);
         o.len = __shfl_sync(0xffffffffu, s.len, src);
-        const int ot = (o.n + tl.TT - 1) / tl.TT;
+        const int ot = tl.tiles(o.n);
         int64_t sum = 0;
         for (int t = lane; t < ot; t += 32) sum += tile_units<BK>(o, tl, t, ot);
 #pragma unroll
@@ -159,8 +163,25 @@ __device__ __forceinline__ int64_t entry_units_warp(const SeqView &s, const Tili
     return mine;
 }
 
+// Sums over the warp's lanes of values >= 0; in 32 bits where they fit, which is
+// less of the chain that a call's first key waits for.
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+    if (!__any_sync(0xffffffffu, v >> 26)) return __reduce_add_sync(0xffffffffu, (unsigned)v);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
 __device__ __forceinline__ int64_t warp_inclusive(int64_t v) {
     const int lane = threadIdx.x & 31;
+    if (!__any_sync(0xffffffffu, v >> 26)) {
+        int x = (int)v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += o;
+        }
+        return x;
+    }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
@@ -183,12 +204,13 @@ __device__ __forceinline__ int64_t mul_div(int64_t a, int64_t b, int64_t c) {
     return a * b / c;
 }
 
-// CTAs that take part in a call of `total` units: no share is smaller than
-// `least` units (at least a block's: every share between a tile's first and
-// last one then holds a block of it).
-__device__ __forceinline__ int sharers(int64_t total, int grid, int least) {
+// CTAs that take part in a call of `total` units: no share is smaller than a
+// block's units (every share between a tile's first and last one then holds a
+// block of it), or a whole tile.
+__device__ __forceinline__ int sharers(int64_t total, int grid, bool whole) {
+    const int least = whole ? 1 : Tiling::kMost;
     if (total >= (int64_t)grid * least) return grid;
-    const int n = (int)total / least;
+    const int n = whole ? (int)total : (int)total / Tiling::kMost;
     return n > 0 ? n : 1;
 }
 __device__ __forceinline__ int64_t share_start(int64_t total, int n, int c) {
@@ -204,7 +226,7 @@ __device__ __forceinline__ int share_owner(int64_t total, int n, int64_t u) {
 // Run by one whole warp.
 template <int BK>
 __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, const Tiling &tl,
-                                            int cta, int grid, int least) {
+                                            int cta, int grid) {
     const int lane = threadIdx.x & 31;
     Share sh;
     SeqView s{0, 0, 0, 0};
@@ -215,11 +237,9 @@ __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, cons
         head = entry_units_warp<BK>(s, tl);
         total += head;
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    sh.total = total * n_kv;
-    sh.n = sharers(sh.total, grid, least);
-    sh.c = Cursor{0, 0, 0, 0, 0, 0, SeqView{0, 0, 0, 0}};
+    sh.total = warp_sum(total) * n_kv;
+    sh.n = sharers(sh.total, grid, tl.whole);
+    sh.c = Cursor{0, 0, 0, 0, false, 0, 0, SeqView{0, 0, 0, 0}};
     if (sh.total == 0 || cta >= sh.n) return sh;
     Cursor &c = sh.c;
     c.at = share_start(sh.total, sh.n, cta);
@@ -244,7 +264,11 @@ __device__ __forceinline__ Share find_share(const PagedBatch &pb, int n_kv, cons
             int64_t at = c.at - (__shfl_sync(0xffffffffu, end, src) - per * n_kv);
             c.h = (int)mul_div(at, 1, per);
             at -= c.h * per;
-            const int tiles = (c.s.n + tl.TT - 1) / tl.TT;
+            const int tiles = tl.tiles(c.s.n);
+            if (tiles == 1) {
+                c.off = (int)at;
+                return sh;
+            }
             int64_t seen = 0;
             for (int i0 = 0; i0 < tiles; i0 += 32) {
                 int64_t u = 0;
@@ -283,9 +307,22 @@ __device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, const
                                            Share &sh, int cta, Piece &p) {
     Cursor &c = sh.c;
     while (c.left > 0) {
+        if (c.done) {
+            c.done = false;
+            c.off = 0;
+            if (++c.t == tl.tiles(c.s.n)) {
+                c.t = 0;
+                if (++c.h == n_kv) {
+                    c.h = 0;
+                    do {
+                        c.s = seq_view(pb, ++c.b);
+                    } while (c.s.n == 0);
+                }
+            }
+        }
         p.s = c.s;
         p.h = c.h;
-        const int tiles = (c.s.n + tl.TT - 1) / tl.TT;
+        const int tiles = tl.tiles(c.s.n);
         p.t0 = tile_at(c.t, tiles) * tl.TT;
         p.t1 = min(p.t0 + tl.TT, c.s.n);
         const KeyRange r = key_range<BK>(c.s, p.t0, p.t1, tl.window);
@@ -299,8 +336,9 @@ __device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, const
             const int w = tl.weight(p.t0, p.t1);
             end = r.nb * w;
             off = (int)min((int64_t)end, c.off + c.left);
-            p.k0 = (c.off + w - 1) / w;
-            p.k1 = (off + w - 1) / w;
+            auto blocks = [&](int units) { return w == 4 ? (units + 3) / 4 : (units + 2) / 3; };
+            p.k0 = blocks(c.off);
+            p.k1 = blocks(off);
             if (p.k0 == 0 && p.k1 < r.nb)
                 p.parts = share_owner(sh.total, sh.n, c.at - c.off + end - w) - cta + 1;
         }
@@ -308,18 +346,7 @@ __device__ __forceinline__ bool next_piece(const PagedBatch &pb, int n_kv, const
         c.left -= took;
         c.at += took;
         c.off = off;
-        if (off == end) {
-            c.off = 0;
-            if (c.left > 0 && ++c.t == tiles) {
-                c.t = 0;
-                if (++c.h == n_kv) {
-                    c.h = 0;
-                    do {
-                        c.s = seq_view(pb, ++c.b);
-                    } while (c.s.n == 0);
-                }
-            }
-        }
+        c.done = off == end;
         if (p.k0 < p.k1) return true;
     }
     return false;
@@ -349,7 +376,6 @@ struct PagedAttnArgs {
     int64_t q_ld, out_ld;
     int n_heads, n_kv, window;
     int box, box_cols;   // keys and columns of 64 dims per TMA box
-    int least;           // fewest units of a CTA's share
     bool whole;          // tiles are not cut
     float scale;
     SplitNote *notes;    // [CTAs]
