@@ -178,6 +178,9 @@ class PagedLlama:
         meta = self._ids(list(seqs) + new_lens + starts + [e - 1 for e in starts[1:]])
         ids, lens, q_starts, rows = meta.split([n, n, n + 1, n])
         paged.pages_reserve(self.pool, self.refs, self.table, self.lens, ids, lens)
+        # (refused: the sequences have their old lengths, and the new tokens would be
+        # written over their last ones; they are padding then)
+        ids = torch.where(self.lens.index_select(0, ids) == lens, ids, -1)
         d, pool, table = self.decoder, self.pool, self.table
         cache = paged.Cache(pool.data_ptr(), pool[0, 1].data_ptr(), pool.shape[2], pool.stride(2),
                             *pool.shape[3:], 1)

@@ -152,6 +152,30 @@ def test_serving_refusals(nqlib, model):
     assert nb.take_device_error() == 0 and srv.lengths() == [0, 40, 16]
 
 
+def test_a_refused_step_leaves_the_cache(nqlib, model):
+    """A step without enough free pages writes no key: all pages, those that sequences
+    share among them, hold what they held, and the sequences go on as if it had not been."""
+    dec = LlamaDecoder(cfg(), model[1])
+    srv = PagedLlama(dec, n_pages=5, page_size=16, max_seqs=3, max_len=200)
+    srv.pool.zero_()
+    toks = torch.randint(0, SMALL["vocab"], (40,), dtype=torch.int32, device="cuda")
+    srv.step([0], toks, [40])
+    srv.fork(0, [1])
+    before = srv.pool.clone()
+    srv.step([0, 1], torch.cat([toks, toks]), [40, 40])  # 3 + 3 pages of 2 free ones
+    assert nb.take_device_error() & 4
+    assert srv.lengths() == [40, 40, 0]
+    assert torch.equal(srv.pool, before)
+    a, _ = srv.step([0, 1], toks[:2].contiguous(), [1, 1])
+    ref = LlamaDecoder(cfg(), model[1])
+    ref.set_prefill_chunk(64)
+    for i in range(2):
+        ref.reset()
+        ref.prefill(toks, logits=False)
+        close(a[i], ref.step(toks[i:i + 1])[0], f"sequence {i}")
+    assert nb.take_device_error() == 0
+
+
 def test_forward_refusals(nqlib, model):
     _, dev = model
     dec = LlamaDecoder(cfg(), dev)
