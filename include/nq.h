@@ -318,8 +318,9 @@ int nq_llama_reset(nq_llama_t dec, void *stream);
 int nq_llama_step(nq_llama_t dec, const int32_t *token, float *logits,
                   int32_t *next_token, void *stream);
 /* n steps over the prompt tokens[0..n) (device), or steps of a chunk each
- * after nq_llama_set_prefill_chunk; logits (optional) gets the last position's.  Afterwards the decoder's next input is the argmax of the
- * last position (the first generated token). */
+ * after nq_llama_set_prefill_chunk; logits (optional) gets the last position's.
+ * Afterwards the decoder's next input is the argmax of the last position (the
+ * first generated token). */
 int nq_llama_prefill(nq_llama_t dec, const int32_t *tokens, int64_t n,
                      float *logits, void *stream);
 /* n greedy steps, each fed the previous step's argmax (the first one token[0]
@@ -431,7 +432,9 @@ int nq_pages_fork(const nq_page_table_t *table, const int32_t *parents, const in
  * and has other holders is replaced by a copy, and free pages are added, the
  * lowest first, in the list's order.  All or nothing: too few free pages, a
  * length below the present one or past the table, a row out of range or a
- * sequence listed twice refuse the whole call.  n * table_width < 2^31.
+ * sequence listed twice refuse the whole call, and lens stays as it was: an
+ * append that follows has to leave these sequences out (as padding), or it writes
+ * over their last tokens.  n * table_width < 2^31.
  * workspace: nq_pages_workspace_size(0, n) bytes, 256-byte aligned. */
 size_t nq_pages_workspace_size(int64_t n_pages, int64_t n);
 int nq_pages_reserve(const nq_page_table_t *table, const nq_page_pool_t *pool, const int32_t *seqs,

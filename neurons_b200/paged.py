@@ -117,7 +117,8 @@ def pages_workspace_size(n_pages, n):
 
 def pages_reserve(pool, refs, table, lens, seqs, new_lens, workspace=None):
     """The sequences grow to new_lens tokens: shared last pages that are not full are
-    copied, free pages added.  All or nothing (see include/nq.h)."""
+    copied, free pages added.  All or nothing; after a refusal lens is as it was, and an
+    append of the new tokens must leave these sequences out (see include/nq.h)."""
     (_module or _native()).reserve(pool, refs, table, lens, seqs, new_lens, workspace)
 
 
