@@ -567,8 +567,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                             x[e] = fmaxf(x[e], fmaxf(s[j + e], s[j + 4 + e]));
                 }
                 const float mn = fmaxf(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-                // (m == -inf: the difference is +inf, or NaN when the row has no key yet)
-                if (__any_sync(0xffffffffu, (mn - m) * cs > 8.f)) {
+                // (m == -inf: the difference is +inf, or NaN when the row has no key yet; rows
+                // behind the tile's own, which the last tile may have left in shared memory,
+                // have no say, or the rounding of this warp's other rows would follow them)
+                if (__any_sync(0xffffffffu, r < valid && (mn - m) * cs > 8.f)) {
                     const float f = m == -INFINITY ? 0.f : ex2((m - mn) * cs);
                     if (i > 0) {
                         // O still takes the last step's product: wait for it

@@ -272,6 +272,21 @@ def test_attention_is_deterministic():
 
 # ------------------------------------------------------------------- append
 
+@pytest.mark.parametrize("group", [33, 7, 65])
+def test_rows_that_fill_no_tile_do_not_see_what_ran_before(group):
+    """128 / group tokens leave rows of a tile of 128 unused; another call's queries in their
+    place must not change a bit of the result."""
+    b = Batch([500], [500], group, 1, 128, 256, HF, seed=12)
+    want = b.call(nb, max_q=500).clone()
+    check_attention(want, b)
+    other = Batch([600], [600], 128, 1, 128, 16, HF, seed=13)
+    q = other.q.clone()
+    for factor in (0.0, 5.0, 40.0, 400.0):
+        other.q.copy_(q * factor)
+        other.call(nb, max_q=600)
+        assert torch.equal(b.call(nb, max_q=500), want)
+
+
 def rotate64(x, pos, freqs):
     f = freqs.numel()
     a = pos.double()[:, None] * freqs.double()
