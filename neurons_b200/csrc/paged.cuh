@@ -134,10 +134,10 @@ __device__ __forceinline__ int tile_units(const SeqView &s, const Tiling &tl, in
 // The list: entries in order, in each its key heads, in each the token tiles in
 // tile_at()'s order, in each its key blocks.  Neighbouring CTAs therefore read
 // the same head's keys at the same time.  CTA c of n takes the units
-// [c * total / n, (c + 1) * total / n) (a block goes with its first unit), so that all CTAs get the same work whatever the lengths are; a
-// tile cut by such a border is finished by a merge kernel.  Where no sequence
-// can be long (`whole`) a tile counts as one and is never cut: no parts, and no
-// merge.
+// [c * total / n, (c + 1) * total / n) (a block goes with its first unit), so
+// that all CTAs get the same work whatever the lengths are; a tile cut by such a
+// border is finished by a merge kernel.  Where no sequence can be long (`whole`)
+// a tile counts as one and is never cut: no parts, and no merge.
 template <int BK>
 __device__ __forceinline__ int64_t entry_units_warp(const SeqView &s, const Tiling &tl) {
     // units of one head of this lane's entry; the lanes sum long entries together
