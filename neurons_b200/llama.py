@@ -136,7 +136,9 @@ class LlamaDecoder:
 class PagedLlama:
     """Continuous batching over a LlamaDecoder's weights: sequences 0 .. max_seqs - 1 of up
     to max_len tokens in a pool of n_pages pages.  The page table, lengths and
-    reference counts live on the device; the host keeps the lengths beside them."""
+    reference counts live on the device, where a step takes the lengths from.  A refused
+    step leaves the host's own lengths too large until lengths() is called, which a call
+    that they would refuse does first."""
 
     def __init__(self, decoder, n_pages, page_size=64, max_seqs=64, max_len=4096):
         c = decoder.cfg
@@ -158,26 +160,37 @@ class PagedLlama:
         if any(s < 0 or s >= len(self.host_lens) for s in seqs) or len(set(seqs)) < len(seqs):
             raise NQError(1, f"sequences must be different numbers below {len(self.host_lens)}")
 
+    def _holds(self, test):
+        """test() by the host's lengths, or else by the device's."""
+        if test():
+            return True
+        self.lengths()
+        return test()
+
     def step(self, seqs, tokens, news, logits=True):
         """news[i] new tokens of sequence seqs[i], one sequence after another in `tokens`
         (int32 CUDA tensor).  Returns the last positions' logits (fp32 [n, vocab], or None)
         and argmax (int32 [n]).  Too few free pages leave the sequences as they were and
-        raise bit 2 of take_device_error(); the step's outputs mean nothing then, and
-        lengths() tells the sequences' lengths."""
+        raise bit 2 of take_device_error(); the step's outputs mean nothing then, the next
+        step goes on behind the tokens that were accepted, and lengths() tells the
+        sequences' lengths."""
         self._check(seqs)
         n, total = len(seqs), sum(news)
         if len(news) != n or n == 0 or min(news) < 1 or tokens.dtype != torch.int32 or \
                 not tokens.is_cuda or not tokens.is_contiguous() or tokens.numel() != total:
             raise NQError(1, "step: tokens must be int32 CUDA, news[i] >= 1 of them for each sequence")
-        new_lens = [self.host_lens[s] + m for s, m in zip(seqs, news)]
-        if max(new_lens) > self.max_len:
+        if not self._holds(lambda: all(self.host_lens[s] + m <= self.max_len
+                                       for s, m in zip(seqs, news))):
             raise NQError(1, f"step: a sequence would pass max_len {self.max_len}")
         starts = [0]
         for m in news:
             starts.append(starts[-1] + m)
-        meta = self._ids(list(seqs) + new_lens + starts + [e - 1 for e in starts[1:]])
-        ids, lens, q_starts, rows = meta.split([n, n, n + 1, n])
+        meta = self._ids(list(seqs) + list(news) + starts + [e - 1 for e in starts[1:]])
+        ids, more, q_starts, rows = meta.split([n, n, n + 1, n])
+        lens = self.lens.index_select(0, ids) + more
         paged.pages_reserve(self.pool, self.refs, self.table, self.lens, ids, lens)
+        for s, m in zip(seqs, news):
+            self.host_lens[s] += m
         # (refused: the sequences have their old lengths, and the new tokens would be
         # written over their last ones; they are padding then)
         ids = torch.where(self.lens.index_select(0, ids) == lens, ids, -1)
@@ -197,14 +210,12 @@ class PagedLlama:
                                  pool.stride(0), ctypes.byref(batch), most, rows.data_ptr(), n,
                                  lg.data_ptr() if logits else None, nxt.data_ptr(), ws.data_ptr(),
                                  need, ops._stream()))
-        for s, m in zip(seqs, new_lens):
-            self.host_lens[s] = m
         return lg, nxt
 
     def fork(self, parent, children):
         """children (empty so far) continue from parent's tokens, sharing its pages."""
         self._check([parent] + list(children))
-        if any(self.host_lens[c] for c in children):
+        if not self._holds(lambda: not any(self.host_lens[c] for c in children)):
             raise NQError(1, "fork: a child has tokens")
         paged.pages_fork(self.refs, self.table, self.lens, self._ids([parent] * len(children)),
                          self._ids(list(children)))
@@ -222,6 +233,6 @@ class PagedLlama:
         paged.pages_compact(self.pool, self.refs, self.table)
 
     def lengths(self):
-        """The lengths as the device has them (waits for it); the host's copy follows."""
+        """The lengths as the device has them (waits for it); the host's follow."""
         self.host_lens = self.lens.tolist()
         return list(self.host_lens)

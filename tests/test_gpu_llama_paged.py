@@ -198,3 +198,56 @@ def test_forward_refusals(nqlib, model):
                dict(cache=Cache(z, z, 2, 4096, 2, 16, 64, 1))):
         assert call(**kw) == 1, kw
     assert call(batch=Batch(z, 1, 1, 1, z, None, None, 0, 0)) == 0
+
+
+def serve_beside(srv, model, toks):
+    """A step of sequence 0 with the token behind toks, held against a decoder that was given
+    the same tokens alone."""
+    lg, _ = srv.step([0], toks[-1:].contiguous(), [1])
+    ref = LlamaDecoder(cfg(), model[1])
+    ref.set_prefill_chunk(64)
+    close(lg[0], ref.prefill(toks.contiguous()), "the step behind a refused one")
+    ref.close()
+
+
+def test_steps_go_on_behind_a_refused_one(nqlib, model):
+    """Nobody asks for the lengths between a refused step and the next one: its tokens still
+    stand right behind the last ones that were accepted, in the sequence and in its forks."""
+    dec = LlamaDecoder(cfg(), model[1])
+    srv = PagedLlama(dec, n_pages=4, page_size=16, max_seqs=4, max_len=64)
+    srv.pool.fill_(float("nan"))
+    toks = torch.randint(0, SMALL["vocab"], (24,), dtype=torch.int32, device="cuda")
+    srv.step([0, 1], torch.cat([toks[:20], toks[:20]]), [20, 20])       # all four pages
+    srv.step([0, 2], torch.zeros(18, dtype=torch.int32, device="cuda"), [1, 17])  # refused
+    serve_beside(srv, model, toks[:21])
+    srv.free([1])
+    serve_beside(srv, model, toks[:22])
+    srv.step([0, 1], torch.zeros(50, dtype=torch.int32, device="cuda"), [40, 10])  # refused
+    srv.fork(0, [2])  # (which the step above left empty, whatever the host thought of it)
+    assert nb.take_device_error() == 4
+    lg, _ = srv.step([2], toks[22:23].contiguous(), [1])
+    serve_beside(srv, model, toks[:23])
+    ref = LlamaDecoder(cfg(), model[1])
+    ref.set_prefill_chunk(64)
+    close(lg[0], ref.prefill(toks[:23].contiguous()), "a fork behind a refused step")
+    assert srv.lengths() == [23, 0, 23, 0]
+    assert nb.take_device_error() == 0
+
+
+def test_a_refused_step_does_not_use_up_max_len(nqlib, model):
+    """Tokens that were refused count neither against max_len nor as a child's."""
+    dec = LlamaDecoder(cfg(), model[1])
+    srv = PagedLlama(dec, n_pages=3, page_size=16, max_seqs=3, max_len=64)
+    t = lambda n: torch.zeros(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    srv.step([0], t(30), [30])
+    srv.step([0, 1], t(64), [30, 34])  # 2 + 3 pages of the one that is left
+    assert nb.take_device_error() == 4
+    srv.step([0], t(10), [10])
+    srv.step([0], t(8), [8])
+    srv.fork(0, [1])
+    assert srv.lengths() == [48, 48, 0]
+    with pytest.raises(nb.NQError):
+        srv.step([0], t(17), [17])
+    with pytest.raises(nb.NQError):
+        srv.fork(0, [1])
+    assert nb.take_device_error() == 0
