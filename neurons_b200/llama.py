@@ -182,23 +182,9 @@ class PagedLlama:
         if not self._holds(lambda: all(self.host_lens[s] + m <= self.max_len
                                        for s, m in zip(seqs, news))):
             raise NQError(1, f"step: a sequence would pass max_len {self.max_len}")
-        starts = [0]
-        for m in news:
-            starts.append(starts[-1] + m)
-        meta = self._ids(list(seqs) + list(news) + starts + [e - 1 for e in starts[1:]])
-        ids, more, q_starts, rows = meta.split([n, n, n + 1, n])
-        lens = self.lens.index_select(0, ids) + more
-        paged.pages_reserve(self.pool, self.refs, self.table, self.lens, ids, lens)
-        for s, m in zip(seqs, news):
-            self.host_lens[s] += m
-        # (refused: the sequences have their old lengths, and the new tokens would be
-        # written over their last ones; they are padding then)
-        ids = torch.where(self.lens.index_select(0, ids) == lens, ids, -1)
+        # Everything that can fail on the host comes before the reserve: a sequence that has
+        # grown and whose tokens are not appended would keep a hole.
         d, pool, table = self.decoder, self.pool, self.table
-        cache = paged.Cache(pool.data_ptr(), pool[0, 1].data_ptr(), pool.shape[2], pool.stride(2),
-                            *pool.shape[3:], 1)
-        batch = paged.Batch(table.data_ptr(), table.shape[1], table.shape[1], table.shape[0],
-                            self.lens.data_ptr(), ids.data_ptr(), q_starts.data_ptr(), n, total)
         lg = torch.empty((n, d.vocab), dtype=torch.float32, device="cuda") if logits else None
         nxt = torch.empty(n, dtype=torch.int32, device="cuda")
         most = max(news)
@@ -206,6 +192,22 @@ class PagedLlama:
         need = f.nq_llama_forward_workspace_size(d.handle, total, n, most,
                                                  table.shape[1] * pool.shape[-2])
         ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        starts = [0]
+        for m in news:
+            starts.append(starts[-1] + m)
+        meta = self._ids(list(seqs) + list(news) + starts + [e - 1 for e in starts[1:]])
+        ids, more, q_starts, rows = meta.split([n, n, n + 1, n])
+        lens = self.lens.index_select(0, ids) + more
+        paged.pages_reserve(pool, self.refs, table, self.lens, ids, lens)
+        for s, m in zip(seqs, news):
+            self.host_lens[s] += m
+        # (refused: the sequences have their old lengths, and the new tokens would be
+        # written over their last ones; they are padding then)
+        ids = torch.where(self.lens.index_select(0, ids) == lens, ids, -1)
+        cache = paged.Cache(pool.data_ptr(), pool[0, 1].data_ptr(), pool.shape[2], pool.stride(2),
+                            *pool.shape[3:], 1)
+        batch = paged.Batch(table.data_ptr(), table.shape[1], table.shape[1], table.shape[0],
+                            self.lens.data_ptr(), ids.data_ptr(), q_starts.data_ptr(), n, total)
         check(f.nq_llama_forward(d.handle, tokens.data_ptr(), ctypes.byref(cache),
                                  pool.stride(0), ctypes.byref(batch), most, rows.data_ptr(), n,
                                  lg.data_ptr() if logits else None, nxt.data_ptr(), ws.data_ptr(),

@@ -251,3 +251,17 @@ def test_a_refused_step_does_not_use_up_max_len(nqlib, model):
     with pytest.raises(nb.NQError):
         srv.fork(0, [1])
     assert nb.take_device_error() == 0
+
+
+def test_a_step_that_cannot_be_made_reserves_nothing(nqlib, model):
+    """Outputs that do not fit the GPU's memory: the sequences stay as they were."""
+    dec = LlamaDecoder(cfg(), model[1])
+    srv = PagedLlama(dec, n_pages=8, page_size=16, max_seqs=2, max_len=64)
+    toks = torch.randint(0, SMALL["vocab"], (12,), dtype=torch.int32, device="cuda")
+    srv.step([0], toks[:10].contiguous(), [10])
+    vocab, dec.vocab = dec.vocab, 1 << 50
+    with pytest.raises(RuntimeError):
+        srv.step([0], toks[:1].contiguous(), [1])
+    dec.vocab = vocab
+    assert srv.lens.tolist() == srv.host_lens == [10, 0]
+    serve_beside(srv, model, toks[:11])
