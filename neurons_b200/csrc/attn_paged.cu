@@ -479,8 +479,8 @@ __global__ void __launch_bounds__(128) paged_merge_rows_kernel(const PagedAttnAr
     pdl_wait();
     __shared__ float sums[4][HD + 2];
     const SplitNote note = a.notes[blockIdx.x];
-    if (note.parts == 0) return;
     const int G = a.n_heads / a.n_kv;
+    if (!note_fits(note, blockIdx.x, gridDim.x, a.pb.n_tokens, a.n_heads, G)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r = blockIdx.y;
     if (r >= note.tokens * G) return;
@@ -549,8 +549,8 @@ __global__ void __launch_bounds__(128) paged_merge_tiles_kernel(const PagedAttnA
     pdl_launch_dependents();
     pdl_wait();
     const SplitNote note = a.notes[blockIdx.x];
-    if (note.parts == 0) return;
     const int G = a.n_heads / a.n_kv;
+    if (!note_fits(note, blockIdx.x, gridDim.x, a.pb.n_tokens, a.n_heads, G)) return;
     const int r = blockIdx.z * 128 + threadIdx.x, d0 = blockIdx.y * 8;
     if (r >= note.tokens * G) return;
     float M = -INFINITY, L = 0.f, acc[8];

@@ -334,7 +334,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         Share sh = find_share<kBlock>(a.pb, a.n_kv, tl, blockIdx.x, gridDim.x);
         Piece p;
         int filled = 0, jobs_out = 0;
-        bool ok = true, note_left = false;
+        bool ok = true;
+        // no tile of this CTA's is cut, until a softmax thread says so (which it does
+        // behind a job, and not where it has given up: the merge always finds a note)
+        if (lane == 0 && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
         auto hand_out = [&](int n) {
             const int slot = jobs_out & 1;
             ok = mbar_wait_or_abort(&job_empty[slot], (uint32_t)(jobs_out / 2 + 1) & 1u, abort,
@@ -347,12 +350,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
             ++jobs_out;
         };
         while (ok && next_piece<kBlock>(a.pb, a.n_kv, tl, sh, blockIdx.x, p)) {
-            note_left |= p.parts > 0;
             hand_out(p.k1 - p.k0);
             ok = ok && load(p, &mk, ring_k, full_k, empty_k, filled);
         }
         if (ok) hand_out(0);
-        if (lane == 0 && !note_left && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
     } else if (warp == T::kValueWarp) {
         int filled = 0;
         for (int pieces = 0;; ++pieces) {
@@ -735,7 +736,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                     *reinterpret_cast<float2 *>(a.part_ml + ((int64_t)slot * T::kRows + row) * 2) =
                         make_float2(M * cs, L);
             }
-            if (threadIdx.x == 0 && job.p.parts > 0)
+            if (threadIdx.x == 0 && ok && job.p.parts > 0)
                 a.notes[blockIdx.x] = SplitNote{p.s.q0 + p.t0, p.h * G, p.t1 - p.t0, p.parts};
             // (the next piece's first product into O waits for this warpgroup's weights,
             // and the barrier above for both warpgroups)

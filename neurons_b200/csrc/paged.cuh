@@ -368,6 +368,16 @@ struct SplitNote {
     int q_row, heads0, tokens, parts;
 };
 
+// Whether the merge may follow CTA `cta`'s note: its parts and rows lie within
+// the call.  A call's own notes do; those that an overlapping call left in a
+// workspace used twice need not, and they say where the merge reads and writes.
+__host__ __device__ __forceinline__ bool note_fits(const SplitNote &n, int cta, int ctas, int n_tokens,
+                                                   int n_heads, int group) {
+    return n.parts > 0 && n.parts <= ctas - cta && n.q_row >= 0 && n.tokens > 0 &&
+           n.tokens <= n_tokens && n.q_row <= n_tokens - n.tokens && n.heads0 >= 0 &&
+           n.heads0 <= n_heads - group;
+}
+
 // An attention call as its kernels take it.
 struct PagedAttnArgs {
     PagedBatch pb;

@@ -606,3 +606,23 @@ def test_serving_run(dtype, dim, heads, kv, page):
     used = int((refs > 0).sum())
     assert (refs[:used] > 0).all() or used <= n_pages
     assert nb.take_device_error() == 0
+
+
+# ------------------------------------------------------------- workspaces
+
+@pytest.mark.parametrize("byte", [0, 1, 0x7f, 0xff])
+@pytest.mark.parametrize("lens,news", [([3000, 40], [1, 1]), ([1500, 700], [1, 90]),
+                                       ([1400], [1400])])
+def test_what_a_workspace_holds_does_not_matter(lens, news, byte):
+    """Cut tiles, and CTAs without a tile of their own, beside any bytes."""
+    b = Batch(lens, news, 8, 2, 128, 16, BF, seed=31)
+    want = b.call(nb, max_q=max(news)).clone()
+    size = nb.paged_attention_workspace_size(8, 2, 128, max(news), b.table.shape[1] * 16)
+    assert size > 0
+    ws = torch.full((size,), byte, dtype=torch.uint8, device="cuda")
+    out = torch.full((b.tokens + 1, 8, 128), 3.0, dtype=BF, device="cuda")
+    b.q = torch.cat([b.q, b.q[:1]])
+    got = b.call(nb, max_q=max(news), workspace=ws, out=out)
+    assert torch.equal(got[:b.tokens], want)
+    assert (got[b.tokens:] == 3).all()
+    assert nb.take_device_error() == 0

@@ -1,6 +1,8 @@
 """Refusals of the paged cache's C entry points: bad arguments return InvalidInput with a
 message before a device is touched."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 
@@ -176,3 +178,14 @@ def test_llama_paged_entry_points_refuse_null(nqlib):
     assert nqlib.nq_llama_forward(None, A, ctypes.byref(c), 0, ctypes.byref(b), 1, A, 1, A, A, A,
                                   1 << 30, None) == 1
     assert nqlib.nq_last_error()
+
+
+def test_notes_of_cut_tiles_are_followed_only_within_the_call(nqlib, tmp_path):
+    """What the merge reads from a workspace says where it reads and writes."""
+    from neurons_b200 import build
+    exe = str(tmp_path / "split_check")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "split_check.cu")
+    subprocess.run([build.NVCC] + build.ARCH + ["-std=c++17", "-O1", "-I" + build.CSRC,
+                                                "-I" + build.INCLUDE, src, "-o", exe], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
