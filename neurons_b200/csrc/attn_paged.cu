@@ -181,28 +181,28 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
     int it = 0;  // blocks so far: stage it % kStages, parity it / kStages
 
     if (warp == kWarps) {
-        while (next_piece<kBlock>(a.pb, a.n_kv, tl, sh, blockIdx.x, p)) {
+        bool ok = true;
+        while (ok && next_piece<kBlock>(a.pb, a.n_kv, tl, sh, blockIdx.x, p)) {
             const int p0 = p.s.len - p.s.n + p.t0, key_hi = p.s.len - p.s.n + p.t1;
             const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
             for (int k = p.k0; k < p.k1; ++k, ++it) {
                 const int st = it % C::kStages;
-                if (!mbar_wait_or_abort(&empty[st], (uint32_t)(it / C::kStages + 1) & 1u, abort,
-                                        a.pb.err)) {
-                    // given up: the copies in flight end before this CTA does
-                    for (int j = max(0, it - C::kStages); j < it; ++j) {
-                        const unsigned long long t0 = global_timer_ns();
-                        while (!mbar_try_wait(&full[j % C::kStages],
-                                              (uint32_t)(j / C::kStages) & 1u) &&
-                               global_timer_ns() - t0 < kWaitLimitNs) {
-                        }
-                    }
-                    return;
-                }
+                ok = mbar_wait_or_abort(&empty[st], (uint32_t)(it / C::kStages + 1) & 1u, abort,
+                                        a.pb.err);
+                if (!ok) break;
                 load_block<HD>(a.pb, &mk, &mv, p, p.lo + k, a.box, key_lo, key_hi,
                                smem + st * C::kStageBytes, &full[st]);
             }
         }
-        return;  // (the consumers wait for every load)
+        // The copies in flight end before this CTA does, also those that a consumer has
+        // given up waiting for (behind each stage's last load its barrier stays as it is).
+        for (int j = max(0, it - C::kStages); j < it; ++j) {
+            const unsigned long long t0 = global_timer_ns();
+            while (!mbar_try_wait(&full[j % C::kStages], (uint32_t)(j / C::kStages) & 1u) &&
+                   global_timer_ns() - t0 < kWaitLimitNs) {
+            }
+        }
+        return;
     }
 
     const float cs = a.scale * 1.4426950408889634f;  // exp(scale x) = 2^(cs x)
