@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
             const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
             for (int k = p.k0; k < p.k1; ++k, ++it) {
                 const int st = it % C::kStages;
-                ok = mbar_wait_or_abort(&empty[st], (uint32_t)(it / C::kStages + 1) & 1u, abort,
+                ok = warp_wait_or_abort(&empty[st], (uint32_t)(it / C::kStages + 1) & 1u, abort,
                                         a.pb.err);
                 if (!ok) break;
                 load_block<HD>(a.pb, &mk, &mv, p, p.lo + k, a.box, key_lo, key_hi,
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
             const int st = it % C::kStages;
             const int key0 = (p.lo + k) * kBlock + warp * 16;  // this warp's keys
             // (given up: the warp still takes part in the barriers below)
-            if (!mbar_wait_or_abort(&full[st], (uint32_t)(it / C::kStages) & 1u, abort, a.pb.err))
+            if (!warp_wait_or_abort(&full[st], (uint32_t)(it / C::kStages) & 1u, abort, a.pb.err))
                 break;
             if (key0 < key_hi && key0 + 16 > key_lo) {
                 uint8_t *ks = smem + st * C::kStageBytes + key_at;

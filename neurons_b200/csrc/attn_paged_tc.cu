@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
 #pragma unroll
             for (int u = 0; u < T::kUnits; ++u, ++g) {
                 const int st = g % T::kStages;
-                if (!mbar_wait_or_abort(&empty[st], (uint32_t)(g / T::kStages + 1) & 1u, abort,
+                if (!warp_wait_or_abort(&empty[st], (uint32_t)(g / T::kStages + 1) & 1u, abort,
                                         a.pb.err))
                     return false;
                 if (lane == 0) mbar_expect_tx(&full[st], T::kUnitBytes);
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         if (lane == 0 && !a.whole) a.notes[blockIdx.x] = SplitNote{0, 0, 0, 0};
         auto hand_out = [&](int n) {
             const int slot = jobs_out & 1;
-            ok = mbar_wait_or_abort(&job_empty[slot], (uint32_t)(jobs_out / 2 + 1) & 1u, abort,
+            ok = warp_wait_or_abort(&job_empty[slot], (uint32_t)(jobs_out / 2 + 1) & 1u, abort,
                                     a.pb.err);
             if (ok && lane == 0) {
                 jobs[slot].p = p;
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
         int filled = 0;
         for (int pieces = 0;; ++pieces) {
             const int slot = pieces & 1;
-            if (!mbar_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort, a.pb.err) ||
+            if (!warp_wait_or_abort(&job_full[slot], (uint32_t)(pieces / 2) & 1u, abort, a.pb.err) ||
                 jobs[slot].n == 0)
                 break;
             const Piece p = jobs[slot].p;

@@ -378,6 +378,14 @@ __host__ __device__ __forceinline__ bool note_fits(const SplitNote &n, int cta, 
            n.heads0 <= n_heads - group;
 }
 
+// mbar_wait_or_abort() by a whole warp, which goes on or gives up as one: where its
+// lanes could part, those that go on would wait in the next warp-wide step for
+// those that have left.
+__device__ __forceinline__ bool warp_wait_or_abort(uint64_t *bar, uint32_t parity,
+                                                   volatile int *abort, unsigned *err) {
+    return __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity, abort, err)) != 0;
+}
+
 // An attention call as its kernels take it.
 struct PagedAttnArgs {
     PagedBatch pb;
