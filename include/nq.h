@@ -370,7 +370,8 @@ typedef struct nq_paged_batch {
  * [n_heads][head_dim], q_ld / out_ld elements apart (multiples of 8, 16-byte
  * aligned).  Keys and values past a sequence's length, and pages that no new
  * token's window reaches, may hold anything; the values that the rows of one
- * call see have to be finite.  max_q: no entry has more new tokens than this (it
+ * call see have to be finite.  A NaN in a query, or in a key that it sees, makes
+ * its row NaN.  max_q: no entry has more new tokens than this (it
  * selects the kernel and the workspace's size, results hold for any; 0:
  * unknown, with the workspace that any would need).  Softmax and sums in fp32;
  * the weights are rounded to the cache's type for the second product, the result

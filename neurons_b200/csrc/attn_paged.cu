@@ -420,7 +420,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                 const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    L += wm[w][r] == -INFINITY ? 0.f : wl[w][r] * ex2((wm[w][r] - M) * cs);
+                    // (by the sum: a warp whose scores are all NaN has no maximum either)
+                    L += wl[w][r] == 0.f ? 0.f : wl[w][r] * ex2((wm[w][r] - M) * cs);
                     const float *src = red + (w * 8 + rr) * HD + (d0 ^ (rr >> 1) * 8);
                     const float4 u = *reinterpret_cast<const float4 *>(src);
                     const float4 v = *reinterpret_cast<const float4 *>(src + 4);

@@ -626,3 +626,34 @@ def test_what_a_workspace_holds_does_not_matter(lens, news, byte):
     assert torch.equal(got[:b.tokens], want)
     assert (got[b.tokens:] == 3).all()
     assert nb.take_device_error() == 0
+
+
+# -------------------------------------------------------------------- NaN
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("lens,news", [([200, 40], [1, 1]), ([6000, 40], [1, 1]), ([900, 700], [3, 1]),
+                                       ([2000, 700], [150, 1])])
+def test_nan_reaches_its_row_alone(lens, news, dtype):
+    """A NaN in a query makes that head's row NaN, however the keys are split over the CTAs, and
+    one in a key the rows that see it; the other rows stay right."""
+    b = Batch(lens, news, 8, 2, 128, 16, dtype, seed=41)
+    want, bound = attention64(b)
+    right = lambda x, rows: ((x.double() - want).abs() <= bound + 1e-12)[rows].all()  # noqa: E731
+    q = b.q.clone()
+    b.q = q.clone()
+    b.q[0, 5, 17] = float("nan")
+    got = b.call(nb, max_q=max(news))
+    assert torch.isnan(got[0, 5]).all()
+    other = torch.ones(got.shape[:2], dtype=torch.bool, device="cuda")
+    other[0, 5] = False
+    assert right(got, other)
+    # a key of the first sequence's second head that all of its new tokens see
+    b.q = q
+    at = lens[0] - news[0] - 3
+    b.k[int(b.table[b.rows[0], at // 16]), 1, at % 16, 9] = float("nan")
+    got = b.call(nb, max_q=max(news))
+    assert torch.isnan(got[:news[0], 4:]).all()
+    other[:] = True
+    other[:news[0], 4:] = False
+    assert right(got, other)
+    assert nb.take_device_error() == 0
