@@ -459,8 +459,12 @@ int nq_pages_copy(const nq_page_pool_t *pool, const int32_t *src, const int32_t 
  * Prompts in chunks: nq_llama_prefill passes up to `chunk` tokens through the
  * layers at a time (M-row quantized matmuls, nq_paged_attention over the
  * decoder's cache) instead of one (0, the default).  The results differ from the
- * one-token steps' by the order of the sums.  Allocates the chunk's workspace;
- * not to be called while calls on the decoder are under way. */
+ * one-token steps' by the order of the sums and the rounding of the angles, which
+ * chunks take in 64 bits; from the first call with chunk > 0 on, the decoder's
+ * one-token steps do so too (those captured in a graph before keep 32 bits), so
+ * that queries and keys of far positions agree.  It is therefore called before a
+ * sequence's first token.  Allocates the chunk's workspace; not to be called while
+ * calls on the decoder are under way. */
 int nq_llama_set_prefill_chunk(nq_llama_t dec, int64_t chunk);
 
 /* The batch's new tokens (tokens: device int32 [batch->n_tokens]) through the

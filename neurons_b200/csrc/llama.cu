@@ -102,13 +102,22 @@ __global__ void embed_kernel(const int32_t *tok_src, const uint32_t *ew, const u
 // RoPE (MLX fast::rope, traditional = false, scale 1): for i < d/2,
 // angle = pos * base^(-i/(d/2)); (x_i, x_{i+d/2}) rotated by it in fp32 and
 // rounded to bf16.  Returns the rotated value of element e of a head.
-__device__ __forceinline__ float rope_elem(const uint16_t *head, int e, int hd, float pos,
-                                           float log2_base) {
+// FREQS: by rope_turn() and the decoder's frequencies, as nq_paged_append turns
+// the keys of a chunk.
+template <bool FREQS>
+__device__ __forceinline__ float rope_elem(const uint16_t *head, int e, int hd, int pos,
+                                           float log2_base, const float *freqs) {
     const int half = hd / 2;
     const int i = e < half ? e : e - half;
-    const float inv_freq = exp2f(-((float)i / (float)half) * log2_base);
     float sn, cs;
-    sincosf(pos * inv_freq, &sn, &cs);
+    if constexpr (FREQS) {
+        const float2 t = rope_turn(pos, freqs[i]);
+        cs = t.x;
+        sn = t.y;
+    } else {
+        const float inv_freq = exp2f(-((float)i / (float)half) * log2_base);
+        sincosf((float)pos * inv_freq, &sn, &cs);
+    }
     const float x1 = bf16_to_f32(head[i]), x2 = bf16_to_f32(head[i + half]);
     const float r = e < half ? x1 * cs - x2 * sn : x1 * sn + x2 * cs;
     return bf16_to_f32(f32_to_bf16(r));
@@ -124,6 +133,7 @@ struct AttnArgs {
     unsigned *err;
     int n_heads, n_kv, hd, max_ctx, ctx_ld, splits;  // ctx_ld: positions a cache has room for
     float log2_base, scale;
+    const float *freqs;         // [hd / 2] radians per position; nullptr: from log2_base, in 32 bits
 };
 
 // kDpl consecutive bf16 values -> fp32 (one 4-, 8- or 16-byte load)
@@ -160,7 +170,7 @@ __device__ __forceinline__ void load_bf16(const uint16_t *p, float *out) {
 // warp and a warp's rows are all in flight together.  Each CTA writes its
 // softmax partials (max, sum, weighted values); the last CTA of a query head
 // (atomic count) merges the chunks in chunk order.  No CTA waits for another.
-template <int HD>
+template <int HD, bool FREQS>
 __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
     pdl_launch_dependents();
     pdl_wait();  // q, k, v come from the qkv projection
@@ -183,14 +193,13 @@ __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
     const int n_active = pos / kAttnChunk + 1;
     if (s >= n_active) return;
     const int t0 = s * kAttnChunk, t1 = min(t0 + kAttnChunk, pos + 1);
-    const float fpos = (float)pos;
     const uint16_t *qraw = a.qkv + (size_t)hq * HD;
     const uint16_t *kraw = a.qkv + (size_t)(a.n_heads + j) * HD;
     const uint16_t *vraw = a.qkv + (size_t)(a.n_heads + a.n_kv + j) * HD;
     const bool has_new = t1 == pos + 1;
     for (int d = tid; d < HD; d += kAttnThreads) {
-        qs[d] = rope_elem(qraw, d, HD, fpos, a.log2_base);
-        if (has_new) kn[d] = rope_elem(kraw, d, HD, fpos, a.log2_base);
+        qs[d] = rope_elem<FREQS>(qraw, d, HD, pos, a.log2_base, a.freqs);
+        if (has_new) kn[d] = rope_elem<FREQS>(kraw, d, HD, pos, a.log2_base, a.freqs);
     }
     uint16_t *kc = a.kc + (size_t)j * a.ctx_ld * HD;
     uint16_t *vc = a.vc + (size_t)j * a.ctx_ld * HD;
@@ -451,6 +460,7 @@ struct LlamaDecoder {
     float *freqs = nullptr;      // [hd / 2] radians per position
     int32_t *one_seq = nullptr;  // page table {0}, length, {0, tokens}, last row of a chunk
     int64_t chunk = 0;           // tokens per step of a prompt (0: one, by the decode step)
+    bool chunked = false;        // the cache may hold keys of chunks: steps take their angles
     void *chunk_ws = nullptr;
     size_t chunk_ws_bytes = 0;
     int splits = 1;
@@ -552,10 +562,11 @@ cudaError_t gemv(const LlamaDecoder &d, const uint16_t *x, int64_t x_ld, const u
 
 }  // namespace
 
+template <bool FREQS>
 cudaError_t launch_attention(int hd, dim3 grid, const AttnArgs &aa, cudaStream_t st) {
-    if (hd == 64) return launch_pdl_ll(attn_kernel<64>, grid, kAttnThreads, 0, st, aa);
-    if (hd == 128) return launch_pdl_ll(attn_kernel<128>, grid, kAttnThreads, 0, st, aa);
-    return launch_pdl_ll(attn_kernel<256>, grid, kAttnThreads, 0, st, aa);
+    if (hd == 64) return launch_pdl_ll(attn_kernel<64, FREQS>, grid, kAttnThreads, 0, st, aa);
+    if (hd == 128) return launch_pdl_ll(attn_kernel<128, FREQS>, grid, kAttnThreads, 0, st, aa);
+    return launch_pdl_ll(attn_kernel<256, FREQS>, grid, kAttnThreads, 0, st, aa);
 }
 
 // One decode step: tok_src holds the input token (device); the argmax goes to
@@ -587,6 +598,7 @@ cudaError_t llama_step(LlamaDecoder &d, const int32_t *tok_src, float *logits_f3
     aa.ctx_ld = d.ctx_ld;
     aa.splits = d.splits;
     aa.log2_base = log2f(c.rope_theta);
+    aa.freqs = d.chunked ? d.freqs : nullptr;
     aa.scale = 1.0f / sqrtf((float)c.head_dim);
     const size_t layer_cache = (size_t)c.n_kv_heads * d.ctx_ld * hd;
     for (int l = 0; l < c.n_layers; ++l) {
@@ -597,7 +609,8 @@ cudaError_t llama_step(LlamaDecoder &d, const int32_t *tok_src, float *logits_f3
         aa.kc = d.kc + (size_t)l * layer_cache;
         aa.vc = d.vc + (size_t)l * layer_cache;
         const dim3 agrid((unsigned)d.splits, (unsigned)c.n_heads);
-        e = launch_attention(c.head_dim, agrid, aa, st);
+        e = aa.freqs ? launch_attention<true>(c.head_dim, agrid, aa, st)
+                     : launch_attention<false>(c.head_dim, agrid, aa, st);
         if (e != cudaSuccess) return e;
         if ((e = gemv(d, d.attn, nq_, L.o_w, L.o_s, L.o_b, H, nq_, d.h, 0, nullptr, d.h, st)) !=
             cudaSuccess)
@@ -1172,6 +1185,7 @@ int nq_llama_set_prefill_chunk(nq_llama_t dec, int64_t chunk) {
         }
     }
     d.chunk = chunk;
+    d.chunked |= chunk > 0;
     return NQ_SUCCESS;
 }
 

@@ -186,6 +186,17 @@ __device__ __forceinline__ uint32_t pack_t2(float lo, float hi) {
     }
 }
 
+// (cosine, sine) of pos * freq: the angle in 64 bits (the product of a 24-bit
+// position and a 32-bit frequency is exact there; in 32 bits the angle of position
+// 100000 would be off by up to 0.004), reduced to a part of a turn before sine and
+// cosine are taken in 32.
+__device__ __forceinline__ float2 rope_turn(int pos, float freq) {
+    const double u = (double)pos * (double)freq * 0.15915494309189535;  // 1 / 2 pi
+    float sn, cs;
+    sincospif((float)(2.0 * (u - rint(u))), &sn, &cs);
+    return make_float2(cs, sn);
+}
+
 struct Dq4h {
     uint32_t s2, b2;  // (s,s), (b,b) as fp16x2
 };

@@ -50,10 +50,7 @@ constexpr int kAppendThreads = 128;
 
 // (x_i, x_{i + half}) turned by pos * freqs[i], for the first 2 * half dims of
 // each head of q and k; the rest, and v, as they are.  k and v go to their
-// page.  One CTA per token: its angles are computed once for all heads, in
-// 64 bits (pos * freq of a 24-bit position and a 32-bit frequency is exact
-// there; in 32 bits the angle of position 100000 would be off by up to 0.004)
-// and reduced to a part of a turn before sine and cosine are taken in 32.
+// page.  One CTA per token: its angles are computed once for all heads.
 // Memory bounds it: the first three vector pairs and one value vector of a thread
 // (all there are for 40 turned heads of 128 dims) are under way before the token's
 // entry, page and angles are looked up (12288 tokens 69 -> 49 us, 5.5 TB/s).
@@ -96,12 +93,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
     const int t = (int)i - s.q0;
     if (t < 0 || t >= s.n) return;  // behind the last sequence, or padding
     const int pos = s.len - s.n + t;
-    for (int f = tid; f < a.half; f += kAppendThreads) {
-        const double u = (double)pos * (double)a.freqs[f] * 0.15915494309189535;  // 1 / 2 pi
-        float sn, cs;
-        sincospif((float)(2.0 * (u - rint(u))), &sn, &cs);
-        turn[f] = make_float2(cs, sn);
-    }
+    for (int f = tid; f < a.half; f += kAppendThreads) turn[f] = rope_turn(pos, a.freqs[f]);
     int page = a.pb.n_pages;
     if (pos >= 0)
         page = page_of(a.pb, s.row, pos);

@@ -96,7 +96,8 @@ class LlamaDecoder:
         return int(lib().nq_llama_position(self.handle))
 
     def set_prefill_chunk(self, chunk):
-        """Prompts in chunks of up to `chunk` tokens (0: one position per step)."""
+        """Prompts in chunks of up to `chunk` tokens (0: one position per step).  Before a
+        sequence's first token: from here on steps take their angles in 64 bits, as chunks do."""
         check(lib().nq_llama_set_prefill_chunk(self.handle, int(chunk)))
 
     def reset(self):

@@ -265,3 +265,28 @@ def test_a_step_that_cannot_be_made_reserves_nothing(nqlib, model):
     dec.vocab = vocab
     assert srv.lens.tolist() == srv.host_lens == [10, 0]
     serve_beside(srv, model, toks[:11])
+
+
+def test_steps_behind_a_long_chunked_prompt(oracle, nqlib):
+    """A step turns its query by the same angles as the chunks turned their keys: at position
+    520000 angles in 32 bits are off by up to 0.03, and with scores of tens over as many keys a
+    step shows that."""
+    far = dict(SMALL, n_layers=1, max_context=520100, rope_theta=100.0)
+    _, dev = make_model(oracle, far, 23)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for n, rows in (("q", 1024), ("k", 256), ("o", 1024)):
+        w = torch.randn(rows, 1024, device="cuda", generator=g) * 0.1
+        dev["layers"][0][n] = nb.quantize(w, far["group_size"], far["bits"], nb.SCHEME_MLX_AFFINE)
+    n = 520000
+    toks = torch.randint(0, far["vocab"], (n + 3,), dtype=torch.int32, device="cuda", generator=g)
+    dec = LlamaDecoder(far, dev)
+    dec.set_prefill_chunk(8192)
+    want = []
+    for i in range(3):
+        dec.reset()
+        want.append(dec.prefill(toks[:n + 1 + i]))
+    dec.reset()
+    dec.prefill(toks[:n], logits=False)
+    for i in range(3):
+        close(dec.step(toks[n + i:n + i + 1])[0], want[i], f"step {i}")
+    assert nb.take_device_error() == 0
