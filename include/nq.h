@@ -375,9 +375,10 @@ typedef struct nq_paged_batch {
  * selects the kernel and the workspace's size, results hold for any; 0:
  * unknown, with the workspace that any would need).  Softmax and sums in fp32;
  * the weights are rounded to the cache's type for the second product, the result
- * once.  workspace: nq_paged_attention_workspace_size() bytes for this max_q and
- * max_keys = table_width * page_size (0: none is needed), 256-byte aligned,
- * contents irrelevant; two calls that overlap on the GPU need one each. */
+ * once.  workspace: nq_paged_attention_workspace_size() bytes for this max_q (or
+ * a larger one) and max_keys = table_width * page_size (0: none is needed),
+ * 256-byte aligned, contents irrelevant; two calls that overlap on the GPU need
+ * one each. */
 size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_dim, int64_t max_q,
                                          int64_t max_keys);
 int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_paged_cache_t *cache,

@@ -1172,10 +1172,7 @@ int nq_llama_set_prefill_chunk(nq_llama_t dec, int64_t chunk) {
     auto &d = dec->d;
     chunk = std::min<int64_t>(chunk, d.c.max_context);
     if (chunk > 0) {
-        // (a shorter chunk may take the attention kernel with the larger workspace)
-        size_t need = 0;
-        for (int64_t T : {chunk, (int64_t)1, std::min<int64_t>(chunk, 16)})
-            need = std::max(need, nq::forward_space(d, chunk, 1, T, d.ctx_ld, nullptr).total);
+        const size_t need = nq::forward_space(d, chunk, 1, chunk, d.ctx_ld, nullptr).total;
         if (need > d.chunk_ws_bytes) {
             void *p = nullptr;
             if (int rc = llama_cuda(cudaMalloc(&p, need), what)) return rc;

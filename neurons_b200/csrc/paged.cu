@@ -636,7 +636,11 @@ size_t nq_paged_attention_workspace_size(int n_heads, int n_kv_heads, int head_d
         n_heads / n_kv_heads > 128 || max_q < 0 || max_keys < 0 ||
         (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return 0;
-    return paged_attention_workspace(n_heads, n_kv_heads, head_dim, max_q, max_keys);
+    const size_t most = paged_attention_workspace(n_heads, n_kv_heads, head_dim, max_q, max_keys);
+    // (a call with fewer new tokens may take the kernel that needs more)
+    return max_q == 0 ? most
+                      : std::max(most, paged_attention_workspace(n_heads, n_kv_heads, head_dim, 1,
+                                                                 max_keys));
 }
 
 int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_paged_cache_t *cache,

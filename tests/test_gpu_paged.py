@@ -657,3 +657,29 @@ def test_nan_reaches_its_row_alone(lens, news, dtype):
     other[:news[0], 4:] = False
     assert right(got, other)
     assert nb.take_device_error() == 0
+
+
+@pytest.mark.parametrize("page,width", [(16, 40), (128, 9)])
+def test_a_step_in_the_workspace_of_a_chunk(page, width):
+    """The workspace of a larger max_q, through the C call without q_starts too."""
+    import ctypes
+    from neurons_b200 import paged
+    from neurons_b200._lib import lib
+    b = Batch([600, 90, 300], [1, 1, 1], 8, 2, 128, page, BF, seed=51)
+    table = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :b.table.shape[1]] = b.table[:, :width]
+    b.table = table
+    size = nb.paged_attention_workspace_size(8, 2, 128, 512, width * page)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    want = b.call(nb, max_q=1)
+    check_attention(want, b)
+    assert torch.equal(b.call(nb, max_q=1, workspace=ws), want)
+    out = torch.zeros_like(want)
+    cache = paged.Cache(b.k.data_ptr(), b.v.data_ptr(), b.n_pages, b.k.stride(0), 2, page, 128, 1)
+    batch = paged.Batch(table.data_ptr(), width, width, 3, b.row_lens.data_ptr(), b.seqs.data_ptr(),
+                        None, 3, 3)
+    assert lib().nq_paged_attention(b.q.data_ptr(), b.q.stride(0), 8, ctypes.byref(cache),
+                                    ctypes.byref(batch), 512, 128 ** -0.5, 0, ws.data_ptr(), size,
+                                    out.data_ptr(), out.stride(0), None) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)

@@ -112,6 +112,18 @@ def test_workspace_size_without_a_known_max_q_is_the_largest(nqlib):
         assert size(heads, kv_heads, 128, 1 << 62, keys) == size(heads, kv_heads, 128, 4096, keys)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (4, 2, 64), (64, 1, 256), (8, 8, 128),
+                                                (16, 1, 64), (128, 1, 128)])
+@pytest.mark.parametrize("keys", [16, 256, 272, 1024, 1280, 1296, 1 << 20])
+def test_a_workspace_serves_every_smaller_max_q(nqlib, heads, kv_heads, dim, keys):
+    """max_q is a bound: a workspace of its size fits calls with fewer new tokens, those
+    without q_starts (one token each) among them."""
+    size = nqlib.nq_paged_attention_workspace_size
+    qs = [1, 2, 3, 4, 8, 15, 16, 17, 64, 300, 4096]
+    sizes = [size(heads, kv_heads, dim, q, keys) for q in qs]
+    assert sizes == sorted(sizes) and sizes[-1] == size(heads, kv_heads, dim, 0, keys)
+
+
 def table(**kw):
     d = dict(refs=A, table=A, lens=A, n_pages=8, n_rows=4, table_ld=4, table_width=4, page_size=16)
     d.update(kw)
