@@ -394,7 +394,8 @@ int nq_paged_attention(const uint16_t *q, int64_t q_ld, int n_heads, const nq_pa
  * once; dims past 2 * n_freqs stay.  n_freqs is a multiple of 8, at most
  * head_dim / 2; 0 turns nothing.  The queries go to q_out (may be q itself).
  * A token at a negative position or whose page is missing is not stored (error
- * word).  Two entries of one call must not be the same sequence, nor hold their
+ * word), and an entry whose row, length or starts are out of range is left out
+ * (error word): it stores nothing, and its queries are not written.  Two entries of one call must not be the same sequence, nor hold their
  * new tokens' pages in common (nq_pages_reserve parts such pages): which of their
  * keys stay is not defined. */
 int nq_paged_append(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t k_ld,

@@ -89,7 +89,10 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 
     const int b = entry_of(a.pb, (int)i);
     if (b < 0) return;
-    const SeqView s = seq_view(a.pb, b);
+    bool cut;
+    const SeqView s = seq_view(a.pb, b, &cut);
+    // (counted from a cut length the tokens would be written over the keys before them)
+    if (cut) return;
     const int t = (int)i - s.q0;
     if (t < 0 || t >= s.n) return;  // behind the last sequence, or padding
     const int pos = s.len - s.n + t;

@@ -34,10 +34,10 @@ struct SeqView {
 
 // Reads entry b.  What the arrays say outside their ranges (a table row, a
 // length past the table's width, token rows past n_tokens) is cut to the range
-// and raises the error word; a padding entry has n == 0.
+// and raises the error word, and is told in *cut; a padding entry has n == 0.
 // (All loads first: each is a trip to L2, and a call waits for them before its
 // first key.)
-__device__ __forceinline__ SeqView seq_view(const PagedBatch &pb, int b) {
+__device__ __forceinline__ SeqView seq_view(const PagedBatch &pb, int b, bool *cut = nullptr) {
     SeqView s;
     s.row = pb.seqs ? pb.seqs[b] : b;
     int end = b + 1;
@@ -70,6 +70,7 @@ __device__ __forceinline__ SeqView seq_view(const PagedBatch &pb, int b) {
         s.len = s.len < 0 ? 0 : (int)most;
     }
     if (bad) atomicOr(pb.err, kErrBadIndex);
+    if (cut) *cut = bad;
     return s;
 }
 

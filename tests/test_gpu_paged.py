@@ -683,3 +683,32 @@ def test_a_step_in_the_workspace_of_a_chunk(page, width):
                                     out.data_ptr(), out.stride(0), None) == 0
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("spoil", ["length", "row", "starts"])
+def test_append_leaves_out_an_entry_that_is_out_of_range(spoil, new):
+    """Its tokens have no position: nothing is written over the keys that are there."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    draw = lambda *shape: torch.randn(shape, device="cuda", generator=g).to(BF)  # noqa: E731
+    k, v = draw(16, 2, 16, 64), draw(16, 2, 16, 64)
+    table = torch.randperm(16, device="cuda", generator=g).to(torch.int32).view(2, 8)  # all full
+    lens = torch.tensor([128, 100], dtype=torch.int32, device="cuda")
+    seqs = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 3, 3 + new], dtype=torch.int32, device="cuda")
+    q, kn, vn = draw(3 + new, 4, 64), draw(3 + new, 2, 64), draw(3 + new, 2, 64)
+    want = [x.clone() for x in (k, v, q)]
+    for t in range(3):  # the entry before it is stored as ever
+        page, slot = int(table[1, (97 + t) // 16]), (97 + t) % 16
+        want[0][page, :, slot], want[1][page, :, slot] = kn[t], vn[t]
+    if spoil == "length":
+        lens[0] = 128 + new
+    elif spoil == "row":
+        seqs[1] = 2
+    else:
+        starts[2] += 1
+    q_out = torch.full_like(q, 9.0)
+    nb.paged_append(q, kn, vn, k, v, table, lens, q_starts=starts, seqs=seqs, q_out=q_out)
+    assert nb.take_device_error() == 2
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    assert torch.equal(q_out[:3], q[:3]) and (q_out[3:] == 9).all()
