@@ -407,8 +407,9 @@ int nq_paged_append(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t 
  * below only enqueue work (and may be captured): refs[p] sequences hold page
  * p (0: free), table and lens as above, -1 in unused table entries.  A pool is
  * [outer][n_pages][page_bytes] (outer: layers x keys and values).  Sequence
- * lists are device int32; negative entries are padding.  A refused request
- * raises bit 2 of the device error word. */
+ * lists are device int32; negative entries are padding.  A list has at most
+ * 2^20 entries, nq_pages_reserve's 2^16 (entries are compared with one another).
+ * A refused request raises bit 2 of the device error word. */
 typedef struct nq_page_table {
     int32_t *refs;
     int32_t *table;

@@ -521,6 +521,12 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 constexpr int64_t kMaxInt = 0x7fffffff;
 
+// The longest lists that are taken.  The kernels compare each entry with those
+// before it, so their time grows with the square of the length: 65536 entries
+// take the reserve's one CTA 49 to 97 ms and a fork 6.7 ms; a list of millions
+// would hold the GPU for minutes.
+constexpr int64_t kMaxReserve = 1 << 16, kMaxList = 1 << 20;
+
 // The checks that attention and append share; fills pb.
 int check_batch(const nq_paged_cache_t *c, const nq_paged_batch_t *b, int n_heads, const char *fn,
                 PagedBatch *pb) {
@@ -584,12 +590,15 @@ int need_gpu(const char *fn) {
     return NQ_SUCCESS;
 }
 
-int check_table(const nq_page_table_t *t, int64_t n, const char *fn, PageTable *a) {
+int check_table(const nq_page_table_t *t, int64_t n, int64_t most, const char *fn, PageTable *a) {
     const std::string what(fn);
     if (!t) return fail(NQ_INVALID_INPUT, what + ": NULL page table");
+    if (n > most)
+        return fail(NQ_INVALID_INPUT,
+                    what + ": a list has at most " + std::to_string(most) + " entries");
     if (t->n_pages <= 0 || t->n_pages >= kMaxInt || t->n_rows <= 0 || t->n_rows >= kMaxInt ||
         t->table_width <= 0 || t->table_ld < t->table_width || t->page_size <= 0 ||
-        t->table_width * (int64_t)t->page_size >= kMaxInt || n < 0 || n >= kMaxInt)
+        t->table_width * (int64_t)t->page_size >= kMaxInt || n < 0)
         return fail(NQ_INVALID_INPUT, what + ": a size is not positive or too large");
     if (!t->refs || !t->table || !t->lens)
         return fail(NQ_INVALID_INPUT, what + ": NULL refs, table or lens");
@@ -736,7 +745,7 @@ int nq_paged_append(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t 
 int nq_pages_free(const nq_page_table_t *table, const int32_t *seqs, int64_t n, void *stream) {
     const char *fn = "nq_pages_free";
     PageTable a{};
-    if (int rc = check_table(table, n, fn, &a)) return rc;
+    if (int rc = check_table(table, n, kMaxList, fn, &a)) return rc;
     if (n == 0) return NQ_SUCCESS;
     if (!seqs) return fail(NQ_INVALID_INPUT, std::string(fn) + ": NULL list");
     if (int rc = need_gpu(fn)) return rc;
@@ -750,7 +759,7 @@ int nq_pages_fork(const nq_page_table_t *table, const int32_t *parents, const in
                   int64_t n, void *stream) {
     const char *fn = "nq_pages_fork";
     PageTable a{};
-    if (int rc = check_table(table, n, fn, &a)) return rc;
+    if (int rc = check_table(table, n, kMaxList, fn, &a)) return rc;
     if (n == 0) return NQ_SUCCESS;
     if (!parents || !children) return fail(NQ_INVALID_INPUT, std::string(fn) + ": NULL list");
     if (int rc = need_gpu(fn)) return rc;
@@ -771,7 +780,7 @@ size_t nq_pages_workspace_size(int64_t n_pages, int64_t n) {
 static int check_plan(const nq_page_table_t *table, const nq_page_pool_t *pool, int64_t n,
                       void *workspace, size_t bytes, size_t need, const char *fn, PageTable *a,
                       PagePool *p) {
-    if (int rc = check_table(table, n, fn, a)) return rc;
+    if (int rc = check_table(table, n, kMaxReserve, fn, a)) return rc;
     if (int rc = check_pool(pool, fn, p)) return rc;
     if (p->n_pages != a->n_pages)
         return fail(NQ_INVALID_INPUT, std::string(fn) + ": refs and the pool differ in pages");
@@ -791,7 +800,7 @@ int nq_pages_reserve(const nq_page_table_t *table, const nq_page_pool_t *pool, c
     PageTable a{};
     PagePool p{};
     // (the plan counts the pages that the list can ask for in 32 bits)
-    if (table && n > 0 && n < kMaxInt && table->table_width < kMaxInt &&
+    if (table && n > 0 && n <= kMaxReserve && table->table_width < kMaxInt &&
         n * table->table_width >= kMaxInt)
         return fail(NQ_INVALID_INPUT, std::string(fn) + ": a size is not positive or too large");
     if (int rc = check_plan(table, pool, n, workspace, workspace_bytes,
@@ -835,7 +844,9 @@ int nq_pages_copy(const nq_page_pool_t *pool, const int32_t *src, const int32_t 
     const char *fn = "nq_pages_copy";
     PagePool p{};
     if (int rc = check_pool(pool, fn, &p)) return rc;
-    if (n < 0 || n >= kMaxInt) return fail(NQ_INVALID_INPUT, std::string(fn) + ": bad count");
+    if (n < 0 || n > kMaxList)
+        return fail(NQ_INVALID_INPUT, std::string(fn) + ": a list has at most " +
+                                          std::to_string(kMaxList) + " entries");
     if (n == 0) return NQ_SUCCESS;
     if (!src || !dst) return fail(NQ_INVALID_INPUT, std::string(fn) + ": NULL list");
     if (int rc = need_gpu(fn)) return rc;

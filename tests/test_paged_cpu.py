@@ -169,6 +169,23 @@ def test_a_list_that_could_ask_for_2_31_pages_is_refused(nqlib):
     assert nqlib.nq_pages_reserve(t_, p_, A, A, 1 << 15, A, 1 << 40, None) == 1
 
 
+def test_lists_whose_checks_would_take_minutes_are_refused(nqlib):
+    t, p = table(table_width=1, table_ld=1), pool()
+    t_, p_ = ctypes.byref(t), ctypes.byref(p)
+    for n in ((1 << 16) + 1, 1 << 30):
+        assert nqlib.nq_pages_reserve(t_, p_, A, A, n, A, 1 << 60, None) == 1
+        assert b"entries" in nqlib.nq_last_error()
+    for n in ((1 << 20) + 1, 1 << 30, 1 << 62):
+        for rc in (nqlib.nq_pages_free(t_, A, n, None), nqlib.nq_pages_fork(t_, A, A, n, None),
+                   nqlib.nq_pages_copy(p_, A, A, n, None)):
+            assert rc == 1 and b"entries" in nqlib.nq_last_error()
+    if nqlib.nq_device_count() == 0:  # (without a device, the longest lists that are taken get as far as that)
+        for rc in (nqlib.nq_pages_reserve(t_, p_, A, A, 1 << 16, A, 1 << 60, None),
+                   nqlib.nq_pages_free(t_, A, 1 << 20, None),
+                   nqlib.nq_pages_copy(p_, A, A, 1 << 20, None)):
+            assert rc not in (0, 1)
+
+
 def test_page_lists_and_counts_are_checked(nqlib):
     t, p = table(), pool()
     t_, p_ = ctypes.byref(t), ctypes.byref(p)
