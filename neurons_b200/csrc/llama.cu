@@ -1205,7 +1205,8 @@ int nq_llama_forward(nq_llama_t dec, const int32_t *tokens, const nq_paged_cache
         return llama_fail(NQ_INVALID_INPUT,
                           what + ": the cache must be bf16, with the decoder's heads");
     if (layer_stride < 0 || layer_stride % 8 || max_q < 0 || n_out < 0 || batch->n_tokens < 0 ||
-        batch->n_tokens >= 0x7fffffff || n_out >= 0x7fffffff)
+        batch->n_tokens >= 0x7fffffff || n_out >= 0x7fffffff || cache->page_size <= 0 ||
+        batch->table_width < 0 || batch->table_width > 0x7fffffff / cache->page_size)
         return llama_fail(NQ_INVALID_INPUT, what + ": a size is negative or too large");
     if (batch->n_tokens == 0 || batch->n_seqs == 0) return NQ_SUCCESS;
     if (!tokens || (n_out > 0 && (!rows || (!logits && !next_tokens))))

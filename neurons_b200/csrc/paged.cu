@@ -527,6 +527,9 @@ constexpr int64_t kMaxInt = 0x7fffffff;
 // would hold the GPU for minutes.
 constexpr int64_t kMaxReserve = 1 << 16, kMaxList = 1 << 20;
 
+// whether a * b, both positive, is less than `limit`
+bool product_below(int64_t a, int64_t b, int64_t limit) { return a <= (limit - 1) / b; }
+
 // The checks that attention and append share; fills pb.
 int check_batch(const nq_paged_cache_t *c, const nq_paged_batch_t *b, int n_heads, const char *fn,
                 PagedBatch *pb) {
@@ -542,7 +545,8 @@ int check_batch(const nq_paged_cache_t *c, const nq_paged_batch_t *b, int n_head
         return fail(NQ_INVALID_INPUT, what + ": page_size must be a positive multiple of 16");
     if (c->n_pages < 0 || c->n_pages >= kMaxInt || b->n_seqs < 0 || b->n_seqs >= kMaxInt ||
         b->n_tokens < 0 || b->n_tokens >= kMaxInt || b->n_rows < 0 || b->n_rows >= kMaxInt ||
-        b->table_width < 0 || b->table_width * (int64_t)c->page_size >= kMaxInt)
+        b->table_width < 0 || !product_below(b->table_width, c->page_size, kMaxInt) ||
+        !product_below((int64_t)c->n_kv_heads * c->head_dim, c->page_size, (int64_t)1 << 62))
         return fail(NQ_INVALID_INPUT, what + ": a size is negative or too large");
     const int64_t page = (int64_t)c->n_kv_heads * c->page_size * c->head_dim;
     if (c->page_stride < page || c->page_stride % 8)
@@ -598,7 +602,7 @@ int check_table(const nq_page_table_t *t, int64_t n, int64_t most, const char *f
                     what + ": a list has at most " + std::to_string(most) + " entries");
     if (t->n_pages <= 0 || t->n_pages >= kMaxInt || t->n_rows <= 0 || t->n_rows >= kMaxInt ||
         t->table_width <= 0 || t->table_ld < t->table_width || t->page_size <= 0 ||
-        t->table_width * (int64_t)t->page_size >= kMaxInt || n < 0)
+        !product_below(t->table_width, t->page_size, kMaxInt) || n < 0)
         return fail(NQ_INVALID_INPUT, what + ": a size is not positive or too large");
     if (!t->refs || !t->table || !t->lens)
         return fail(NQ_INVALID_INPUT, what + ": NULL refs, table or lens");

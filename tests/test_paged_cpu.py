@@ -186,6 +186,23 @@ def test_lists_whose_checks_would_take_minutes_are_refused(nqlib):
             assert rc not in (0, 1)
 
 
+def test_sizes_whose_products_pass_64_bits_are_refused(nqlib):
+    for call in (attend, append):
+        for c, b in ((cache(), batch(table_width=1 << 60, table_ld=1 << 60)),
+                     (cache(), batch(table_width=(1 << 60) + 4, table_ld=1 << 61)),
+                     (cache(n_kv_heads=1 << 30, page_size=1 << 28), batch(table_width=1))):
+            heads = c.n_kv_heads
+            assert call(nqlib, c=c, b=b, heads=heads) == 1
+            assert b"too large" in nqlib.nq_last_error()
+    for width in (1 << 60, (1 << 60) + 4):
+        t, p = table(table_width=width, table_ld=width), pool()
+        t_, p_ = ctypes.byref(t), ctypes.byref(p)
+        for rc in (nqlib.nq_pages_free(t_, A, 1, None), nqlib.nq_pages_fork(t_, A, A, 1, None),
+                   nqlib.nq_pages_reserve(t_, p_, A, A, 1, A, 1 << 40, None),
+                   nqlib.nq_pages_compact(t_, p_, A, 1 << 40, None)):
+            assert rc == 1 and b"too large" in nqlib.nq_last_error()
+
+
 def test_page_lists_and_counts_are_checked(nqlib):
     t, p = table(), pool()
     t_, p_ = ctypes.byref(t), ctypes.byref(p)
