@@ -290,3 +290,49 @@ def test_steps_behind_a_long_chunked_prompt(oracle, nqlib):
     for i in range(3):
         close(dec.step(toks[n + i:n + i + 1])[0], want[i], f"step {i}")
     assert nb.take_device_error() == 0
+
+
+def test_compaction_between_steps(nqlib, model):
+    """Right after srv.compact() the used pages are the lowest, and the next steps' logits are
+    those of a decoder of each sequence's own."""
+    dec = LlamaDecoder(cfg(), model[1])
+    srv = PagedLlama(dec, n_pages=40, page_size=16, max_seqs=4, max_len=300)
+    toks = torch.randint(0, SMALL["vocab"], (230,), dtype=torch.int32, device="cuda")
+    srv.step([0, 1, 2], torch.cat([toks[:200], toks[:50], toks[:120]]), [200, 50, 120])
+    srv.fork(2, [3])
+    srv.free([0])
+    used = int((srv.refs > 0).sum())
+    assert int(srv.table.max()) >= used
+    srv.compact()
+    assert (srv.refs[:used] > 0).all() and (srv.refs[used:] == 0).all()
+    assert int(srv.table.max()) == used - 1
+    lg, _ = srv.step([1, 2, 3], torch.cat([toks[50:51], toks[120:150], toks[7:8]]), [1, 30, 1])
+    ref = LlamaDecoder(cfg(), model[1])
+    ref.set_prefill_chunk(300)
+    for got, said in zip(lg, (toks[:51], toks[:150], torch.cat([toks[:120], toks[7:8]]))):
+        ref.reset()
+        close(got, ref.prefill(said.contiguous()), f"{said.numel()} tokens")
+    assert nb.take_device_error() == 0
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 4, 64), (16, 2, 64), (4, 2, 256)])
+def test_other_head_dims(oracle, nqlib, heads, kv, dim):
+    """Chunks, steps behind them and paged serving with heads of 64 and 256 dims."""
+    from oracle.llama_oracle import LlamaOracle
+    c = dict(SMALL, n_heads=heads, n_kv_heads=kv, head_dim=dim, max_context=200)
+    host, dev = make_model(oracle, c, dim)
+    dec, ora = LlamaDecoder(c, dev), LlamaOracle(c, host)
+    toks = np.random.default_rng(6).integers(0, c["vocab"], 41).astype(np.int32)
+    td = torch.from_numpy(toks).cuda()
+    refs = [ora.step(int(t))[0] for t in toks]
+    dec.set_prefill_chunk(24)
+    check_logits(oracle, dec.prefill(td[:40].contiguous()), refs[39], "chunks")
+    check_logits(oracle, dec.step(td[40:])[0], refs[40], "step")
+    srv = PagedLlama(dec, n_pages=10, page_size=16, max_seqs=2, max_len=64)
+    lg, _ = srv.step([0, 1], torch.cat([td[:40], td[:3]]), [40, 3])
+    check_logits(oracle, lg[0], refs[39], "paged prompt")
+    check_logits(oracle, lg[1], refs[2], "short paged prompt")
+    lg, _ = srv.step([0, 1], torch.cat([td[40:], td[3:4]]), [1, 1])
+    check_logits(oracle, lg[0], refs[40], "paged step")
+    check_logits(oracle, lg[1], refs[3], "short paged step")
+    assert nb.take_device_error() == 0

@@ -712,3 +712,73 @@ def test_append_leaves_out_an_entry_that_is_out_of_range(spoil, new):
     assert nb.take_device_error() == 2
     assert torch.equal(k, want[0]) and torch.equal(v, want[1])
     assert torch.equal(q_out[:3], q[:3]) and (q_out[3:] == 9).all()
+
+
+# ------------------------------------------------------- what sits side by side
+
+@pytest.mark.parametrize("lens,news,heads,kv,dim,page,dtype,window", [
+    ([2400, 1700], [700, 90], 4, 2, 256, 16, BF, 1024),   # 32 boxes a block, a ring of one block
+    ([1500], [33], 8, 4, 256, 16, HF, 300),
+    ([1400, 1300], [150, 1], 8, 4, 256, 128, BF, 1024),
+    ([3000], [200], 4, 1, 128, 16, HF, 1024),
+    ([900, 2000], [600, 3], 4, 2, 64, 16, BF, 500),
+])
+def test_windows_over_many_blocks(lens, news, heads, kv, dim, page, dtype, window):
+    b = Batch(lens, news, heads, kv, dim, page, dtype, seed=61, window=window)
+    check_attention(b.call(nb, window=window, max_q=max(news)), b, window)
+    assert nb.take_device_error() == 0
+
+
+@pytest.mark.parametrize("lens,news", [([200], [1]), ([1, 17, 250, 64], [1] * 4), ([90, 300], [30, 1])])
+def test_short_sequences_in_a_wide_table(lens, news):
+    """A server's table has room for its longest sequence: short ones are cut and joined
+    there, where a table as wide as they are leaves their tiles whole."""
+    b = Batch(lens, news, 8, 2, 128, 16, BF, seed=62)
+    want = b.call(nb, max_q=max(news))
+    wide = torch.full((len(lens), 600), -1, dtype=torch.int32, device="cuda")
+    wide[:, :b.table.shape[1]] = b.table
+    b.table = wide
+    got = b.call(nb, max_q=max(news))
+    check_attention(got, b)
+    check_attention(want, b)
+    assert nb.take_device_error() == 0
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_attention_at_random(seed):
+    """Batches of any make: group sizes that do and do not divide a tile, pages, windows,
+    entries without tokens or longer than their sequence; and the same bits again."""
+    rng = random.Random(1000 + seed)
+    kv = rng.choice([1, 2, 3])
+    group = rng.choice([1, 2, 3, 4, 5, 7, 8, 12, 16, 17, 33, 64, 100])
+    dim, page = rng.choice([64, 128, 256]), rng.choice([16, 32, 48, 64, 80, 128, 144, 256])
+    dtype, window = rng.choice([BF, HF]), rng.choice([0, 0, 1, 15, 64, 200, 1000])
+    n = rng.choice([1, 2, 5, 40])
+    lens = [rng.choice([0, 1, rng.randint(2, 70), rng.randint(100, 1500)]) for _ in range(n)]
+    many = rng.choice([1, 1, 4, 40, 300])
+    news = [rng.choice([0, 1, rng.randint(1, many)]) for _ in range(n)]
+    news[0] = max(news[0], 1)
+    if rng.random() < 0.7:  # (else some rows have no key)
+        lens = [max(a, m) for a, m in zip(lens, news)]
+    b = Batch(lens, news, kv * group, kv, dim, page, dtype, seed=seed, window=window)
+    max_q = rng.choice([None, max(news), 1])
+    got = b.call(nb, window=window, max_q=max_q)
+    check_attention(got, b, window)
+    assert torch.equal(b.call(nb, window=window, max_q=max_q), got)
+    assert nb.take_device_error() == 0
+
+
+def test_compaction_leaves_the_used_pages_in_front():
+    """refs and table right after a compaction, beside shared and half-used pages."""
+    d = Device(120, 10, 8)
+    d.reserve([0, 1, 2, 3], [100, 40, 128, 1])
+    d.fork([0, 2], [4, 5])
+    d.reserve([4, 5, 6], [101, 128, 60])
+    d.free([1, 0])
+    nb.take_device_error()
+    used = int((d.refs > 0).sum())
+    assert int(d.table.max()) >= used  # (there is something to move)
+    d.compact()
+    assert (d.refs[:used] > 0).all() and (d.refs[used:] == 0).all()
+    assert int(d.table.max()) == used - 1
+    d.check()
