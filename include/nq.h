@@ -374,7 +374,8 @@ typedef struct nq_paged_batch {
  * its row NaN.  max_q: no entry has more new tokens than this (it
  * selects the kernel and the workspace's size, results hold for any; 0:
  * unknown, with the workspace that any would need).  Softmax and sums in fp32;
- * the weights are rounded to the cache's type for the second product, the result
+ * for the second product the weights are two terms of the cache's type where
+ * max_q * G <= 16, and rounded to one where it is more; the result is rounded
  * once.  workspace: nq_paged_attention_workspace_size() bytes for this max_q (or
  * a larger one) and max_keys = table_width * page_size (0: none is needed),
  * 256-byte aligned, contents irrelevant; two calls that overlap on the GPU need

@@ -344,7 +344,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                             }
                         }
                 }
-                uint32_t pf[NT][2];
+                // The weights go to the tensor cores, which take both factors in one type, as
+                // two terms of it, a weight's rounding and what that left out: 16 bits of
+                // precision or more, as much as the sum l has of use, where one term made a
+                // result's error 1.4 times that of its own rounding.  (The tensor pipe is
+                // idle for nine tenths of a decode step: 64 sequences 94.6 -> 94.9 us, one
+                // token over 200 keys 7.23 -> 7.32.)
+                uint32_t pf[NT][2], pl[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float w[4];
@@ -355,23 +361,37 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                         w[e + 2] = ex2(fmaf(s[nt][e + 2], cs, -z));
                         l[nt][e] += w[e] + w[e + 2];
                     }
-                    // the weights are rounded to the cache's type, as the tensor cores
-                    // take both factors in one type
-                    pf[nt][0] = transpose8(pack_t2<F16>(w[0], w[1]));
-                    pf[nt][1] = transpose8(pack_t2<F16>(w[2], w[3]));
+                    const uint32_t h0 = pack_t2<F16>(w[0], w[1]), h1 = pack_t2<F16>(w[2], w[3]);
+                    pf[nt][0] = transpose8(h0);
+                    pf[nt][1] = transpose8(h1);
+                    pl[nt][0] = transpose8(pack_t2<F16>(w[0] - t16_to_f32<F16>((uint16_t)h0),
+                                                        w[1] - t16_to_f32<F16>((uint16_t)(h0 >> 16))));
+                    pl[nt][1] = transpose8(pack_t2<F16>(w[2] - t16_to_f32<F16>((uint16_t)h1),
+                                                        w[3] - t16_to_f32<F16>((uint16_t)(h1 >> 16))));
                 }
                 {
-                    // matrices: dims 0-7 / keys 0-7, dims 8-15 / keys 0-7, then keys 8-15
+                    // matrices: dims 0-7 / keys 0-7, dims 8-15 / keys 0-7, then keys 8-15;
+                    // four dims' products between the two that add to the same sums
                     const int row = (lane & 7) + ((lane >> 4) << 3);
                     const uint32_t rowa = smem_u32(vs) + row * 128;
 #pragma unroll
-                    for (int t = 0; t < HD / 16; ++t) {
-                        const int ch = (t & 3) * 2 + ((lane >> 3) & 1);
-                        uint32_t f[4];
-                        ldsm4_t(f, rowa + (t >> 2) * col_ld + ((ch ^ (row & 7)) << 4));
+                    for (int t = 0; t < HD / 16; t += 4) {
+                        uint32_t f[4][4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int ch = ((t + e) & 3) * 2 + ((lane >> 3) & 1);
+                            ldsm4_t(f[e], rowa + (t >> 2) * col_ld + ((ch ^ (row & 7)) << 4));
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            mma16816<F16>(o[t][nt], f, pf[nt][0], pf[nt][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                mma16816<F16>(o[t + e][nt], f[e], pf[nt][0], pf[nt][1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                mma16816<F16>(o[t + e][nt], f[e], pl[nt][0], pl[nt][1]);
                     }
                 }
                 if (key0 < key_lo || key0 + 16 > key_hi) fence_proxy_async_smem();

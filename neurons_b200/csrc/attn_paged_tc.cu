@@ -635,7 +635,9 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                                                make_float2(cs, cs), make_float2(-z, -z));
                         const float e0 = ex2(x2.x), e1 = ex2(x2.y);
                         sum[e & 1] = add2(sum[e & 1], make_float2(e0, e1));
-                        // rounded to the cache's type: both factors of an MMA are of one type
+                        // Rounded to the cache's type: both factors of an MMA are of one type.
+                        // (A second term, as attn_paged.cu's kernel takes, would be as many
+                        // MMAs and stores again on the chain that bounds this one.)
                         pk[e] = pack_t2<F16>(e0, e1);
                     }
                     tmem_st_32x32b_x16(sc + j * 16, pk);

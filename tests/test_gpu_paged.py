@@ -782,3 +782,17 @@ def test_compaction_leaves_the_used_pages_in_front():
     assert (d.refs[:used] > 0).all() and (d.refs[used:] == 0).all()
     assert int(d.table.max()) == used - 1
     d.check()
+
+
+@pytest.mark.parametrize("lens,news,heads,kv,dim,page,dtype", [
+    ([200], [1], 32, 8, 128, 16, BF), ([1, 2, 1000, 37, 513], [1] * 5, 8, 1, 128, 32, BF),
+    ([5000, 3], [1, 1], 4, 2, 64, 16, BF), ([700, 33], [1, 1], 8, 4, 256, 16, BF),
+    ([900, 64], [4, 2], 8, 2, 128, 64, BF), ([900, 5000], [2, 1], 32, 4, 64, 64, HF)])
+def test_few_rows_keep_the_weights(lens, news, heads, kv, dim, page, dtype):
+    """A decode step's weights are held in two terms of the cache's type: what is left of
+    their rounding is u^2."""
+    b = Batch(lens, news, heads, kv, dim, page, dtype, seed=71)
+    want, bound = attention64(b, terms=2)
+    got = b.call(nb, max_q=max(news)).double()
+    over = (got - want).abs() - bound
+    assert (over <= 1e-12).all(), f"{over.max().item():.3e} over the bound"
