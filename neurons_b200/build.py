@@ -93,8 +93,15 @@ def build(force: bool = False, verbose: bool = False) -> str:
                        check=True)
         os.replace(tmp, LIB)
     build_dist(force, verbose)
-    build_paged(force)
+    if has_torch():
+        build_paged(force)
     return LIB
+
+
+def has_torch():
+    """Whether a torch is installed for _paged.so to be built against (libnq.so needs none)."""
+    import importlib.util
+    return importlib.util.find_spec("torch") is not None
 
 
 def build_paged(force: bool = False) -> str:

@@ -636,8 +636,10 @@ __global__ void __launch_bounds__(Tc<HD>::kThreads, 1) paged_tiles_kernel(
                         const float e0 = ex2(x2.x), e1 = ex2(x2.y);
                         sum[e & 1] = add2(sum[e & 1], make_float2(e0, e1));
                         // Rounded to the cache's type: both factors of an MMA are of one type.
-                        // (A second term, as attn_paged.cu's kernel takes, would be as many
-                        // MMAs and stores again on the chain that bounds this one.)
+                        // (A second term, as attn_paged.cu's kernel takes, is as many MMAs and
+                        // stores again on the chain that bounds this one: a prompt of 8192
+                        // tokens 559 -> 754 us, for an error against 64 bits of 0.0017 instead
+                        // of 0.0023; the result's own rounding makes 0.0017.)
                         pk[e] = pack_t2<F16>(e0, e1);
                     }
                     tmem_st_32x32b_x16(sc + j * 16, pk);

@@ -23,3 +23,15 @@ def test_build_targets_sm100a_only(nqlib):
     assert "sm_90" not in flags and "compute_90" not in flags
     for path in (build.LIB, build.DIST_LIB):
         assert os.path.exists(path), path
+
+
+def test_libnq_is_built_without_torch(nqlib, monkeypatch):
+    """Only the Python binding of the paged cache needs torch's headers."""
+    from neurons_b200 import build
+    asked = []
+    monkeypatch.setattr(build, "build_paged", lambda *a: asked.append(a))
+    build.build()
+    assert len(asked) == 1
+    monkeypatch.setattr(build, "has_torch", lambda: False)
+    assert build.build() == build.LIB
+    assert len(asked) == 1
