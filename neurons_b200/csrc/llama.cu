@@ -74,10 +74,13 @@ __device__ __forceinline__ uint16_t dq_value(uint32_t q, uint16_t s, uint16_t b)
 }
 
 // h = row `token` of the embedding (quantized: dequantized exactly as
-// nq_dequantize; dense: copied).  The token comes from device memory.
+// nq_dequantize; dense: copied).  The token comes from device memory.  turn
+// (unless NULL) gets this position's `half` turns (cosine, sine) for the step's
+// attention.
 __global__ void embed_kernel(const int32_t *tok_src, const uint32_t *ew, const uint16_t *es,
                              const uint16_t *eb, const uint16_t *dense, int64_t hidden, int bits,
-                             int gs, int64_t vocab, uint16_t *h, unsigned *err) {
+                             int gs, int64_t vocab, uint16_t *h, unsigned *err, const int32_t *pos,
+                             const float *freqs, int half, float2 *turn) {
     pdl_launch_dependents();
     pdl_wait();  // the token may be the previous step's argmax
     int64_t t = *tok_src;
@@ -85,6 +88,8 @@ __global__ void embed_kernel(const int32_t *tok_src, const uint32_t *ew, const u
         if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(err, kErrBadIndex);
         t = 0;
     }
+    if (turn && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < half; i += blockDim.x) turn[i] = rope_turn(*pos, freqs[i]);
     for (int64_t k = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; k < hidden;
          k += (int64_t)gridDim.x * blockDim.x) {
         if (dense) {
@@ -102,21 +107,21 @@ __global__ void embed_kernel(const int32_t *tok_src, const uint32_t *ew, const u
 // RoPE (MLX fast::rope, traditional = false, scale 1): for i < d/2,
 // angle = pos * base^(-i/(d/2)); (x_i, x_{i+d/2}) rotated by it in fp32 and
 // rounded to bf16.  Returns the rotated value of element e of a head.
-// FREQS: by rope_turn() and the decoder's frequencies, as nq_paged_append turns
-// the keys of a chunk.
-template <bool FREQS>
-__device__ __forceinline__ float rope_elem(const uint16_t *head, int e, int hd, int pos,
-                                           float log2_base, const float *freqs) {
+// turn (unless NULL): this position's turns, those of nq_paged_append's keys
+// (rope_turn()), in place of the angle in 32 bits, which is computed all the same:
+// it costs nothing, and a kernel compiled without it took a step of the 28-layer
+// Llama-3.2-3B shape 1.64 instead of 1.55 ms.
+__device__ __forceinline__ float rope_elem(const uint16_t *head, int e, int hd, float pos,
+                                           float log2_base, const float2 *turn) {
     const int half = hd / 2;
     const int i = e < half ? e : e - half;
+    const float inv_freq = exp2f(-((float)i / (float)half) * log2_base);
     float sn, cs;
-    if constexpr (FREQS) {
-        const float2 t = rope_turn(pos, freqs[i]);
+    sincosf(pos * inv_freq, &sn, &cs);
+    if (turn) {
+        const float2 t = turn[i];
         cs = t.x;
         sn = t.y;
-    } else {
-        const float inv_freq = exp2f(-((float)i / (float)half) * log2_base);
-        sincosf((float)pos * inv_freq, &sn, &cs);
     }
     const float x1 = bf16_to_f32(head[i]), x2 = bf16_to_f32(head[i + half]);
     const float r = e < half ? x1 * cs - x2 * sn : x1 * sn + x2 * cs;
@@ -133,7 +138,7 @@ struct AttnArgs {
     unsigned *err;
     int n_heads, n_kv, hd, max_ctx, ctx_ld, splits;  // ctx_ld: positions a cache has room for
     float log2_base, scale;
-    const float *freqs;         // [hd / 2] radians per position; nullptr: from log2_base, in 32 bits
+    const float2 *turn;         // [hd / 2] this position's; nullptr: from log2_base, in 32 bits
 };
 
 // kDpl consecutive bf16 values -> fp32 (one 4-, 8- or 16-byte load)
@@ -170,7 +175,7 @@ __device__ __forceinline__ void load_bf16(const uint16_t *p, float *out) {
 // warp and a warp's rows are all in flight together.  Each CTA writes its
 // softmax partials (max, sum, weighted values); the last CTA of a query head
 // (atomic count) merges the chunks in chunk order.  No CTA waits for another.
-template <int HD, bool FREQS>
+template <int HD>
 __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
     pdl_launch_dependents();
     pdl_wait();  // q, k, v come from the qkv projection
@@ -193,13 +198,14 @@ __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
     const int n_active = pos / kAttnChunk + 1;
     if (s >= n_active) return;
     const int t0 = s * kAttnChunk, t1 = min(t0 + kAttnChunk, pos + 1);
+    const float fpos = (float)pos;
     const uint16_t *qraw = a.qkv + (size_t)hq * HD;
     const uint16_t *kraw = a.qkv + (size_t)(a.n_heads + j) * HD;
     const uint16_t *vraw = a.qkv + (size_t)(a.n_heads + a.n_kv + j) * HD;
     const bool has_new = t1 == pos + 1;
     for (int d = tid; d < HD; d += kAttnThreads) {
-        qs[d] = rope_elem<FREQS>(qraw, d, HD, pos, a.log2_base, a.freqs);
-        if (has_new) kn[d] = rope_elem<FREQS>(kraw, d, HD, pos, a.log2_base, a.freqs);
+        qs[d] = rope_elem(qraw, d, HD, fpos, a.log2_base, a.turn);
+        if (has_new) kn[d] = rope_elem(kraw, d, HD, fpos, a.log2_base, a.turn);
     }
     uint16_t *kc = a.kc + (size_t)j * a.ctx_ld * HD;
     uint16_t *vc = a.vc + (size_t)j * a.ctx_ld * HD;
@@ -461,6 +467,7 @@ struct LlamaDecoder {
     int32_t *one_seq = nullptr;  // page table {0}, length, {0, tokens}, last row of a chunk
     int64_t chunk = 0;           // tokens per step of a prompt (0: one, by the decode step)
     bool chunked = false;        // the cache may hold keys of chunks: steps take their angles
+    float2 *turn = nullptr;      // [hd / 2] a step's own, then
     void *chunk_ws = nullptr;
     size_t chunk_ws_bytes = 0;
     int splits = 1;
@@ -562,11 +569,10 @@ cudaError_t gemv(const LlamaDecoder &d, const uint16_t *x, int64_t x_ld, const u
 
 }  // namespace
 
-template <bool FREQS>
 cudaError_t launch_attention(int hd, dim3 grid, const AttnArgs &aa, cudaStream_t st) {
-    if (hd == 64) return launch_pdl_ll(attn_kernel<64, FREQS>, grid, kAttnThreads, 0, st, aa);
-    if (hd == 128) return launch_pdl_ll(attn_kernel<128, FREQS>, grid, kAttnThreads, 0, st, aa);
-    return launch_pdl_ll(attn_kernel<256, FREQS>, grid, kAttnThreads, 0, st, aa);
+    if (hd == 64) return launch_pdl_ll(attn_kernel<64>, grid, kAttnThreads, 0, st, aa);
+    if (hd == 128) return launch_pdl_ll(attn_kernel<128>, grid, kAttnThreads, 0, st, aa);
+    return launch_pdl_ll(attn_kernel<256>, grid, kAttnThreads, 0, st, aa);
 }
 
 // One decode step: tok_src holds the input token (device); the argmax goes to
@@ -577,10 +583,12 @@ cudaError_t llama_step(LlamaDecoder &d, const int32_t *tok_src, float *logits_f3
     unsigned *err = device_error_word();
     const int64_t H = c.hidden, hd = c.head_dim, nq_ = (int64_t)c.n_heads * hd,
                   nkv = (int64_t)c.n_kv_heads * hd, I = c.intermediate;
+    float2 *turn = d.chunked ? d.turn : nullptr;
     cudaError_t e;
     if ((e = launch_pdl_ll(embed_kernel, dim3((unsigned)((H + 255) / 256)), 256, 0, st, tok_src,
                            d.embed.w, d.embed.scales, d.embed.biases, d.embed_dense, H, c.bits,
-                           c.group_size, (int64_t)c.vocab, d.h, err)) != cudaSuccess)
+                           c.group_size, (int64_t)c.vocab, d.h, err, (const int32_t *)d.pos,
+                           (const float *)d.freqs, c.head_dim / 2, turn)) != cudaSuccess)
         return e;
     AttnArgs aa;
     aa.qkv = d.qkv;
@@ -598,7 +606,7 @@ cudaError_t llama_step(LlamaDecoder &d, const int32_t *tok_src, float *logits_f3
     aa.ctx_ld = d.ctx_ld;
     aa.splits = d.splits;
     aa.log2_base = log2f(c.rope_theta);
-    aa.freqs = d.chunked ? d.freqs : nullptr;
+    aa.turn = turn;
     aa.scale = 1.0f / sqrtf((float)c.head_dim);
     const size_t layer_cache = (size_t)c.n_kv_heads * d.ctx_ld * hd;
     for (int l = 0; l < c.n_layers; ++l) {
@@ -609,8 +617,7 @@ cudaError_t llama_step(LlamaDecoder &d, const int32_t *tok_src, float *logits_f3
         aa.kc = d.kc + (size_t)l * layer_cache;
         aa.vc = d.vc + (size_t)l * layer_cache;
         const dim3 agrid((unsigned)d.splits, (unsigned)c.n_heads);
-        e = aa.freqs ? launch_attention<true>(c.head_dim, agrid, aa, st)
-                     : launch_attention<false>(c.head_dim, agrid, aa, st);
+        e = launch_attention(c.head_dim, agrid, aa, st);
         if (e != cudaSuccess) return e;
         if ((e = gemv(d, d.attn, nq_, L.o_w, L.o_s, L.o_b, H, nq_, d.h, 0, nullptr, d.h, st)) !=
             cudaSuccess)
@@ -717,7 +724,8 @@ cudaError_t llama_create(LlamaDecoder &d, const nq_llama_config_t &c,
         (e = d.alloc(&d.counter, (size_t)c.n_heads)) || (e = d.alloc(&d.pos, 1)) ||
         (e = d.alloc(&d.tok, 1)) || (e = d.alloc(&d.part_v, kArgmaxBlocks)) ||
         (e = d.alloc(&d.part_i, kArgmaxBlocks)) || (e = d.alloc(&d.amax_counter, 1)) ||
-        (e = d.alloc(&d.freqs, hd / 2)) || (e = d.alloc(&d.one_seq, 8)))
+        (e = d.alloc(&d.freqs, hd / 2)) || (e = d.alloc(&d.turn, hd / 2)) ||
+        (e = d.alloc(&d.one_seq, 8)))
         return e;
     std::vector<float> freqs(hd / 2);
     for (size_t i = 0; i < freqs.size(); ++i)
