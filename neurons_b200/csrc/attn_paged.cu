@@ -19,10 +19,12 @@
 // until the tile's end.
 //
 // Bounded by HBM where there are many keys: 64 sequences of up to 8192 keys (554
-// MB) 94 us, 5.9 TB/s or 0.90 of a copy's rate; two of 100003 (331 MB) 59 us,
-// 0.86; the rest is the start (about 4 us until a CTA's first keys are there:
-// lengths, table and keys are one memory trip after another) and the merge (2 us).
-// One token over 200 keys, 7.3 us, is these trips alone.
+// MB) 95 us, 5.8 TB/s or 0.89 of a copy's rate; two of 100003 and 61805 (331 MB)
+// 60 us, 0.84; the rest is the start (about 4 us until a CTA's first keys are
+// there: lengths, table and keys are one memory trip after another) and the merge
+// (2 us).  One token over 200 keys, 7.3 us, is these trips alone where the table
+// has room for 256 keys at most; in a wider one (any server's) its tiles are cut
+// and joined, 10.4 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -346,10 +348,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kCtas) paged_rows_kernel(
                 }
                 // The weights go to the tensor cores, which take both factors in one type, as
                 // two terms of it, a weight's rounding and what that left out: 16 bits of
-                // precision or more, as much as the sum l has of use, where one term made a
-                // result's error 1.4 times that of its own rounding.  (The tensor pipe is
-                // idle for nine tenths of a decode step: 64 sequences 94.6 -> 94.9 us, one
-                // token over 200 keys 7.23 -> 7.32.)
+                // precision or more, where one term made a result's error 1.4 times that of
+                // its own rounding.  (The tensor pipe, 10 % busy with one term, is 15 % busy
+                // with two: 64 sequences 94.8 -> 95.2 us, one token over 200 keys 7.21 ->
+                // 7.31.)
                 uint32_t pf[NT][2], pl[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -630,11 +632,14 @@ int rows_grid(int hd) {
 // Which kernel serves a call: paged_rows_kernel while a sequence's new tokens
 // make one tile of 16 rows, so that each key is read once; the tensor-core
 // kernel (128- or 256-row tiles) from there on.
-// Tiles are left whole where no sequence, or no window with a tile's tokens, has
-// more than kWholeKeys (kWholeKeysTiles) keys: a few blocks take less than the
-// parts and their merge, about 10 us for the tensor-core kernel (a windowed
-// chunk 45 -> 37 us).  Where the tiles are as many as the SMs, twice as many keys
-// (a prompt of 2048 tokens 71 -> 59 us).
+// Tiles are left whole where no sequence, or no window with a tile's tokens, can
+// have more than kWholeKeys (kWholeKeysTiles) keys, by the table's width: a few
+// blocks take less than the parts and their merge.  Cut -> whole, us: one token
+// over 256 keys 8.7 -> 7.3, over 512 8.7 -> 10.5; a windowed chunk (1024 keys)
+// 45.6 -> 35.2; prompts of 512 / 1024 / 1280 tokens, 32 heads of 8 key heads, 26.5 ->
+// 18.2, 37.7 -> 26.4, 43.5 -> 37.3 (but 4 heads of one key head, a few tiles on 148
+// SMs, 18.9 -> 17.1, 20.5 -> 24.3, 21.4 -> 27.9).  Where the tiles are as many as the
+// SMs, twice as many keys (a prompt of 2048 62.0 -> 50.8; 2560 81 -> 94).
 struct Shape {
     bool tiles, whole;
     int grid, rows, block;  // CTAs, rows of a part, keys of a block

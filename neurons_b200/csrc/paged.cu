@@ -53,7 +53,8 @@ constexpr int kAppendThreads = 128;
 // page.  One CTA per token: its angles are computed once for all heads.
 // Memory bounds it: the first three vector pairs and one value vector of a thread
 // (all there are for 40 turned heads of 128 dims) are under way before the token's
-// entry, page and angles are looked up (12288 tokens 69 -> 49 us, 5.5 TB/s).
+// entry, page and angles are looked up (four chunks of 11091 tokens 69 -> 49 us
+// when it came; 51 to 54 us over several GPUs, 5.1 to 5.3 TB/s).
 template <bool F16>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
     pdl_launch_dependents();
@@ -432,8 +433,8 @@ struct PagePool {
     int n_pages;
 };
 
-// Four 16-byte vectors a thread and step: 2.85 GB of reads and writes take 477 us,
-// 0.91 of a plain copy's rate; eight vectors, or loads that pass by the caches,
+// Four 16-byte vectors a thread and step: 2.85 GB of reads and writes take 476 us,
+// 0.92 of a plain copy's rate; eight vectors, or loads that pass by the caches,
 // gained nothing.
 constexpr int kCopyThreads = 256, kCopyBytes = kCopyThreads * 16 * 4;  // per step of a CTA
 
