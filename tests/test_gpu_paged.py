@@ -796,3 +796,61 @@ def test_few_rows_keep_the_weights(lens, news, heads, kv, dim, page, dtype):
     got = b.call(nb, max_q=max(news)).double()
     over = (got - want).abs() - bound
     assert (over <= 1e-12).all(), f"{over.max().item():.3e} over the bound"
+
+
+@pytest.mark.parametrize("many", [1, 60])
+def test_batches_of_padding_gaps_and_repeats(many):
+    """Nothing but padding; rows in front of the first entry; a sequence listed twice."""
+    b = Batch([900, 300], [many, many], 8, 2, 128, 16, BF, seed=81)
+    want = b.call(nb, max_q=many).clone()
+    kw = dict(max_q=many, scale=None)
+    out = torch.full_like(want, 4.0)
+    nb.paged_attention(b.q, b.k, b.v, b.table, b.row_lens, q_starts=b.starts,
+                       seqs=torch.full_like(b.seqs, -1), out=out, **kw)
+    assert (out == 4).all()
+    # five rows of another's before the first entry
+    q = torch.cat([torch.full_like(want[:1], float("nan")).repeat(5, 1, 1), b.q])
+    out = torch.full((len(q), 8, 128), 4.0, dtype=BF, device="cuda")
+    nb.paged_attention(q, b.k, b.v, b.table, b.row_lens, q_starts=b.starts + 5, seqs=b.seqs, out=out,
+                       **kw)
+    assert (out[:5] == 4).all()
+    check_attention(out[5:], b)
+    # each sequence twice, for the same new tokens
+    starts = torch.cat([b.starts, b.starts[1:] + b.starts[-1]])
+    got = nb.paged_attention(torch.cat([b.q, b.q]), b.k, b.v, b.table, b.row_lens, q_starts=starts,
+                             seqs=torch.cat([b.seqs, b.seqs]), **kw)
+    check_attention(got[:b.tokens], b)
+    check_attention(got[b.tokens:], b)
+    assert nb.take_device_error() == 0
+
+
+@pytest.mark.parametrize("most", [1, 20])
+def test_a_batch_of_many_sequences(most):
+    """1500 entries, padding among them: more than a warp's lanes many times over."""
+    rng = random.Random(9)
+    lens = [rng.choice([1, 16, 40, rng.randint(1, 90)]) for _ in range(1500)]
+    news = [min(n, rng.randint(1, most)) for n in lens]
+    b = Batch(lens, news, 4, 2, 64, 16, BF, seed=82)
+    check_attention(b.call(nb, max_q=most), b)
+    check_attention(b.call(nb), b)
+    want = b.call(nb, max_q=most)
+    seqs = b.seqs.clone()
+    gone = torch.rand(1500, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) < 0.4
+    seqs[gone] = -1
+    out = torch.full_like(want, 4.0)
+    nb.paged_attention(b.q, b.k, b.v, b.table, b.row_lens, q_starts=b.starts, seqs=seqs, max_q=most,
+                       out=out)
+    row_gone = gone.repeat_interleave(torch.tensor(news, device="cuda"))
+    assert (out[row_gone] == 4).all()
+    out[row_gone] = want[row_gone]
+    check_attention(out, b)
+    assert nb.take_device_error() == 0
+
+
+def test_values_that_are_the_keys():
+    """One tensor as keys and values, in pages of a whole sequence."""
+    b = Batch([700, 1500], [1, 30], 4, 1, 128, 2048, BF, seed=83)
+    b.v = b.k
+    b.dense = [(k, k) for k, _ in b.dense]
+    check_attention(b.call(nb), b)
+    check_attention(b.call(nb, max_q=1), b)
