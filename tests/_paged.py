@@ -67,12 +67,11 @@ class Batch:
                                   q_starts=self.starts, seqs=self.seqs, **kw)
 
 
-def attention64(b, window=0, scale=None, terms=1):
+def attention64(b, window=0, scale=None):
     """(result, bound) [tokens, heads, dim] in 64 bits.  bound: how far a result in the
     cache's type may be off, element by element:
       u |o|                      the result's rounding, u = eps / 2 of the type
-      (u + r) sum p |v| / sum p  u: the weights' rounding (u^terms where they are held in
-                                 so many terms of the type); r: the scores' error (dim + 2
+      (u + r) sum p |v| / sum p  u: the weights' rounding; r: the scores' error (dim + 2
                                  roundings of 2^-24 on scale |q|.|k|, in numerator and
                                  denominator), the sums over n keys and over parts
                                  (n + 64 roundings in each) and exp's 2^-20
@@ -99,7 +98,7 @@ def attention64(b, window=0, scale=None, terms=1):
             mag = (torch.where(see, q.abs() @ kk.abs().t(), 0.0).amax(1, keepdim=True) * scale)
             r = 2 * (b.dim + 2) * 2.0 ** -24 * mag + 2 * (n + 64) * 2.0 ** -24 + 2.0 ** -20
             out[at:at + m, h] = o
-            bound[at:at + m, h] = u * o.abs() + (u ** terms + r) * (p @ vv.abs() / total)
+            bound[at:at + m, h] = u * o.abs() + (u + r) * (p @ vv.abs() / total)
             if b.dtype == torch.float16:
                 bound[at:at + m, h] += n * 2.0 ** -25 * vv.abs().amax()
         at += m

@@ -789,10 +789,14 @@ def test_compaction_leaves_the_used_pages_in_front():
     ([5000, 3], [1, 1], 4, 2, 64, 16, BF), ([700, 33], [1, 1], 8, 4, 256, 16, BF),
     ([900, 64], [4, 2], 8, 2, 128, 64, BF), ([900, 5000], [2, 1], 32, 4, 64, 64, HF)])
 def test_few_rows_keep_the_weights(lens, news, heads, kv, dim, page, dtype):
-    """A decode step's weights are held in two terms of the cache's type: what is left of
-    their rounding is u^2."""
+    """A decode step's weights are held in two terms of the cache's type: of their rounding,
+    u sum p |v| in attention64()'s bound, u^2 sum p |v| is left."""
     b = Batch(lens, news, heads, kv, dim, page, dtype, seed=71)
-    want, bound = attention64(b, terms=2)
+    want, bound = attention64(b)
+    u = torch.finfo(dtype).eps / 2
+    dense, b.dense = b.dense, [(k, v.abs()) for k, v in b.dense]
+    bound -= (u - u * u) * attention64(b)[0]  # (its result with |v|: sum p |v| / sum p)
+    b.dense = dense
     got = b.call(nb, max_q=max(news)).double()
     over = (got - want).abs() - bound
     assert (over <= 1e-12).all(), f"{over.max().item():.3e} over the bound"
