@@ -477,7 +477,9 @@ int nq_llama_set_prefill_chunk(nq_llama_t dec, int64_t chunk);
  * decoder's own cache and position are not touched.  Row rows[i] of the batch
  * (device int32 [n_out]; negative: left out, its outputs are not meaningful)
  * yields logits [n_out][vocab] (fp32, optional) and next_tokens [n_out] (int32
- * argmax, optional).  max_q as in nq_paged_attention.  The pages for the new
+ * argmax, optional).  Every row's token is looked up, those of padding too: one
+ * outside of the vocabulary counts as 0 and raises bit 1 of the error word.
+ * max_q as in nq_paged_attention.  The pages for the new
  * tokens are the caller's to reserve.  workspace: nq_llama_forward_workspace_
  * size() bytes (max_keys = table_width * page_size), 256-byte aligned. */
 size_t nq_llama_forward_workspace_size(nq_llama_t dec, int64_t n_tokens, int64_t n_out, int64_t max_q,
